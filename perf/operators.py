@@ -188,7 +188,7 @@ def _shared_exponent(amax, mantissa):
     """The exponent of amax rounded to the element's mantissa bits, less the elements' largest exponent, 2."""
     m, e = torch.frexp(amax)   # amax = m 2^e, m in [0.5, 1)
     up = m >= 1 - 2.0 ** -(mantissa + 2)   # rounds to 1, the next power of two
-    return torch.where(amax > 0, (e - 1 + up.to(e.dtype) - 2).clamp_min(-127), -127)
+    return torch.where(amax > 0, (e - 1 + up.to(e.dtype) - 2).clamp_min(-121), -121)
 
 
 def _round_element(a, mantissa):
@@ -330,7 +330,7 @@ def _exact_mx(x, fmt):
     e = torch.floor(torch.log2(top.clamp_min(2.0 ** -140)))
     # log2 may be one off at powers of two
     e = e + (torch.exp2(e + 1) <= top).double() - (torch.exp2(e) > top).double() - 2
-    e = (e + (top >= limit * torch.exp2(e))).clamp_min(-127)
+    e = (e + (top >= limit * torch.exp2(e))).clamp_min(-121)
     a = (x / torch.exp2(e)).abs()
     hi = torch.searchsorted(grid, a).clamp_(1, len(grid) - 1)
     lo = hi - 1

@@ -32,12 +32,29 @@ extern "C" {
 #define MI_MOE_Q8_0 0
 #define MI_MOE_Q4_0 1
 #define MI_MOE_W4A16 2
+/* MXFP4 weights, MXFP6 activations (no reference counterpart): blocks of 32
+ * along K with one power-of-two scale, as the MX formats below. */
+#define MI_MOE_MXFP4 3
 
 /* dtype codes for activations and scales (and router logits, which may also
  * be MI_MOE_F32) */
 #define MI_MOE_F16 0
 #define MI_MOE_BF16 1
 #define MI_MOE_F32 2
+
+/* MX block formats of mi_moe_mx_quantize: 32 elements share an E8M0 scale byte
+ * s that stands for 2^(s-127) (255: the block is NaN).
+ * MI_MOE_MX_FP4: E2M1 elements (0, .5, 1, 1.5, 2, 3, 4, 6), 16 B a block,
+ *   element 2i in the low half of byte i.
+ * MI_MOE_MX_FP6: E2M3 elements (multiples of 1/8 to 2, 1/4 to 4, 1/2 to 7.5),
+ *   24 B a block, element i in bits 6i .. 6i+5 (little endian).
+ * The sign is the element's highest bit. */
+#define MI_MOE_MX_FP4 0
+#define MI_MOE_MX_FP6 1
+
+/* score functions of mi_moe_topk_scores */
+#define MI_MOE_SCORE_SOFTMAX 0
+#define MI_MOE_SCORE_SIGMOID 1
 
 typedef struct mi_moe_handle mi_moe_handle;
 
@@ -51,7 +68,7 @@ int mi_moe_version(void);
  * Replaces MoEInfer::MoEInfer (Int8-gemm/moe_infer.cpp:18-75) and the
  * TorchBind constructor MoEInfer(E,H,I,quant_type)
  * (Int8-gemm/nanovllm_ops.cpp:28-30,353).  Requires H%32==0, I%32==0
- * (W4A16: H%512==0, I%128==0).  Allocates nothing on the device until weights
+ * (W4A16: H%512==0, I%128==0; MXFP4: H%64==0, H and I at most 65536).  Allocates nothing on the device until weights
  * are stored; uses the current HIP device. */
 int mi_moe_create(int64_t num_experts, int64_t hidden, int64_t intermediate,
                   int quant_type, mi_moe_handle** out);
@@ -81,8 +98,10 @@ int mi_moe_store_quantized(mi_moe_handle* h, const void* gate_up_qs,
  * Replaces MoEInfer::quantize_and_store_expert (Int8-gemm/moe_infer.cpp:
  * 284-360; rule of quantize_weight_only, Int8-gemm/q8_gemm.cpp:197-260).
  * proj: 0 = gate_proj [I,H], 1 = up_proj [I,H], 2 = down_proj [H,I];
- * w_dtype: 0 fp16, 1 bf16, 2 fp32.  Q8_0 handles only (the reference rejects
- * Q4_0, Int8-gemm/nanovllm_ops.cpp:359-363).  Scales are stored as fp16. */
+ * w_dtype: 0 fp16, 1 bf16, 2 fp32.  Q8_0 handles (the reference rejects
+ * Q4_0, Int8-gemm/nanovllm_ops.cpp:359-363), whose scales are stored as fp16,
+ * and MXFP4 handles, which quantize as mi_moe_mx_quantize does (device
+ * sources 16-byte aligned). */
 int mi_moe_quantize_and_store_expert(mi_moe_handle* h, int64_t expert,
                                      int proj, const void* w, int w_dtype,
                                      int src_on_device, void* stream);
@@ -98,6 +117,15 @@ int mi_moe_store_awq(mi_moe_handle* h, const int32_t* w13_qweight,
                      const int32_t* w2_qweight, const int32_t* w2_qzeros,
                      const void* w2_scales, int64_t group, int scale_dtype,
                      int src_on_device, void* stream);
+
+/* MXFP4 weights -> device layout (no reference counterpart).
+ *   gate_up_codes [E,2I,H/2] (rows [0,I) gate, [I,2I) up), gate_up_scales [E,2I,H/32],
+ *   down_codes [E,H,I/2], down_scales [E,H,I/32], as mi_moe_mx_quantize writes
+ *   them.  Any scale byte is taken; 255 makes the block's products NaN.
+ *   Device codes are 16-byte aligned. */
+int mi_moe_store_mxfp4(mi_moe_handle* h, const uint8_t* gate_up_codes,
+                       const uint8_t* gate_up_scales, const uint8_t* down_codes,
+                       const uint8_t* down_scales, int src_on_device, void* stream);
 
 /* The fused MoE layer: y[t] = sum_k topk_w[t,k] * Expert_{ids[t,k]}(x[t]).
  * Replaces MoEInfer::ExecuteFn (Int8-gemm/moe_infer.h:51-61) /
@@ -116,7 +144,11 @@ int mi_moe_store_awq(mi_moe_handle* h, const int32_t* w13_qweight,
  * all.  Once a call on the handle has been captured, workspace that a later,
  * larger call outgrows is kept until mi_moe_destroy instead of being freed,
  * so captured graphs stay valid through eager calls of any size.  A graph
- * must not outlive its handle. */
+ * must not outlive its handle.
+ * MXFP4 handles quantize x and the intermediate silu(gate) * up to MXFP6
+ * blocks (mi_moe_mx_quantize's rounding) and sum exact products in fp32; they
+ * use the workspace at every size (reserve it before a capture).  A NaN or an
+ * infinity in x makes its token's y NaN. */
 int mi_moe_forward(mi_moe_handle* h, const void* x, void* y,
                    const float* topk_w, const int32_t* topk_ids, int64_t T,
                    int64_t K, int act_dtype, void* stream);
@@ -233,6 +265,61 @@ int mi_moe_topk_softmax(const void* logits, int logits_dtype, int64_t T,
  * (Int8-gemm/test/fused_moe_cpu.py:20-37) for the CPU dispatch key. */
 int mi_moe_cpu_topk_softmax(const float* logits, int64_t T, int64_t E, int64_t K,
                             int renormalize, int32_t* topk_ids, float* topk_w);
+
+/* Router with scores: logits [T,E] (fp16, bf16 or fp32, device) -> topk_ids
+ * [T,K] int32, topk_w [T,K] fp32 (device).  No reference counterpart.
+ *   s = sigmoid(logit) or the softmax over all E; c = s + bias (fp32 [E] on the
+ *   device, or null); the E experts are n_group groups of E / n_group
+ *   consecutive ones, a group's score is the sum of its group_top (1 or 2)
+ *   largest c; in the topk_group best groups the K largest c are picked, in
+ *   descending order (ties: the lower group, the lower expert).
+ *   topk_w = scale * s, with renormalize scale * s / (sum of the picks' s), 0
+ *   where that sum is 0.  The bias only decides the choice.
+ * Scores, choices and sums are in 64 bits; topk_w is rounded once.  An expert
+ * whose logit (or bias) is -infinity is masked: never picked, -infinity in its
+ * group's sum; where fewer than K experts are left the remaining ids are -1,
+ * which mi_moe_forward drops, with weight 0.  A token with a NaN score (a NaN
+ * logit or bias; an infinite logit under softmax) gets ids 0 .. K-1 and NaN
+ * weights.  E <= 512, n_group <= 64, K <= 64.  Stream-ordered, no workspace. */
+int mi_moe_topk_scores(const void* logits, int logits_dtype, int64_t T, int64_t E,
+                       int64_t K, const float* bias, int score, int64_t n_group,
+                       int64_t topk_group, int64_t group_top, int renormalize,
+                       float scale, int32_t* topk_ids, float* topk_w, void* stream);
+
+/* mi_moe_topk_scores on host memory and host cores: fp32 logits [T,E], bias
+ * [E] or null. */
+int mi_moe_cpu_topk_scores(const float* logits, int64_t T, int64_t E, int64_t K,
+                           const float* bias, int score, int64_t n_group,
+                           int64_t topk_group, int64_t group_top, int renormalize,
+                           float scale, int32_t* topk_ids, float* topk_w);
+
+/* mi_moe_topk_scores followed by mi_moe_forward on the same stream, E the
+ * handle's expert count; the picks go to topk_ids_out / topk_w_out when both
+ * are given, else to a buffer of the handle, as in mi_moe_forward_logits. */
+int mi_moe_forward_scores(mi_moe_handle* h, const void* x, void* y,
+                          const void* router_logits, int logits_dtype, int64_t T,
+                          int64_t K, const float* bias, int score, int64_t n_group,
+                          int64_t topk_group, int64_t group_top, int renormalize,
+                          float scale, int act_dtype, int32_t* topk_ids_out,
+                          float* topk_w_out, void* stream);
+
+/* MX block quantization: x, rows of cols values (fp16, bf16 or fp32) row_stride
+ * elements apart, device -> codes [rows][cols/32][16 or 24 B], scales
+ * [rows][cols/32].  The scale is 2^(e-2), e the exponent of the block's largest
+ * magnitude rounded to the element's mantissa, at least 2^-121, so that no
+ * element is off by more than half a step; elements round to nearest, ties to
+ * even.  A block that holds a NaN or an infinity gets scale 255 and zero codes.
+ * cols%32==0, rows * cols <= 2^40; x, its rows and codes 16-byte aligned.
+ * Stream-ordered, no workspace.  No reference counterpart. */
+int mi_moe_mx_quantize(const void* x, int dtype, int64_t rows, int64_t cols,
+                       int64_t row_stride, int format, uint8_t* codes,
+                       uint8_t* scales, void* stream);
+
+/* The values that codes and scales stand for, rounded once to dtype: out
+ * [rows, cols] fp16, bf16 or fp32, device, 16-byte aligned. */
+int mi_moe_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows,
+                         int64_t cols, int format, void* out, int dtype,
+                         void* stream);
 
 /* Router top-k + softmax followed by mi_moe_forward on the same stream:
  * router_logits [T,E] with E the handle's expert count.  The picks go to

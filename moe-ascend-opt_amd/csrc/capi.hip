@@ -48,6 +48,12 @@ hipError_t launch_qint_gemm(const QArgs&, int, int, int, hipStream_t);
 hipError_t launch_quant_route(const void*, int, int64_t, int64_t, int8_t*, float*, const int32_t*, int, int, int,
                               const RouteGlobal&, hipStream_t, int);
 hipError_t launch_topk_softmax(const void*, int, int, int, int, int, int32_t*, float*, hipStream_t);
+hipError_t launch_topk_scores(const void*, int, const float*, const ScoreArgs&, int32_t*, float*, hipStream_t);
+hipError_t launch_mx_sorted(const MxArgs&, int, int, hipStream_t, hipEvent_t);
+hipError_t launch_mx_quantize(const void*, int, int64_t, int, int64_t, int, unsigned char*, unsigned char*, hipStream_t);
+hipError_t launch_mx_dequantize(const unsigned char*, const unsigned char*, int64_t, int, void*, int, hipStream_t);
+hipError_t launch_mx_repack(const void*, const void*, int64_t, int, int, int, void*, void*, hipStream_t);
+hipError_t launch_mx_online(const void*, int, int64_t, int, int, int, void*, void*, hipStream_t);
 hipError_t launch_q_repack(int, const void*, const uint16_t*, void*, uint16_t*, int, int, int, int,
                            int, hipStream_t);
 hipError_t launch_q8_online_quant(const void*, int, int, int, int, int, int, void*, uint16_t*,
@@ -166,6 +172,12 @@ int check_handle(const mi_moe_handle* h) {
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
+// Bytes of the intermediate's row of one pair, and of a token's quantized hidden row.
+size_t act_row_bytes(const mi_moe_handle* h) {
+  return h->quant == MI_MOE_MXFP4 ? mx_row_bytes((int)h->I) : (size_t)h->I * 2;
+}
+size_t xq_row_bytes(const mi_moe_handle* h) { return h->quant == MI_MOE_MXFP4 ? mx_row_bytes((int)h->H) : (size_t)h->H; }
+
 int ensure_workspace(mi_moe_handle* h, int64_t T, int64_t n, hipStream_t st) {
   if (h->r_U.p == nullptr) {
     HIPCHK(h->r_counts.alloc((size_t)h->E * sizeof(int32_t)));
@@ -185,7 +197,7 @@ int ensure_workspace(mi_moe_handle* h, int64_t T, int64_t n, hipStream_t st) {
     for (DevBuf* b : {&h->act, &h->act_d, &h->eout, &h->r_tok, &h->r_scat, &h->r_tiles, &h->r_chunk, &h->xq, &h->xd})
       b->retire(h->retired);
   }
-  HIPCHK(h->act.alloc((size_t)capn * h->I * 2));
+  HIPCHK(h->act.alloc((size_t)capn * act_row_bytes(h)));
   HIPCHK(h->act_d.alloc((size_t)capn * (h->I / 32) * sizeof(float)));
   HIPCHK(h->eout.alloc((size_t)capn * h->H * sizeof(float)));
   HIPCHK(h->r_tok.alloc((size_t)capn * sizeof(int32_t)));
@@ -193,7 +205,7 @@ int ensure_workspace(mi_moe_handle* h, int64_t T, int64_t n, hipStream_t st) {
   HIPCHK(h->r_tiles.alloc((size_t)gemm_tiles_max(capn, (int)h->E) * 4 * sizeof(int32_t)));
   HIPCHK(h->r_chunk.alloc((size_t)route_chunks((int)capn) * h->E * sizeof(int32_t)));
   if (h->quant != MI_MOE_W4A16) {
-    HIPCHK(h->xq.alloc((size_t)capT * h->H));
+    HIPCHK(h->xq.alloc((size_t)capT * xq_row_bytes(h)));
     HIPCHK(h->xd.alloc((size_t)capT * (h->H / 32) * sizeof(float)));
   }
   h->cap_T = capT;
@@ -218,10 +230,10 @@ RouteGlobal route_view(mi_moe_handle* h) {
 // Device workspace of one forward call: the handle's grown buffers
 // (mi_moe_forward) or slices of the no-alloc scratch (mi_moe_forward_noalloc).
 struct Work {
-  void* act = nullptr;      // [n, I] act dtype (W4A16) or int8 (Q8_0 / Q4_0)
+  void* act = nullptr;      // [n, I] act dtype (W4A16) or int8 (Q8_0 / Q4_0), [n, mx_row_bytes(I)] (MXFP4)
   float* act_d = nullptr;   // [n, I/32] intermediate Q8_0 scales
   float* eout = nullptr;    // [n, H] per-pair outputs (paths with a separate combine)
-  int8_t* xq = nullptr;     // [T, H] Q8_0 activations (int8 grouped GEMMs)
+  int8_t* xq = nullptr;     // [T, H] Q8_0 activations (int8 grouped GEMMs), [T, mx_row_bytes(H)] (MXFP4)
   float* xd = nullptr;      // [T, H/32]
   unsigned long long* tact = nullptr; // tagged act units of the one-launch decode kernel
   RouteGlobal rg{};
@@ -286,11 +298,11 @@ size_t carve_work(unsigned char* base, const mi_moe_handle* h, int64_t T, int64_
   w.rg.scat = (int32_t*)take((size_t)n * 4);
   w.rg.tiles = (int32_t*)take((size_t)gemm_tiles_max(n, (int)E) * 16);
   w.rg.chunk = (int32_t*)take((size_t)route_chunks((int)n) * E * 4);
-  w.act = take((size_t)n * I * 2);
+  w.act = take((size_t)n * act_row_bytes(h));
   w.act_d = (float*)take((size_t)n * (I / 32) * 4);
   w.eout = need_eout ? (float*)take((size_t)n * H * 4) : nullptr;
   if (h->quant != MI_MOE_W4A16) {
-    w.xq = (int8_t*)take((size_t)T * H);
+    w.xq = (int8_t*)take((size_t)T * xq_row_bytes(h));
     w.xd = (float*)take((size_t)T * (H / 32) * 4);
   }
   return off;
@@ -446,6 +458,44 @@ int forward_q(mi_moe_handle* h, const void* x, void* y, const float* tw, const i
   return MI_MOE_OK;
 }
 
+int mx_alloc_weights(mi_moe_handle* h) {
+  const size_t E = (size_t)h->E, t13 = E * (h->I / 32) * mx_ktiles((int)h->H), t2 = E * (h->H / 64) * mx_ktiles((int)h->I);
+  HIPCHK(h->w13.alloc(t13 * kMxTileBytes));
+  HIPCHK(h->w13_s.alloc(t13 * kMxTileScaleBytes));
+  HIPCHK(h->w2.alloc(t2 * kMxTileBytes));
+  HIPCHK(h->w2_s.alloc(t2 * kMxTileScaleBytes));
+  // zeros stay where K is no multiple of 128, and in what has not been stored
+  for (DevBuf* b : {&h->w13, &h->w13_s, &h->w2, &h->w2_s}) HIPCHK(hipMemset(b->p, 0, b->bytes));
+  return MI_MOE_OK;
+}
+
+int forward_mx(mi_moe_handle* h, const void* x, void* y, const float* tw, const int32_t* ids, int64_t T, int64_t K,
+               int act, bool noalloc, hipStream_t st) {
+  const int64_t n = T * K;
+  Work w;
+  const int rc = get_work(h, T, n, true, noalloc, st, w);
+  if (rc) return rc;
+  MxArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.x = (const uint16_t*)x;
+  a.y = (uint16_t*)y;
+  a.tw = tw;
+  a.ids = ids;
+  a.T = (int)T; a.K = (int)K; a.E = (int)h->E; a.H = (int)h->H; a.I = (int)h->I; a.n = (int)n;
+  a.rg = w.rg;
+  a.w13 = (const unsigned char*)h->w13.p; a.w13_s = (const unsigned char*)h->w13_s.p;
+  a.w2 = (const unsigned char*)h->w2.p; a.w2_s = (const unsigned char*)h->w2_s.p;
+  a.xq = (unsigned char*)w.xq;
+  a.act = (unsigned char*)w.act;
+  a.eout = (int16_t*)w.eout;   // the fp32 rows' room holds both
+  a.eout_d = (float*)((unsigned char*)w.eout + (size_t)n * h->H * 2);
+  hipEvent_t mid = h->timing && !noalloc ? h->evmid : nullptr;
+  HIPCHK(launch_route_global(ids, (int)n, (int)K, (int)h->E, a.rg, st, 0, 0));
+  HIPCHK(launch_mx_sorted(a, act, (int)gemm_tiles_max(n, (int)h->E), st, mid));
+  if (!noalloc) h->mid_recorded = mid != nullptr;
+  return MI_MOE_OK;
+}
+
 // Argument checks shared by mi_moe_forward and mi_moe_forward_noalloc.
 int check_forward_args(mi_moe_handle* h, const void* x, void* y, const float* topk_w, const int32_t* topk_ids,
                        int64_t T, int64_t K, int act_dtype) {
@@ -477,7 +527,7 @@ int api_fail(int code, const char* msg) {
 
 int check_dims(int64_t E, int64_t H, int64_t I, int quant_type) {
   if (E <= 0 || H <= 0 || I <= 0) return fail(MI_MOE_EINVAL, "E, H, I must be positive");
-  if (quant_type < 0 || quant_type > 2) return fail(MI_MOE_EINVAL, "quant_type must be 0, 1 or 2");
+  if (quant_type < 0 || quant_type > 3) return fail(MI_MOE_EINVAL, "quant_type must be 0, 1, 2 or 3");
   if (H % 32 != 0) return fail(MI_MOE_EINVAL, "hidden_size must be multiple of 32");
   if (I % 32 != 0) return fail(MI_MOE_EINVAL, "intermediate_size must be multiple of 32");
   if (quant_type != MI_MOE_W4A16 && H % 64 != 0)
@@ -485,6 +535,10 @@ int check_dims(int64_t E, int64_t H, int64_t I, int quant_type) {
   if (quant_type == MI_MOE_W4A16 && (H % 512 != 0 || I % 128 != 0))
     return fail(MI_MOE_EINVAL, "W4A16 needs hidden_size %% 512 == 0 and intermediate_size %% 128 == 0");
   if (E > 512) return fail(MI_MOE_EUNSUPPORTED, "at most 512 experts");
+  if (quant_type == MI_MOE_MXFP4) {
+    if (H > 65536 || I > 65536) return fail(MI_MOE_EUNSUPPORTED, "MXFP4: at most 65536 hidden and intermediate columns");
+    return MI_MOE_OK;
+  }
   // one path must serve calls of every size: the W4A16 grouped GEMMs, or for
   // Q8_0 / Q4_0 the int8 grouped GEMMs or else the lane-per-row kernels at
   // the largest in-LDS routing
@@ -664,12 +718,35 @@ MI_API int mi_moe_store_quantized(mi_moe_handle* h, const void* gate_up_qs, cons
   return MI_MOE_OK;
 }
 
+MI_API int mi_moe_store_mxfp4(mi_moe_handle* h, const uint8_t* gate_up_codes, const uint8_t* gate_up_scales,
+                              const uint8_t* down_codes, const uint8_t* down_scales, int src_on_device, void* stream) {
+  int rc = check_handle(h);
+  if (rc) return rc;
+  if (h->quant != MI_MOE_MXFP4) return fail(MI_MOE_EINVAL, "store_mxfp4 needs an MXFP4 handle (quant_type 3)");
+  if (!gate_up_codes || !gate_up_scales || !down_codes || !down_scales) return fail(MI_MOE_EINVAL, "null weight pointer");
+  if (src_on_device && !(aligned16(gate_up_codes) && aligned16(down_codes)))
+    return fail(MI_MOE_EINVAL, "codes must be 16-byte aligned");
+  hipStream_t st = (hipStream_t)stream;
+  const int64_t E = h->E, H = h->H, I = h->I;
+  Staged a, b, c, d;
+  HIPCHK(a.stage(gate_up_codes, (size_t)E * 2 * I * (H / 2), src_on_device, st));
+  HIPCHK(b.stage(gate_up_scales, (size_t)E * 2 * I * (H / 32), src_on_device, st));
+  HIPCHK(c.stage(down_codes, (size_t)E * H * (I / 2), src_on_device, st));
+  HIPCHK(d.stage(down_scales, (size_t)E * H * (I / 32), src_on_device, st));
+  if (!h->w13.p) { rc = mx_alloc_weights(h); if (rc) return rc; }
+  HIPCHK(launch_mx_repack(a.ptr, b.ptr, E, 0, (int)H, (int)I, h->w13.p, h->w13_s.p, st));
+  HIPCHK(launch_mx_repack(c.ptr, d.ptr, E, 1, (int)H, (int)I, h->w2.p, h->w2_s.p, st));
+  HIPCHK(hipStreamSynchronize(st));
+  h->loaded = true;
+  return MI_MOE_OK;
+}
+
 MI_API int mi_moe_quantize_and_store_expert(mi_moe_handle* h, int64_t expert, int proj,
                                             const void* w, int w_dtype, int src_on_device,
                                             void* stream) {
   int rc = check_handle(h);
   if (rc) return rc;
-  if (h->quant != MI_MOE_Q8_0)
+  if (h->quant != MI_MOE_Q8_0 && h->quant != MI_MOE_MXFP4)
     return fail(MI_MOE_EINVAL, "Q4_0 does not support online quantization. "
                                "Use store_quantized_repack() with pre-quantized weights.");
   if (expert < 0 || expert >= h->E) return fail(MI_MOE_EINVAL, "expert index out of range");
@@ -681,6 +758,15 @@ MI_API int mi_moe_quantize_and_store_expert(mi_moe_handle* h, int64_t expert, in
   const size_t esz = w_dtype == 2 ? 4 : 2;
   Staged a;
   HIPCHK(a.stage(w, (size_t)N * K * esz, src_on_device, st));
+  if (h->quant == MI_MOE_MXFP4) {
+    if (!aligned16(a.ptr)) return fail(MI_MOE_EINVAL, "weight must be 16-byte aligned");
+    if (!h->w13.p) { rc = mx_alloc_weights(h); if (rc) return rc; }
+    HIPCHK(launch_mx_online(a.ptr, w_dtype, expert, proj, (int)h->H, (int)h->I, (proj == 2 ? h->w2 : h->w13).p,
+                            (proj == 2 ? h->w2_s : h->w13_s).p, st));
+    HIPCHK(hipStreamSynchronize(st));
+    h->loaded = true;
+    return MI_MOE_OK;
+  }
   if (!h->w13.p) { rc = q_alloc_weights(h); if (rc) return rc; }
   void* wdst = proj == 2 ? h->w2.p : h->w13.p;
   uint16_t* ddst = (uint16_t*)(proj == 2 ? h->w2_s.p : h->w13_s.p);
@@ -744,7 +830,8 @@ MI_API int mi_moe_forward(mi_moe_handle* h, const void* x, void* y, const float*
   if (hipStreamIsCapturing(st, &cs) == hipSuccess && cs != hipStreamCaptureStatusNone) h->captured = true;
   if (h->timing) HIPCHK(hipEventRecord(h->ev0, st));
   h->mid_recorded = false;
-  if (h->quant == MI_MOE_W4A16) rc = forward_w4a16(h, x, y, topk_w, topk_ids, T, K, act_dtype, false, st);
+  if (h->quant == MI_MOE_MXFP4) rc = forward_mx(h, x, y, topk_w, topk_ids, T, K, act_dtype, false, st);
+  else if (h->quant == MI_MOE_W4A16) rc = forward_w4a16(h, x, y, topk_w, topk_ids, T, K, act_dtype, false, st);
   else rc = forward_q(h, x, y, topk_w, topk_ids, T, K, act_dtype, false, st);
   if (rc) return rc;
   if (h->timing) {
@@ -760,6 +847,7 @@ MI_API int mi_moe_forward_noalloc(mi_moe_handle* h, const void* x, void* y, cons
   int rc = check_forward_args(h, x, y, topk_w, topk_ids, T, K, act_dtype);
   if (rc || T == 0) return rc;
   hipStream_t st = (hipStream_t)stream;
+  if (h->quant == MI_MOE_MXFP4) return forward_mx(h, x, y, topk_w, topk_ids, T, K, act_dtype, true, st);
   if (h->quant == MI_MOE_W4A16) return forward_w4a16(h, x, y, topk_w, topk_ids, T, K, act_dtype, true, st);
   return forward_q(h, x, y, topk_w, topk_ids, T, K, act_dtype, true, st);
 }
@@ -778,6 +866,106 @@ MI_API int mi_moe_topk_softmax(const void* logits, int logits_dtype, int64_t T, 
   return MI_MOE_OK;
 }
 
+namespace {
+
+// Where a call with a router puts its picks: the caller's arrays, or the
+// handle's buffer (grown on demand; growth synchronizes the stream).
+int picks_buffer(mi_moe_handle* h, int64_t need, hipStream_t st, int32_t*& ids, float*& w) {
+  if (ids) return MI_MOE_OK;
+  if (need > h->cap_r) {
+    int64_t cap = h->cap_r ? h->cap_r : 1024;
+    while (cap < need) cap *= 2;
+    HIPCHK(hipStreamSynchronize(st));   // the buffers may be in use by queued work
+    if (h->captured) {                  // or by captured graphs
+      h->r_rids.retire(h->retired);
+      h->r_rw.retire(h->retired);
+    }
+    HIPCHK(h->r_rids.alloc((size_t)cap * sizeof(int32_t)));
+    HIPCHK(h->r_rw.alloc((size_t)cap * sizeof(float)));
+    h->cap_r = cap;
+  }
+  ids = (int32_t*)h->r_rids.p;
+  w = (float*)h->r_rw.p;
+  return MI_MOE_OK;
+}
+
+}  // namespace
+
+MI_API int mi_moe_topk_scores(const void* logits, int logits_dtype, int64_t T, int64_t E, int64_t K, const float* bias,
+                              int score, int64_t n_group, int64_t topk_group, int64_t group_top, int renormalize,
+                              float scale, int32_t* topk_ids, float* topk_w, void* stream) {
+  if (logits_dtype != MI_MOE_F16 && logits_dtype != MI_MOE_BF16 && logits_dtype != MI_MOE_F32)
+    return fail(MI_MOE_EINVAL, "logits dtype must be fp16, bf16 or fp32");
+  const char* bad = score_args_error(T, E, K, score, n_group, topk_group, group_top);
+  if (bad) return fail(MI_MOE_EINVAL, "%s", bad);
+  if (T == 0) return MI_MOE_OK;
+  if (!logits || !topk_ids || !topk_w) return fail(MI_MOE_EINVAL, "null pointer");
+  const ScoreArgs a = {(int)T, (int)E, (int)K, score == MI_MOE_SCORE_SIGMOID, (int)n_group, (int)topk_group, (int)group_top,
+                       renormalize != 0, (double)scale};
+  HIPCHK(launch_topk_scores(logits, logits_dtype, bias, a, topk_ids, topk_w, (hipStream_t)stream));
+  return MI_MOE_OK;
+}
+
+MI_API int mi_moe_forward_scores(mi_moe_handle* h, const void* x, void* y, const void* router_logits, int logits_dtype,
+                                 int64_t T, int64_t K, const float* bias, int score, int64_t n_group, int64_t topk_group,
+                                 int64_t group_top, int renormalize, float scale, int act_dtype, int32_t* topk_ids_out,
+                                 float* topk_w_out, void* stream) {
+  int rc = check_handle(h);
+  if (rc) return rc;
+  const char* bad = score_args_error(T, h->E, K, score, n_group, topk_group, group_top);
+  if (bad) return fail(MI_MOE_EINVAL, "%s", bad);
+  if (T == 0) return MI_MOE_OK;
+  if ((topk_ids_out == nullptr) != (topk_w_out == nullptr))
+    return fail(MI_MOE_EINVAL, "topk_ids_out and topk_w_out must both be given or both be null");
+  if (!router_logits) return fail(MI_MOE_EINVAL, "null router logits");
+  int32_t* ids = topk_ids_out;
+  float* w = topk_w_out;
+  rc = picks_buffer(h, T * K, (hipStream_t)stream, ids, w);
+  if (rc) return rc;
+  rc = check_forward_args(h, x, y, w, ids, T, K, act_dtype);   // nothing is launched for a call that cannot end
+  if (rc) return rc;
+  rc = mi_moe_topk_scores(router_logits, logits_dtype, T, h->E, K, bias, score, n_group, topk_group, group_top,
+                          renormalize, scale, ids, w, stream);
+  if (rc) return rc;
+  return mi_moe_forward(h, x, y, w, ids, T, K, act_dtype, stream);
+}
+
+namespace {
+int check_mx(int64_t rows, int64_t cols, int fmt, int dtype) {
+  if (fmt != MI_MOE_MX_FP4 && fmt != MI_MOE_MX_FP6) return fail(MI_MOE_EINVAL, "format must be 0 (MXFP4) or 1 (MXFP6)");
+  if (dtype != MI_MOE_F16 && dtype != MI_MOE_BF16 && dtype != MI_MOE_F32)
+    return fail(MI_MOE_EINVAL, "values must be fp16, bf16 or fp32");
+  if (rows < 0 || cols <= 0 || cols % 32) return fail(MI_MOE_EINVAL, "cols=%lld must be a positive multiple of 32", (long long)cols);
+  if (cols > ((int64_t)1 << 30) || rows > ((int64_t)1 << 40) / cols) return fail(MI_MOE_EINVAL, "more than 2^40 values");
+  return MI_MOE_OK;
+}
+}  // namespace
+
+MI_API int mi_moe_mx_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, int format,
+                              uint8_t* codes, uint8_t* scales, void* stream) {
+  const int rc = check_mx(rows, cols, format, dtype);
+  if (rc) return rc;
+  if (rows == 0) return MI_MOE_OK;
+  if (!x || !codes || !scales) return fail(MI_MOE_EINVAL, "null pointer");
+  const int64_t per16 = dtype == MI_MOE_F32 ? 4 : 8;
+  if (row_stride < cols || row_stride % per16 || row_stride > ((int64_t)1 << 40) / rows)
+    return fail(MI_MOE_EINVAL, "row_stride=%lld must be at least cols and whole 16-byte pieces", (long long)row_stride);
+  if (!aligned16(x) || !aligned16(codes)) return fail(MI_MOE_EINVAL, "x and codes must be 16-byte aligned");
+  HIPCHK(launch_mx_quantize(x, dtype, rows, (int)cols, row_stride, format, codes, scales, (hipStream_t)stream));
+  return MI_MOE_OK;
+}
+
+MI_API int mi_moe_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, int format,
+                                void* out, int dtype, void* stream) {
+  const int rc = check_mx(rows, cols, format, dtype);
+  if (rc) return rc;
+  if (rows == 0) return MI_MOE_OK;
+  if (!out || !codes || !scales) return fail(MI_MOE_EINVAL, "null pointer");
+  if (!aligned16(out) || !aligned16(codes)) return fail(MI_MOE_EINVAL, "codes and out must be 16-byte aligned");
+  HIPCHK(launch_mx_dequantize(codes, scales, rows * (cols / 32), format, out, dtype, (hipStream_t)stream));
+  return MI_MOE_OK;
+}
+
 MI_API int mi_moe_forward_logits(mi_moe_handle* h, const void* x, void* y, const void* router_logits,
                                  int logits_dtype, int64_t T, int64_t K, int renormalize, int act_dtype,
                                  int32_t* topk_ids_out, float* topk_w_out, void* stream) {
@@ -787,26 +975,10 @@ MI_API int mi_moe_forward_logits(mi_moe_handle* h, const void* x, void* y, const
   if (T == 0) return MI_MOE_OK;
   if ((topk_ids_out == nullptr) != (topk_w_out == nullptr))
     return fail(MI_MOE_EINVAL, "topk_ids_out and topk_w_out must both be given or both be null");
-  hipStream_t st = (hipStream_t)stream;
   int32_t* ids = topk_ids_out;
   float* w = topk_w_out;
-  if (!ids) {
-    const int64_t need = T * K;
-    if (need > h->cap_r) {
-      int64_t cap = h->cap_r ? h->cap_r : 1024;
-      while (cap < need) cap *= 2;
-      HIPCHK(hipStreamSynchronize(st));   // the buffers may be in use by queued work
-      if (h->captured) {                  // or by captured graphs
-        h->r_rids.retire(h->retired);
-        h->r_rw.retire(h->retired);
-      }
-      HIPCHK(h->r_rids.alloc((size_t)cap * sizeof(int32_t)));
-      HIPCHK(h->r_rw.alloc((size_t)cap * sizeof(float)));
-      h->cap_r = cap;
-    }
-    ids = (int32_t*)h->r_rids.p;
-    w = (float*)h->r_rw.p;
-  }
+  rc = picks_buffer(h, T * K, (hipStream_t)stream, ids, w);
+  if (rc) return rc;
   rc = mi_moe_topk_softmax(router_logits, logits_dtype, T, h->E, K, renormalize, ids, w, stream);
   if (rc) return rc;
   return mi_moe_forward(h, x, y, w, ids, T, K, act_dtype, stream);

@@ -9,6 +9,7 @@
 
 #include "cpu_moe.hpp"
 #include "mi_moe.h"
+#include "score_args.hpp"
 
 #define MI_API extern "C" __attribute__((visibility("default")))
 
@@ -171,6 +172,18 @@ MI_API int mi_moe_cpu_topk_softmax(const float* logits, int64_t T, int64_t E, in
   if (T == 0) return MI_MOE_OK;
   if (!logits || !topk_ids || !topk_w) return fail(MI_MOE_EINVAL, "null pointer");
   mimoe_cpu::topk_softmax(logits, T, E, K, renormalize, topk_ids, topk_w);
+  return MI_MOE_OK;
+}
+
+MI_API int mi_moe_cpu_topk_scores(const float* logits, int64_t T, int64_t E, int64_t K, const float* bias, int score,
+                                  int64_t n_group, int64_t topk_group, int64_t group_top, int renormalize, float scale,
+                                  int32_t* topk_ids, float* topk_w) {
+  const char* bad = mimoe::score_args_error(T, E, K, score, n_group, topk_group, group_top);
+  if (bad) return fail(MI_MOE_EINVAL, bad);
+  if (T == 0) return MI_MOE_OK;
+  if (!logits || !topk_ids || !topk_w) return fail(MI_MOE_EINVAL, "null pointer");
+  mimoe_cpu::topk_scores(logits, T, E, K, bias, score == MI_MOE_SCORE_SIGMOID, n_group, topk_group, group_top,
+                         renormalize != 0, scale, topk_ids, topk_w);
   return MI_MOE_OK;
 }
 

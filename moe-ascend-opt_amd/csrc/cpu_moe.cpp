@@ -385,6 +385,75 @@ void topk_softmax(const float* logits, int64_t T, int64_t E, int64_t K, int reno
   }
 }
 
+void topk_scores(const float* logits, int64_t T, int64_t E, int64_t K, const float* bias, bool sigmoid, int64_t n_group,
+                 int64_t topk_group, int64_t group_top, bool renorm, float scale, int32_t* ids, float* w) {
+  const double ninf = -INFINITY;
+  double s[512], c[512];
+  const int64_t gs = E / n_group;
+  for (int64_t t = 0; t < T; ++t) {
+    const float* l = logits + t * E;
+    int32_t* oi = ids + t * K;
+    float* ow = w + t * K;
+    if (sigmoid) {
+      for (int64_t e = 0; e < E; ++e) s[e] = 1.0 / (1.0 + std::exp(-(double)l[e]));
+    } else {
+      float m = -INFINITY;
+      for (int64_t e = 0; e < E; ++e) m = l[e] > m ? l[e] : m;
+      if (m == -INFINITY) m = 0.0f;   // every expert masked
+      double sum = 0.0;
+      for (int64_t e = 0; e < E; ++e) {
+        s[e] = std::exp((double)l[e] - (double)m);
+        sum += s[e];
+      }
+      for (int64_t e = 0; e < E; ++e) s[e] = sum == 0.0 ? 0.0 : s[e] / sum;
+    }
+    bool nan = false;
+    for (int64_t e = 0; e < E; ++e) {
+      c[e] = bias ? s[e] + (double)bias[e] : s[e];
+      nan |= c[e] != c[e];
+      if (l[e] == -INFINITY) c[e] = ninf;
+    }
+    if (nan) {
+      for (int64_t k = 0; k < K; ++k) {
+        oi[k] = (int32_t)k;
+        ow[k] = NAN;
+      }
+      continue;
+    }
+    if (topk_group < n_group) {
+      double g[64];
+      for (int64_t i = 0; i < n_group; ++i) {
+        double b1 = ninf, b2 = ninf;
+        for (int64_t e = i * gs; e < (i + 1) * gs; ++e) {
+          if (c[e] > b1) { b2 = b1; b1 = c[e]; }
+          else if (c[e] > b2) b2 = c[e];
+        }
+        g[i] = group_top == 1 ? b1 : b2 == ninf ? ninf : b1 + b2;
+      }
+      for (int64_t i = 0; i < n_group; ++i) {
+        int64_t ahead = 0;
+        for (int64_t o = 0; o < n_group; ++o) ahead += g[o] > g[i] || (g[o] == g[i] && o < i);
+        if (ahead >= topk_group)
+          for (int64_t e = i * gs; e < (i + 1) * gs; ++e) c[e] = ninf;
+      }
+    }
+    double picked[64], sum = 0.0;
+    for (int64_t k = 0; k < K; ++k) {
+      int64_t best = -1;
+      for (int64_t e = 0; e < E; ++e)
+        if (c[e] > (best < 0 ? ninf : c[best])) best = e;
+      oi[k] = (int32_t)best;
+      picked[k] = best < 0 ? 0.0 : s[best];
+      sum += picked[k];
+      if (best >= 0) c[best] = ninf;
+    }
+    for (int64_t k = 0; k < K; ++k) {
+      const double v = renorm ? (sum > 0.0 ? picked[k] / sum : 0.0) : picked[k];
+      ow[k] = (float)(v * (double)scale);
+    }
+  }
+}
+
 void quant_hidden_row(bool simd, const uint16_t* x, int64_t n, int dt, int8_t* q, uint8_t* qb, float* d,
                       int32_t* s) {
   if (simd) quant_hidden_avx2(x, n, dt, q, qb, d, s);

@@ -27,6 +27,12 @@ float half_to_f32(uint16_t v, int dt);
 void topk_softmax(const float* logits, int64_t T, int64_t E, int64_t K, int renormalize, int32_t* ids,
                   float* w);
 
+// Score router (mi_moe_topk_scores on host memory): softmax or sigmoid scores
+// in 64 bits, selection bias, groups, top-k, renormalized and scaled weights.
+// Arguments as score_args_error allows them (E <= 512).
+void topk_scores(const float* logits, int64_t T, int64_t E, int64_t K, const float* bias, bool sigmoid, int64_t n_group,
+                 int64_t topk_group, int64_t group_top, bool renorm, float scale, int32_t* ids, float* w);
+
 // Q8_0 of n values (n % 32 == 0) into q, q ^ 0x80, block scales d and int32
 // block sums s: a hidden row of fp16 / bf16 bits (Stage A), or SiLU(gate) * up
 // (the intermediate).  simd picks the AVX2 + FMA form (same bytes and scales).

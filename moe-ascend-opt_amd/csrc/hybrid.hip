@@ -329,6 +329,7 @@ MI_API int mi_moe_hybrid_create(int64_t E, int64_t H, int64_t I, int quant_type,
   *out = nullptr;
   if (!host_mask) return hfail(MI_MOE_EINVAL, "host_mask is null");
   if (num_threads < 0 || num_threads > 256) return hfail(MI_MOE_EINVAL, "num_threads must be in [0, 256]");
+  if (quant_type == MI_MOE_MXFP4) return hfail(MI_MOE_EUNSUPPORTED, "the host executor has no MXFP4 experts");
   int rc = check_dims(E, H, I, quant_type);   // the device handle's shape rules
   if (rc) return rc;
   mi_moe_hybrid* hh = new (std::nothrow) mi_moe_hybrid();

@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "score_args.hpp"
+
 namespace mimoe {
 
 // Routing done inside the fused kernel (LDS) up to this many (t,k) pairs;
@@ -240,5 +242,47 @@ static_assert(q_part_unit0(kTagActMaxI) + (size_t)kQFusedMaxPairs * 2 * kTagActM
 __host__ __device__ inline size_t q_fused_down_lds_bytes(int I) {
   return (size_t)kQFusedWaves * (I + (I / 32) * 8 + 64 * 4 + 16 * 4 + 8);
 }
+
+// ---------------------------------------------------------------- score router (router.hip)
+struct ScoreArgs {
+  int T, E, K;
+  int sigmoid;                 // 1 sigmoid, 0 softmax scores
+  int n_group, topk_group, group_top;
+  int renorm;
+  double scale;
+};
+
+// ---------------------------------------------------------------- MXFP4 layer (mx.hip)
+// Element formats of the MX blocks (mx_device.hpp): the wire codes of
+// mi_moe_mx_quantize.
+constexpr int kMxFp4 = 0, kMxFp6 = 1;
+__host__ __device__ constexpr int mx_block_bytes(int fmt) { return fmt == kMxFp4 ? 16 : 24; }
+
+// K runs in tiles of 128 (4 blocks); rows whose length is no multiple end in
+// blocks of zeros.  Weights are stored in units of 64 rows, four 16-row
+// tiles: a gate_up unit is a slice of 32 rows of I (tiles gate 0-15, gate
+// 16-31, up 0-15, up 16-31), a down unit 64 rows of H.
+__host__ __device__ constexpr int mx_ktiles(int K) { return (K + 127) >> 7; }
+constexpr int kMxTileBytes = 4096;        // codes of one unit's k tile: [4 tiles][64 lanes][16 B]
+constexpr int kMxTileScaleBytes = 256;    // its scales: [64 lanes][4 tiles]
+constexpr int kMxPacketBytes = 32;        // an activation block: 24 B of codes, its scale byte
+__host__ __device__ constexpr size_t mx_row_bytes(int K) { return (size_t)mx_ktiles(K) * 4 * kMxPacketBytes; }
+
+struct MxArgs {
+  const uint16_t* x;       // [T,H] act dtype bits
+  uint16_t* y;             // [T,H]
+  const float* tw;         // [T,K]
+  const int32_t* ids;      // [T,K]
+  int T, K, E, H, I, n;
+  RouteGlobal rg;
+  const unsigned char* w13;     // [E][I/32 units][ktiles(H)][kMxTileBytes]
+  const unsigned char* w13_s;   // [E][I/32][ktiles(H)][kMxTileScaleBytes]
+  const unsigned char* w2;      // [E][H/64 units][ktiles(I)][...]
+  const unsigned char* w2_s;
+  unsigned char* xq;       // [T][mx_row_bytes(H)] quantized hidden rows
+  unsigned char* act;      // [n][mx_row_bytes(I)] quantized intermediate, row = sorted position
+  int16_t* eout;           // [n][H] expert outputs, row = pair, 16-bit integers
+  float* eout_d;           // [n][H/64] their scales
+};
 
 }  // namespace mimoe

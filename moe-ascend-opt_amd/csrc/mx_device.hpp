@@ -1,0 +1,140 @@
+// mx_device.hpp -- microscaled (MX) block formats on gfx950: 32 consecutive
+// elements share one power-of-two scale, an E8M0 byte s that stands for
+// 2^(s-127) (s = 255: NaN).
+//
+//   MXFP4: E2M1 elements {0, .5, 1, 1.5, 2, 3, 4, 6} and their negatives, 16 B a block
+//   MXFP6: E2M3 elements, multiples of 1/8 up to 2, of 1/4 up to 4, of 1/2 up to 7.5, 24 B a block
+//
+// Both element types end at 2^2 * (2 - 2^-M).  The shared exponent is that of
+// the block's largest magnitude rounded to the element's mantissa, less 2, so
+// that the largest element never saturates and no element is off by more than
+// half a step.  (An exponent taken before the rounding saturates magnitudes
+// in [7, 8) to 6, a whole step of E2M1.)  Elements round to nearest, ties to
+// the even mantissa.
+#pragma once
+#include "mi_moe_device.hpp"
+#include "mi_moe_internal.hpp"
+
+namespace mimoe {
+
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+typedef unsigned int u32x6_t __attribute__((ext_vector_type(6)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x32_t __attribute__((ext_vector_type(32)));
+typedef _Float16 f16x32_t __attribute__((ext_vector_type(32)));
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+
+// The E8M0 byte of a block from the bits of its largest magnitude (fp32,
+// sign cleared; NaN above infinity above all numbers).  Adding half a
+// mantissa step carries into the exponent iff the magnitude rounds up to the
+// next power of two.  The smallest scale is 2^-121: a subnormal fp32 element
+// is then below half the smallest step, so no result hangs on how subnormals
+// are treated.
+constexpr int kMxMinScale = 6;
+template <int FMT>
+__device__ __forceinline__ int mx_scale_byte(uint32_t amax_bits) {
+  if (amax_bits >= 0x7f800000u) return 255;
+  constexpr uint32_t half = FMT == kMxFp4 ? 0x00200000u : 0x00080000u;
+  const int e = (int)((amax_bits + half) >> 23) - 2;
+  return e < kMxMinScale ? kMxMinScale : e;
+}
+// the scale as a float (for a NaN block: 1, its codes are not used)
+__device__ __forceinline__ float mx_scale_f32(int s) { return __uint_as_float((uint32_t)(s == 255 ? 127 : s) << 23); }
+
+// Largest magnitude of 32 16-bit values in 16 words, as fp32 bits.  Their
+// bit patterns order like the magnitudes (NaN on top), so this is a maximum
+// of unsigned halves.
+template <int DT>
+__device__ __forceinline__ uint32_t mx_amax16(const uint32_t (&w)[16]) {
+  u16x2_t m = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, w[i] & 0x7fff7fffu));
+  const uint32_t a = m.x > m.y ? m.x : m.y;
+  if constexpr (DT == 1) return a << 16;
+  return __float_as_uint(f16_to_f32(a));
+}
+
+// 32 16-bit values -> E2M3 codes (bit 6 i.. of the block holds element i).
+template <int DT>
+__device__ __forceinline__ u32x6_t mx_fp6_codes16(const uint32_t (&w)[16], int s) {
+  typedef unsigned int u32x16_t __attribute__((ext_vector_type(16)));
+  u32x16_t v;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = s == 255 ? 0u : w[i];
+  if constexpr (DT == 1) return __builtin_amdgcn_cvt_scalef32_pk32_fp6_bf16(__builtin_bit_cast(bf16x32_t, v), mx_scale_f32(s));
+  return __builtin_amdgcn_cvt_scalef32_pk32_fp6_f16(__builtin_bit_cast(f16x32_t, v), mx_scale_f32(s));
+}
+
+__device__ __forceinline__ uint32_t mx_amax32(const float (&v)[32]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
+    m = a > m ? a : m;
+  }
+  return m;
+}
+// 32 fp32 values -> E2M3 codes.  The conversion takes the even and the odd
+// elements as two vectors.
+__device__ __forceinline__ u32x6_t mx_fp6_codes32(const float (&v)[32], int s) {
+  f32x16_t a, b;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    a[i] = s == 255 ? 0.0f : v[2 * i];
+    b[i] = s == 255 ? 0.0f : v[2 * i + 1];
+  }
+  return __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, mx_scale_f32(s));
+}
+// 32 fp32 values -> E2M1 codes, element 2 i in the low half of byte i.
+__device__ __forceinline__ u32x4_t mx_fp4_codes32(const float (&v)[32], int s) {
+  const float sc = mx_scale_f32(s);
+  u32x4_t o;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    uint32_t c = 0;
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * w], v[8 * w + 1], sc, 0);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * w + 2], v[8 * w + 3], sc, 1);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * w + 4], v[8 * w + 5], sc, 2);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * w + 6], v[8 * w + 7], sc, 3);
+    o[w] = s == 255 ? 0u : c;
+  }
+  return o;
+}
+
+// Two adjacent elements of row data of type DT (0 fp16, 1 bf16, 2 fp32) as floats.
+template <int DT>
+__device__ __forceinline__ void mx_unpack16(const uint32_t (&w)[16], float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    v[2 * i] = to_f32<DT>(w[i]);
+    v[2 * i + 1] = to_f32<DT>(w[i] >> 16);
+  }
+}
+
+// An activation block as the matrix instructions take it: 24 B of E2M3 codes,
+// the scale byte in the seventh word, so that two 16-byte LDS reads fetch a
+// lane's operand with its scale.
+struct MxPacket {
+  u32x4_t lo, hi;
+};
+__device__ __forceinline__ MxPacket mx_packet(const u32x6_t& c, int s) {
+  return MxPacket{u32x4_t{c[0], c[1], c[2], c[3]}, u32x4_t{c[4], c[5], (uint32_t)s, 0u}};
+}
+__device__ __forceinline__ i32x8_t mx_operand(const u32x4_t& lo, const u32x4_t& hi) {
+  return i32x8_t{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+}
+
+// D += W (16 rows x 128, E2M1) * X (128 x 16 columns, E2M3), fp32.  Lane
+// 16 q + r holds block q of row r of W and of column r of X, and rows
+// 4 q .. 4 q + 3 of D's column r.  T: the byte of ws that holds W's scale.
+// The instruction adds its products in groups of 8, in fixed point with 13
+// bits below the group's largest: products of one E2M3 and one E2M1 block
+// are multiples of 2^-4 below 2^6, so the groups are exact (E4M3
+// activations spread further and lose bits: 4e-6 of the sum on Gaussian data).
+template <int T>
+__device__ __forceinline__ f32x4_t mx_mfma(const u32x4_t& w, uint32_t ws, const u32x4_t& lo, const u32x4_t& hi, const f32x4_t& d) {
+  const i32x8_t a = {(int)w.x, (int)w.y, (int)w.z, (int)w.w, 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, mx_operand(lo, hi), d, 4, 2, T, (int)ws, 0, (int)hi.z);
+}
+
+}  // namespace mimoe

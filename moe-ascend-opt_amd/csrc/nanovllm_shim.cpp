@@ -5,14 +5,18 @@
 // plus the build-defined W4A16 loader store_awq_repack, the out variant
 // moe_forward_out, and the router step the reference runs in its Python
 // harness (make_topk_from_logits_cpu, Int8-gemm/test/fused_moe_cpu.py:20-37)
-// as moe_topk_softmax / moe_forward_logits.  Only this file sees torch types; it calls the C ABI of
+// as moe_topk_softmax / moe_forward_logits, the score router as moe_topk_scores /
+// moe_forward_scores, and the MX formats: store_mxfp4_repack, mx_quantize,
+// mx_dequantize.  Only this file sees torch types; it calls the C ABI of
 // include/mi_moe.h: HIP tensors run the device kernels on the current HIP stream; CPU tensors run the
 // host engine (the reference's CPU algorithm for Q8_0 / Q4_0; every expert on the host executor for
 // W4A16), which needs weights stored from host tensors (kept by default when no HIP device is present,
 // or with MIMOE_HOST_WEIGHTS=1; never with MIMOE_HOST_WEIGHTS=0).
+#include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/custom_class.h>
 #include <tuple>
+#include <optional>
 #include <vector>
 #include <torch/library.h>
 #include <ATen/ATen.h>
@@ -77,14 +81,16 @@ struct MoEInferHandle : torch::CustomClassHolder {
   bool last_cpu = false;           // the last forward ran on the host
   double last_cpu_ms = -1.0;
 
-  // Int8-gemm/nanovllm_ops.cpp:28-30 (quant_type: 0 Q8_0, 1 Q4_0; 2 W4A16)
+  // Int8-gemm/nanovllm_ops.cpp:28-30 (quant_type: 0 Q8_0, 1 Q4_0; 2 W4A16, 3 MXFP4)
   MoEInferHandle(int64_t E_, int64_t H_, int64_t I_, int64_t qt) : E(E_), H(H_), I(I_), quant_type(qt) {
-    TORCH_CHECK(qt >= 0 && qt <= 2, "quant_type must be 0 (Q8_0), 1 (Q4_0) or 2 (W4A16)");
+    TORCH_CHECK(qt >= 0 && qt <= 3, "quant_type must be 0 (Q8_0), 1 (Q4_0), 2 (W4A16) or 3 (MXFP4)");
     const bool dev = hip_device_present();
+    TORCH_CHECK(dev || qt != 3, "MoEInfer: MXFP4 layers need a HIP device");
     if (dev) check_status(mi_moe_create(E, H, I, (int)qt, &h), "MoEInfer");
     const char* kh = getenv("MIMOE_HOST_WEIGHTS");
     keep_host = kh ? atoi(kh) != 0 : !dev;
-    if (!dev) TORCH_CHECK(keep_host, "MoEInfer: no HIP device and MIMOE_HOST_WEIGHTS=0: nowhere to keep the weights");
+    if (qt == 3) keep_host = false;   // the host engines have no MXFP4
+    else if (!dev) TORCH_CHECK(keep_host, "MoEInfer: no HIP device and MIMOE_HOST_WEIGHTS=0: nowhere to keep the weights");
   }
   ~MoEInferHandle() override {
     if (h) mi_moe_destroy(h);
@@ -92,7 +98,7 @@ struct MoEInferHandle : torch::CustomClassHolder {
     if (hcpu) mi_moe_hybrid_destroy(hcpu);
   }
   std::string get_quant_type() const {
-    return quant_type == 1 ? "Q4_0" : (quant_type == 2 ? "W4A16" : "Q8_0");
+    return quant_type == 1 ? "Q4_0" : quant_type == 2 ? "W4A16" : quant_type == 3 ? "MXFP4" : "Q8_0";
   }
   int64_t info(int which) const { return which == 0 ? E : (which == 1 ? H : I); }
   mi_moe_handle* dev() const {
@@ -167,6 +173,7 @@ void forward_into(const at::Tensor& hidden, const at::Tensor& topk_ids, const at
 void forward_into_cpu(const at::Tensor& hidden, const at::Tensor& topk_ids, const at::Tensor& topk_w,
                       const c10::intrusive_ptr<MoEInferHandle>& moe, at::Tensor& out) {
   check_forward_tensors(hidden, topk_ids, topk_w, moe, out);
+  TORCH_CHECK(moe->quant_type != 3, "moe_forward (CPU): MXFP4 layers run on HIP tensors only");
   at::Tensor x = contig(hidden), ids = contig(topk_ids), w = contig(topk_w);
   const int64_t T = x.size(0), K = ids.size(1);
   if (moe->quant_type == 2) {
@@ -287,6 +294,157 @@ at::Tensor moe_forward_logits_cpu(const at::Tensor& hidden, const at::Tensor& ro
   return moe_forward_cpu(hidden, std::get<0>(picks), std::get<1>(picks), moe);
 }
 
+// Score router: arguments as mi_moe_topk_scores, score "softmax" or "sigmoid".
+int score_code(c10::string_view s) {
+  TORCH_CHECK(s == "softmax" || s == "sigmoid", "score must be 'softmax' or 'sigmoid', got '", s, "'");
+  return s == "sigmoid" ? MI_MOE_SCORE_SIGMOID : MI_MOE_SCORE_SOFTMAX;
+}
+
+// The selection bias as fp32 [E] beside the logits (an undefined tensor: none).
+at::Tensor score_bias(const std::optional<at::Tensor>& bias, const at::Tensor& logits) {
+  if (!bias.has_value() || !bias->defined()) return at::Tensor();
+  TORCH_CHECK(bias->dim() == 1 && bias->size(0) == logits.size(1) && bias->scalar_type() == at::kFloat,
+              "bias must be a float32 [E] tensor");
+  TORCH_CHECK(bias->device() == logits.device(), "bias and logits must be on one device");
+  return contig(*bias);
+}
+
+void check_scores(const at::Tensor& logits, int64_t top_k) {
+  TORCH_CHECK(logits.dim() == 2, "router logits must be [T,E]");
+  TORCH_CHECK(top_k >= 1 && top_k <= 64, "top_k=", top_k, " must be in [1, 64]");
+}
+
+std::tuple<at::Tensor, at::Tensor> moe_topk_scores_hip(const at::Tensor& logits, int64_t top_k,
+                                                       const std::optional<at::Tensor>& bias, c10::string_view score,
+                                                       int64_t n_group, int64_t topk_group, int64_t group_top,
+                                                       bool renormalize, double scale) {
+  check_scores(logits, top_k);
+  c10::hip::HIPGuard guard(logits.get_device());
+  at::Tensor x = contig(logits), b = score_bias(bias, logits);
+  const int64_t T = x.size(0), E = x.size(1);
+  at::Tensor ids = at::empty({T, top_k}, x.options().dtype(at::kInt));
+  at::Tensor w = at::empty({T, top_k}, x.options().dtype(at::kFloat));
+  check_status(mi_moe_topk_scores(x.data_ptr(), logits_code(x), T, E, top_k, b.defined() ? b.data_ptr<float>() : nullptr,
+                                  score_code(score), n_group, topk_group, group_top, renormalize ? 1 : 0, (float)scale,
+                                  ids.data_ptr<int32_t>(), w.data_ptr<float>(), stream_of(x)),
+               "moe_topk_scores");
+  return {ids, w};
+}
+
+std::tuple<at::Tensor, at::Tensor> moe_topk_scores_cpu(const at::Tensor& logits, int64_t top_k,
+                                                       const std::optional<at::Tensor>& bias, c10::string_view score,
+                                                       int64_t n_group, int64_t topk_group, int64_t group_top,
+                                                       bool renormalize, double scale) {
+  check_scores(logits, top_k);
+  logits_code(logits);
+  at::Tensor x = contig(logits).to(at::kFloat), b = score_bias(bias, logits);
+  const int64_t T = x.size(0), E = x.size(1);
+  at::Tensor ids = at::empty({T, top_k}, x.options().dtype(at::kInt));
+  at::Tensor w = at::empty({T, top_k}, x.options().dtype(at::kFloat));
+  check_status(mi_moe_cpu_topk_scores(x.data_ptr<float>(), T, E, top_k, b.defined() ? b.data_ptr<float>() : nullptr,
+                                      score_code(score), n_group, topk_group, group_top, renormalize ? 1 : 0, (float)scale,
+                                      ids.data_ptr<int32_t>(), w.data_ptr<float>()),
+               "moe_topk_scores");
+  return {ids, w};
+}
+
+at::Tensor moe_forward_scores_hip(const at::Tensor& hidden, const at::Tensor& router_logits, int64_t top_k,
+                                  const std::optional<at::Tensor>& bias, c10::string_view score, int64_t n_group,
+                                  int64_t topk_group, int64_t group_top, bool renormalize, double scale,
+                                  const c10::intrusive_ptr<MoEInferHandle>& moe) {
+  check_scores(router_logits, top_k);
+  TORCH_CHECK(hidden.is_cuda() && router_logits.is_cuda() && hidden.device() == router_logits.device(),
+              "moe_forward_scores: hidden and router_logits must be HIP tensors on one device");
+  TORCH_CHECK(hidden.dim() == 2 && router_logits.size(0) == hidden.size(0),
+              "moe_forward_scores: expected hidden [T,H], router_logits [T,E]");
+  TORCH_CHECK(router_logits.size(1) == moe->info(0), "router_logits has ", router_logits.size(1),
+              " experts, handle has ", moe->info(0));
+  TORCH_CHECK(hidden.size(1) == moe->info(1), "hidden size ", hidden.size(1), " != handle H ", moe->info(1));
+  c10::hip::HIPGuard guard(hidden.get_device());
+  at::Tensor x = contig(hidden), g = contig(router_logits), b = score_bias(bias, router_logits);
+  at::Tensor out = at::empty_like(x);
+  check_status(mi_moe_forward_scores(moe->dev(), x.data_ptr(), out.data_ptr(), g.data_ptr(), logits_code(g), x.size(0),
+                                     top_k, b.defined() ? b.data_ptr<float>() : nullptr, score_code(score), n_group,
+                                     topk_group, group_top, renormalize ? 1 : 0, (float)scale, act_code(x), nullptr, nullptr,
+                                     stream_of(x)),
+               "moe_forward_scores");
+  moe->last_cpu = false;
+  return out;
+}
+
+at::Tensor moe_forward_scores_cpu(const at::Tensor& hidden, const at::Tensor& router_logits, int64_t top_k,
+                                  const std::optional<at::Tensor>& bias, c10::string_view score, int64_t n_group,
+                                  int64_t topk_group, int64_t group_top, bool renormalize, double scale,
+                                  const c10::intrusive_ptr<MoEInferHandle>& moe) {
+  check_scores(router_logits, top_k);
+  TORCH_CHECK(hidden.dim() == 2 && router_logits.size(0) == hidden.size(0),
+              "moe_forward_scores: expected hidden [T,H], router_logits [T,E]");
+  TORCH_CHECK(router_logits.size(1) == moe->info(0), "router_logits has ", router_logits.size(1),
+              " experts, handle has ", moe->info(0));
+  auto picks = moe_topk_scores_cpu(router_logits, top_k, bias, score, n_group, topk_group, group_top, renormalize, scale);
+  return moe_forward_cpu(hidden, std::get<0>(picks), std::get<1>(picks), moe);
+}
+
+// MX block formats: "mxfp4" (E2M1) or "mxfp6" (E2M3), see mi_moe_mx_quantize.
+int mx_format(c10::string_view f) {
+  TORCH_CHECK(f == "mxfp4" || f == "mxfp6", "format must be 'mxfp4' or 'mxfp6', got '", f, "'");
+  return f == "mxfp4" ? MI_MOE_MX_FP4 : MI_MOE_MX_FP6;
+}
+int64_t mx_block(int fmt) { return fmt == MI_MOE_MX_FP4 ? 16 : 24; }
+
+int mx_value_code(at::ScalarType t) {
+  if (t == at::kFloat) return MI_MOE_F32;
+  if (t == at::kBFloat16) return MI_MOE_BF16;
+  TORCH_CHECK(t == at::kHalf, "values must be float32, bfloat16 or float16, got ", t);
+  return MI_MOE_F16;
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
+// x [..., C] -> codes uint8 [..., C/2] (mxfp4) or [..., C/32*24] (mxfp6),
+// scales uint8 [..., C/32].  A 2-D view whose rows are whole 16-byte pieces
+// apart is read in place, any other layout is copied first.
+std::tuple<at::Tensor, at::Tensor> mx_quantize_hip(const at::Tensor& x, c10::string_view format) {
+  const int fmt = mx_format(format), dt = mx_value_code(x.scalar_type());
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0 && x.size(-1) % 32 == 0,
+              "mx_quantize: the last dimension must be a positive multiple of 32");
+  c10::hip::HIPGuard guard(x.get_device());
+  const int64_t C = x.size(-1), rows = x.numel() / C, per16 = dt == MI_MOE_F32 ? 4 : 8;
+  const bool in_place = aligned16(x.data_ptr()) &&
+                        (x.is_contiguous() || (x.dim() == 2 && x.stride(1) == 1 && x.stride(0) >= C && x.stride(0) % per16 == 0));
+  at::Tensor v = in_place ? x : x.contiguous();
+  if (!aligned16(v.data_ptr())) v = v.clone(at::MemoryFormat::Contiguous);
+  std::vector<int64_t> cs = x.sizes().vec(), ss = cs;
+  cs.back() = C / 32 * mx_block(fmt);
+  ss.back() = C / 32;
+  at::Tensor codes = at::empty(cs, x.options().dtype(at::kByte)), scales = at::empty(ss, x.options().dtype(at::kByte));
+  check_status(mi_moe_mx_quantize(v.data_ptr(), dt, rows, C, v.is_contiguous() ? C : v.stride(0), fmt,
+                                  codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), stream_of(x)),
+               "mx_quantize");
+  return {codes, scales};
+}
+
+at::Tensor mx_dequantize_hip(const at::Tensor& codes, const at::Tensor& scales, c10::string_view format, at::ScalarType dtype) {
+  const int fmt = mx_format(format), dt = mx_value_code(dtype);
+  TORCH_CHECK(codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte, "codes and scales must be uint8");
+  TORCH_CHECK(scales.is_cuda() && scales.device() == codes.device(), "codes and scales must be on one device");
+  TORCH_CHECK(codes.dim() >= 1 && codes.dim() == scales.dim() && scales.size(-1) > 0 &&
+                  codes.size(-1) == scales.size(-1) * mx_block(fmt) &&
+                  codes.sizes().slice(0, codes.dim() - 1) == scales.sizes().slice(0, scales.dim() - 1),
+              "mx_dequantize: codes and scales do not belong together in format ", format);
+  c10::hip::HIPGuard guard(codes.get_device());
+  at::Tensor c = contig(codes), s = contig(scales);
+  if (!aligned16(c.data_ptr())) c = c.clone(at::MemoryFormat::Contiguous);
+  std::vector<int64_t> os = s.sizes().vec();
+  const int64_t C = 32 * os.back(), rows = s.numel() / os.back();
+  os.back() = C;
+  at::Tensor out = at::empty(os, c.options().dtype(dtype));
+  check_status(mi_moe_mx_dequantize(c.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), rows, C, fmt, out.data_ptr(), dt,
+                                    stream_of(c)),
+               "mx_dequantize");
+  return out;
+}
+
 int scale_code(const at::Tensor& d) {
   if (d.scalar_type() == at::kBFloat16) return MI_MOE_BF16;
   TORCH_CHECK(d.scalar_type() == at::kHalf, "scales must be float16 or bfloat16");
@@ -345,7 +503,7 @@ TORCH_LIBRARY_FRAGMENT(nanovllm, m) {
       .def("quantize_and_store_expert",
            [](const c10::intrusive_ptr<MoEInferHandle>& self, int64_t expert_idx,
               const std::string& proj_name, const at::Tensor& w) {
-             TORCH_CHECK(self->quant_type == 0,
+             TORCH_CHECK(self->quant_type == 0 || self->quant_type == 3,
                          "Q4_0 does not support online quantization. "
                          "Use store_quantized_repack() with pre-quantized weights.");
              int proj = proj_name == "gate_proj" ? 0 : proj_name == "up_proj" ? 1
@@ -362,6 +520,7 @@ TORCH_LIBRARY_FRAGMENT(nanovllm, m) {
              } else {
                TORCH_CHECK(wc.size(0) == H && wc.size(1) == I, "down weight must be [H,I]");
              }
+             if (wc.is_cuda() && !aligned16(wc.data_ptr())) wc = wc.clone(at::MemoryFormat::Contiguous);
              if (self->h)
                check_status(mi_moe_quantize_and_store_expert(self->h, expert_idx, proj, wc.data_ptr(),
                                                              wd, wc.is_cuda() ? 1 : 0, stream_of(wc)),
@@ -450,6 +609,30 @@ TORCH_LIBRARY_FRAGMENT(nanovllm, m) {
                                                     f.data_ptr(), g, scale_code(c), 0, nullptr),
                             "store_awq_repack (host)");
            })
+      // MXFP4 weights as mx_quantize writes them; see mi_moe_store_mxfp4
+      .def("store_mxfp4_repack",
+           [](const c10::intrusive_ptr<MoEInferHandle>& self, const at::Tensor& gate_up_codes,
+              const at::Tensor& gate_up_scales, const at::Tensor& down_codes, const at::Tensor& down_scales) {
+             TORCH_CHECK(self->quant_type == 3, "store_mxfp4_repack needs an MXFP4 handle (quant_type 3)");
+             const int64_t E = self->info(0), H = self->info(1), I = self->info(2);
+             TORCH_CHECK(gate_up_codes.sizes() == at::IntArrayRef({E, 2 * I, H / 2}) &&
+                             gate_up_scales.sizes() == at::IntArrayRef({E, 2 * I, H / 32}),
+                         "gate_up tensors must be [E,2I,H/2] and [E,2I,H/32]");
+             TORCH_CHECK(down_codes.sizes() == at::IntArrayRef({E, H, I / 2}) &&
+                             down_scales.sizes() == at::IntArrayRef({E, H, I / 32}),
+                         "down tensors must be [E,H,I/2] and [E,H,I/32]");
+             at::Tensor t[4] = {contig(gate_up_codes), contig(gate_up_scales), contig(down_codes), contig(down_scales)};
+             const bool dev = t[0].is_cuda();
+             for (auto& v : t) {
+               TORCH_CHECK(v.scalar_type() == at::kByte, "codes and scales must be uint8");
+               TORCH_CHECK(v.device() == t[0].device(), "all weight tensors must be on one device");
+               if (dev && !aligned16(v.data_ptr())) v = v.clone(at::MemoryFormat::Contiguous);
+             }
+             check_status(mi_moe_store_mxfp4(self->dev(), t[0].data_ptr<uint8_t>(), t[1].data_ptr<uint8_t>(),
+                                             t[2].data_ptr<uint8_t>(), t[3].data_ptr<uint8_t>(), dev ? 1 : 0,
+                                             stream_of(t[0])),
+                          "store_mxfp4_repack");
+           })
       .def("get_last_run_time_ms",
            [](const c10::intrusive_ptr<MoEInferHandle>& self) {
              if (self->last_cpu || !self->h) return self->last_cpu_ms;
@@ -492,6 +675,13 @@ TORCH_LIBRARY_FRAGMENT(nanovllm, m) {
         "Tensor(a!) out) -> ()");
   m.def("moe_forward_logits(Tensor hidden, Tensor router_logits, int top_k, bool renormalize, "
         "__torch__.torch.classes.nanovllm.MoEInfer moe) -> Tensor");
+  m.def("moe_topk_scores(Tensor logits, int top_k, Tensor? bias=None, str score='softmax', int n_group=1, "
+        "int topk_group=1, int group_top=2, bool renormalize=True, float scale=1.0) -> (Tensor, Tensor)");
+  m.def("moe_forward_scores(Tensor hidden, Tensor router_logits, int top_k, Tensor? bias, str score, int n_group, "
+        "int topk_group, int group_top, bool renormalize, float scale, "
+        "__torch__.torch.classes.nanovllm.MoEInfer moe) -> Tensor");
+  m.def("mx_quantize(Tensor x, str format) -> (Tensor, Tensor)");
+  m.def("mx_dequantize(Tensor codes, Tensor scales, str format, ScalarType dtype) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(nanovllm, CUDA, m) {
@@ -499,6 +689,10 @@ TORCH_LIBRARY_IMPL(nanovllm, CUDA, m) {
   m.impl("moe_forward_out", &moe_forward_out_hip);
   m.impl("moe_topk_softmax", &moe_topk_softmax_hip);
   m.impl("moe_forward_logits", &moe_forward_logits_hip);
+  m.impl("moe_topk_scores", &moe_topk_scores_hip);
+  m.impl("moe_forward_scores", &moe_forward_scores_hip);
+  m.impl("mx_quantize", &mx_quantize_hip);
+  m.impl("mx_dequantize", &mx_dequantize_hip);
   m.impl("moe_forward_npu_stream", &moe_forward_hip);
   m.impl("moe_forward_npu_graph_out", &moe_forward_graph_out_impl);
 }
@@ -508,6 +702,8 @@ TORCH_LIBRARY_IMPL(nanovllm, CPU, m) {
   m.impl("moe_forward_out", &moe_forward_out_cpu);
   m.impl("moe_topk_softmax", &moe_topk_softmax_cpu);
   m.impl("moe_forward_logits", &moe_forward_logits_cpu);
+  m.impl("moe_topk_scores", &moe_topk_scores_cpu);
+  m.impl("moe_forward_scores", &moe_forward_scores_cpu);
   m.impl("moe_forward_npu_stream", &moe_forward_cpu);
   m.impl("moe_forward_npu_graph_out", &moe_forward_graph_out_impl);
 }

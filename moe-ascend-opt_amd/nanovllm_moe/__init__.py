@@ -3,10 +3,17 @@
 
 After ``nanovllm_moe.load()`` (or ``import nanovllm_ext``):
 
-    h = torch.classes.nanovllm.MoEInfer(E, H, I, quant_type)   # 0 Q8_0, 1 Q4_0, 2 W4A16
+    h = torch.classes.nanovllm.MoEInfer(E, H, I, quant_type)   # 0 Q8_0, 1 Q4_0, 2 W4A16, 3 MXFP4
     h.store_quantized_repack(gate_up_qs, gate_up_d, down_qs, down_d)   # Q8_0 / Q4_0
     h.store_awq_repack(w13_q, w13_z, w13_s, w2_q, w2_z, w2_s, 128)      # W4A16
+    h.store_mxfp4_repack(gate_up_codes, gate_up_scales, down_codes, down_scales)   # MXFP4
     y = torch.ops.nanovllm.moe_forward(hidden, topk_ids, topk_w, h)     # HIP tensors
+
+Routers: ``moe_topk_softmax(logits, k)``, and ``moe_topk_scores(logits, k, bias,
+score, n_group, topk_group, group_top, renormalize, scale)`` (softmax or
+sigmoid scores, a bias for the choice alone, expert groups); ``moe_forward_logits``
+and ``moe_forward_scores`` run them in front of the layer.  MX block formats:
+``mx_quantize(x, "mxfp4" | "mxfp6")`` and ``mx_dequantize``.
 
 The op dispatches on the tensors' device, like the reference's registration
 (Int8-gemm/nanovllm_ops.cpp:410-412).  HIP tensors run the hand-written HIP
@@ -14,7 +21,8 @@ kernels of ``libmimoe.so`` on the current stream; a missing library raises,
 and the HIP key never falls back to the host.  CPU tensors run the reference
 CPU algorithm on host cores (the CPU key: Q8_0 / Q4_0 on the host engine,
 W4A16 on the host executor), from the host copy of the weights a handle keeps
-when no HIP device is present or MIMOE_HOST_WEIGHTS=1.
+when no HIP device is present or MIMOE_HOST_WEIGHTS=1.  MXFP4 layers and the MX
+ops run on HIP tensors only.
 """
 from __future__ import annotations
 
@@ -28,8 +36,10 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG_DIR, "libmimoe.so")
 SHIM_PATH = os.path.join(PKG_DIR, "libnanovllm_shim.so")
 
-Q8_0, Q4_0, W4A16 = 0, 1, 2
-F16, BF16, F32 = 0, 1, 2   # dtype codes (F32: router logits only)
+Q8_0, Q4_0, W4A16, MXFP4 = 0, 1, 2, 3
+F16, BF16, F32 = 0, 1, 2   # dtype codes (F32: router logits and MX values only)
+MX_FP4, MX_FP6 = 0, 1
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 
 _loaded = False
 _capi = None
@@ -47,6 +57,8 @@ C_SYMBOLS = (
     "mi_moe_hybrid_get_stats", "mi_moe_cpu_create", "mi_moe_cpu_destroy", "mi_moe_cpu_store_quantized",
     "mi_moe_cpu_quantize_and_store_expert", "mi_moe_cpu_forward", "mi_moe_cpu_get_info", "mi_moe_cpu_set_isa",
     "mi_moe_cpu_isa_name", "mi_moe_cpu_topk_softmax", "mi_moe_cpu_create_numa",
+    "mi_moe_store_mxfp4", "mi_moe_topk_scores", "mi_moe_cpu_topk_scores", "mi_moe_forward_scores",
+    "mi_moe_mx_quantize", "mi_moe_mx_dequantize",
 )
 
 
@@ -117,6 +129,13 @@ def capi():
     L.mi_moe_cpu_set_isa.argtypes = [P, I]
     L.mi_moe_cpu_topk_softmax.argtypes = [P, I64, I64, I64, I, P, P]
     L.mi_moe_cpu_create_numa.argtypes = [I64, I64, I64, I, I, I, ctypes.POINTER(P)]
+    F32c = ctypes.c_float
+    L.mi_moe_store_mxfp4.argtypes = [P, P, P, P, P, I, P]
+    L.mi_moe_topk_scores.argtypes = [P, I, I64, I64, I64, P, I, I64, I64, I64, I, F32c, P, P, P]
+    L.mi_moe_cpu_topk_scores.argtypes = [P, I64, I64, I64, P, I, I64, I64, I64, I, F32c, P, P]
+    L.mi_moe_forward_scores.argtypes = [P, P, P, P, I, I64, I64, P, I, I64, I64, I64, I, F32c, I, P, P, P]
+    L.mi_moe_mx_quantize.argtypes = [P, I, I64, I64, I64, I, P, P, P]
+    L.mi_moe_mx_dequantize.argtypes = [P, P, I64, I64, I, P, I, P]
     L.mi_moe_cpu_isa_name.restype = ctypes.c_char_p
     L.mi_moe_cpu_isa_name.argtypes = [I]
     for name in C_SYMBOLS:

@@ -23,7 +23,8 @@ SHIM = os.path.join(PKG_DIR, "libnanovllm_shim.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 
-HIP_SOURCES = ["capi.hip", "common_kernels.hip", "w4a16.hip", "w4a16_fused.hip", "qint.hip", "hybrid.hip"]
+HIP_SOURCES = ["capi.hip", "common_kernels.hip", "w4a16.hip", "w4a16_fused.hip", "qint.hip", "hybrid.hip", "mx.hip",
+               "router.hip"]
 # Host-only C++ (no HIP): the host executor of the hybrid offload path and the
 # CPU engine of the Q8_0 / Q4_0 layer (its C ABI too).  Inner loops are
 # compiled per instruction set (target attributes) and picked at run time;
@@ -45,6 +46,8 @@ NO_PK_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 FILE_FLAGS = {"qint.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-amdgpu-kernarg-preload-count=16"],
               "w4a16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-amdgpu-kernarg-preload-count=16"],
               "w4a16_fused.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-amdgpu-kernarg-preload-count=16"],
+              "mx.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-amdgpu-kernarg-preload-count=16"],
+              "router.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
               "common_kernels.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"]}
 
 

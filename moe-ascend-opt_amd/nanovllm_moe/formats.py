@@ -16,6 +16,12 @@ Formats (all per expert, stacked on a leading E axis):
   ``w2_qzeros`` [E,I/g,H/8], ``w2_scales`` [E,I/g,H].  Output columns are packed
   8 per int32 with nibble slot s holding column ``8j + AWQ_ORDER[s]``.
   Dequantized weight: ``W[n,k] = (q[k,n] - z[k//g,n]) * s[k//g,n]``.
+* MX (microscaled blocks; MXFP4 weights) -- 32 consecutive elements share a
+  power-of-two scale, an E8M0 byte ``s`` for ``2**(s-127)`` (255: NaN).
+  ``mxfp4``: E2M1 codes, uint8 [...,C/2], element 2i in the low half of byte i;
+  ``mxfp6``: E2M3 codes, uint8 [...,C/32*24], element i of a block in its bits
+  6i..6i+5; scales uint8 [...,C/32].  A handle takes ``mxfp4`` of gate||up
+  [E,2I,H] and down [E,H,I].
 
 All producers are plain torch and run on any device.
 """
@@ -129,6 +135,63 @@ def q4_0_random(shape_rows, K: int, generator=None, device="cpu", scale_dtype=to
     return _to_i32_wrap(words), d
 
 
+_MX = {"mxfp4": (1, 4), "mxfp6": (3, 6)}   # mantissa bits, bits of an element
+
+
+def _mx_elements(fmt: str, device) -> torch.Tensor:
+    """The values of a format's codes 0 .. 2^bits - 1."""
+    m, bits = _MX[fmt]
+    c = torch.arange(2 ** (bits - 1), device=device)
+    e, f = c >> m, (c & (2 ** m - 1)).to(torch.float32) / 2 ** m
+    v = torch.where(e == 0, f, (1 + f) * torch.exp2((e - 1).to(torch.float32)))
+    return torch.cat([v, -v])
+
+
+def mx_quantize(x: torch.Tensor, fmt: str):
+    """[..., C] -> (codes, scales).  The scale's exponent is that of the block's
+    largest magnitude rounded to the element's mantissa, less 2, at least -121;
+    elements round to nearest, ties to even; a block with a NaN or an infinity
+    gets scale 255 and zero codes."""
+    m, bits = _MX[fmt]
+    *lead, C = x.shape
+    assert C % 32 == 0
+    b = x.to(torch.float32).reshape(*lead, C // 32, 32)
+    amax = b.abs().amax(dim=-1)
+    bad = ~torch.isfinite(b).all(dim=-1)
+    amax = torch.where(bad, torch.ones_like(amax), amax)
+    s = ((amax.view(torch.int32) + (1 << (21 - 2 * (m == 3)))) >> 23) - 2   # biased; half a step carries
+    s = s.clamp_min(6)
+    v = torch.ldexp(torch.where(bad.unsqueeze(-1), torch.zeros_like(b), b), (127 - s).unsqueeze(-1))
+    a = v.abs()
+    # the code of a magnitude: its exponent (0 below 2: one scale for codes of exponent 0 and 1) and mantissa
+    ex = (a >= 2).to(torch.int32) + (a >= 4).to(torch.int32)
+    code = torch.round(torch.ldexp(a, m - ex)).to(torch.int32) + (ex << m)
+    code = torch.where(bad.unsqueeze(-1), torch.zeros_like(code), code | (torch.signbit(v).to(torch.int32) << (bits - 1)))
+    if bits == 4:
+        p = code.reshape(*lead, C // 2, 2)
+        packed = p[..., 0] | (p[..., 1] << 4)
+    else:
+        p = code.reshape(*lead, C // 4, 4)
+        w = p[..., 0] | (p[..., 1] << 6) | (p[..., 2] << 12) | (p[..., 3] << 18)
+        packed = torch.stack([w & 255, (w >> 8) & 255, w >> 16], dim=-1).reshape(*lead, C // 4 * 3)
+    return packed.to(torch.uint8), torch.where(bad, torch.full_like(s, 255), s).to(torch.uint8)
+
+
+def mx_dequant(codes: torch.Tensor, scales: torch.Tensor, fmt: str) -> torch.Tensor:
+    """Codes and scales -> fp32 values [..., C]."""
+    *lead, nb = scales.shape
+    c = codes.to(torch.int64)
+    if _MX[fmt][1] == 4:
+        i = torch.stack([c & 15, c >> 4], dim=-1)
+    else:
+        t = c.reshape(*lead, nb * 8, 3)
+        w = t[..., 0] | (t[..., 1] << 8) | (t[..., 2] << 16)
+        i = torch.stack([(w >> k) & 63 for k in (0, 6, 12, 18)], dim=-1)
+    v = _mx_elements(fmt, codes.device)[i].reshape(*lead, nb, 32)
+    s = scales.to(torch.int32).unsqueeze(-1)
+    return torch.where(s == 255, torch.full_like(v, float("nan")), torch.ldexp(v, s - 127)).reshape(*lead, nb * 32)
+
+
 def q8_0_dequant(qs: torch.Tensor, d: torch.Tensor) -> torch.Tensor:
     """Q8_0 wire [..., K] int8 + d [..., K/32] -> fp32 [..., K]."""
     return (qs.to(torch.float32).reshape(*qs.shape[:-1], -1, 32)
@@ -147,5 +210,7 @@ def bytes_per_expert(quant: int, H: int, I: int, group: int = 128) -> int:
         return n + n // 32 * 2
     if quant == 1:      # Q4_0: 4-bit + fp16 d per 32
         return n // 2 + n // 32 * 2
+    if quant == 3:      # MXFP4: 4-bit + a scale byte per 32
+        return n // 2 + n // 32
     # W4A16: 4-bit + 2-byte scale + 4-bit zero per group
     return n // 2 + n // group * 2 + n // group // 2

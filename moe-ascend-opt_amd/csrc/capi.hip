@@ -50,6 +50,7 @@ hipError_t launch_quant_route(const void*, int, int64_t, int64_t, int8_t*, float
 hipError_t launch_topk_softmax(const void*, int, int, int, int, int, int32_t*, float*, hipStream_t);
 hipError_t launch_topk_scores(const void*, int, const float*, const ScoreArgs&, int32_t*, float*, hipStream_t);
 hipError_t launch_mx_sorted(const MxArgs&, int, int, hipStream_t, hipEvent_t);
+hipError_t launch_mx_decode(const MxArgs&, int, hipStream_t, hipEvent_t);
 hipError_t launch_mx_quantize(const void*, int, int64_t, int, int64_t, int, unsigned char*, unsigned char*, hipStream_t);
 hipError_t launch_mx_dequantize(const unsigned char*, const unsigned char*, int64_t, int, void*, int, hipStream_t);
 hipError_t launch_mx_repack(const void*, const void*, int64_t, int, int, int, void*, void*, hipStream_t);
@@ -472,8 +473,9 @@ int mx_alloc_weights(mi_moe_handle* h) {
 int forward_mx(mi_moe_handle* h, const void* x, void* y, const float* tw, const int32_t* ids, int64_t T, int64_t K,
                int act, bool noalloc, hipStream_t st) {
   const int64_t n = T * K;
+  const bool decode = mx_decode_ok(n, K), fused = mx_decode_fused(n, K, (int)h->I);
   Work w;
-  const int rc = get_work(h, T, n, true, noalloc, st, w);
+  const int rc = get_work(h, T, n, !decode, noalloc, st, w);
   if (rc) return rc;
   MxArgs a;
   std::memset(&a, 0, sizeof(a));
@@ -489,7 +491,13 @@ int forward_mx(mi_moe_handle* h, const void* x, void* y, const float* tw, const 
   a.act = (unsigned char*)w.act;
   a.eout = (int16_t*)w.eout;   // the fp32 rows' room holds both
   a.eout_d = (float*)((unsigned char*)w.eout + (size_t)n * h->H * 2);
-  hipEvent_t mid = h->timing && !noalloc ? h->evmid : nullptr;
+  a.tact = w.tact;
+  hipEvent_t mid = h->timing && !noalloc && !fused ? h->evmid : nullptr;
+  if (decode) {
+    HIPCHK(launch_mx_decode(a, act, st, mid));
+    if (!noalloc) h->mid_recorded = mid != nullptr;
+    return MI_MOE_OK;
+  }
   HIPCHK(launch_route_global(ids, (int)n, (int)K, (int)h->E, a.rg, st, 0, 0));
   HIPCHK(launch_mx_sorted(a, act, (int)gemm_tiles_max(n, (int)h->E), st, mid));
   if (!noalloc) h->mid_recorded = mid != nullptr;

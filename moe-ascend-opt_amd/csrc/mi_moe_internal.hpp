@@ -283,6 +283,13 @@ struct MxArgs {
   unsigned char* act;      // [n][mx_row_bytes(I)] quantized intermediate, row = sorted position
   int16_t* eout;           // [n][H] expert outputs, row = pair, 16-bit integers
   float* eout_d;           // [n][H/64] their scales
+  unsigned long long* tact;   // one-launch decode: tagged units [n][I/32][8] (within tagged_act_bytes(I))
 };
+
+// Decode calls (mx_decode.hip): up to 64 routed pairs (a wave's ballot), a
+// wave of the down workgroup per routed expert; in one launch where its
+// workgroups' 8 waves hold the top-k and the handle has a hand-over buffer.
+inline bool mx_decode_ok(int64_t n, int64_t K) { return n <= 64 && K <= 16; }
+inline bool mx_decode_fused(int64_t n, int64_t K, int I) { return mx_decode_ok(n, K) && K <= 8 && I <= kTagActMaxI; }
 
 }  // namespace mimoe

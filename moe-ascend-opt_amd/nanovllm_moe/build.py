@@ -24,7 +24,7 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 
 HIP_SOURCES = ["capi.hip", "common_kernels.hip", "w4a16.hip", "w4a16_fused.hip", "qint.hip", "hybrid.hip", "mx.hip",
-               "router.hip"]
+               "mx_decode.hip", "router.hip"]
 # Host-only C++ (no HIP): the host executor of the hybrid offload path and the
 # CPU engine of the Q8_0 / Q4_0 layer (its C ABI too).  Inner loops are
 # compiled per instruction set (target attributes) and picked at run time;
@@ -47,6 +47,7 @@ FILE_FLAGS = {"qint.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-amdgp
               "w4a16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-amdgpu-kernarg-preload-count=16"],
               "w4a16_fused.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-amdgpu-kernarg-preload-count=16"],
               "mx.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-amdgpu-kernarg-preload-count=16"],
+              "mx_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-mllvm", "-amdgpu-kernarg-preload-count=16"],
               "router.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
               "common_kernels.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"]}
 

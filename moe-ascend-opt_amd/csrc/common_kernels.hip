@@ -5,6 +5,7 @@
 
 #include "mi_moe_device.hpp"
 #include "mi_moe_internal.hpp"
+#include "mx_device.hpp"
 
 namespace mimoe {
 
@@ -48,20 +49,23 @@ __device__ __forceinline__ int tile_class(int rows) { return kTileClasses - ((ro
 
 // Wave 0: per-expert totals counts[E] (LDS) -> counts_out, starts_out, the
 // active list, U and the row tiles; counts[] becomes the starts.  Tiles are
-// listed by class (lpt: heaviest first; otherwise one class), within a class
-// by expert, then by row.
+// listed by class (lpt 1: heaviest first; otherwise one class), within a class
+// by expert, then by row.  lpt kRouteBigTiles: one class, tiles of 2 kGemmRows.
 __device__ void route_finish(int* counts, int E, int lane, int32_t* counts_out, int32_t* starts_out,
                              int32_t* active_out, int32_t* U_out, int32_t* tiles_out, int32_t* ntiles_out,
                              int lpt) {
   const int per = (E + kWave - 1) / kWave;
   const int base = lane * per;
+  const int trows = lpt == kRouteBigTiles ? 2 * kGemmRows : kGemmRows, tlog = lpt == kRouteBigTiles ? 7 : 6;
+  static_assert(kGemmRows == 64, "tlog");
+  lpt &= 1;
   // rows, active experts and row tiles per class of this lane's experts
   int s = 0, a = 0, t0 = 0, t1 = 0, t2 = 0, t3 = 0;
   for (int i = 0; i < per; ++i) {
     const int e = base + i;
     if (e < E) {
-      const int c = counts[e], rem = c % kGemmRows, k = lpt ? tile_class(rem) : 0;
-      s += c; a += (c > 0); t0 += c / kGemmRows;
+      const int c = counts[e], rem = c & (trows - 1), k = lpt ? tile_class(rem) : 0;
+      s += c; a += (c > 0); t0 += c >> tlog;
       if (rem) { t0 += k == 0; t1 += k == 1; t2 += k == 2; t3 += k == 3; }
     }
   }
@@ -86,8 +90,8 @@ __device__ void route_finish(int* counts, int E, int lane, int32_t* counts_out, 
       counts[e] = sx;
       if (c > 0) active_out[ax++] = e;
       if (tiles_out)
-        for (int r0 = 0; r0 < c; r0 += kGemmRows) {
-          const int rows = min(kGemmRows, c - r0), k = lpt ? tile_class(rows) : 0;
+        for (int r0 = 0; r0 < c; r0 += trows) {
+          const int rows = min(trows, c - r0), k = lpt ? tile_class(rows) : 0;
           const int tx = k == 0 ? x0++ : k == 1 ? x1++ : k == 2 ? x2++ : x3++;
           *reinterpret_cast<int4*>(tiles_out + 4 * tx) = int4{e, sx + r0, rows, 0};
         }
@@ -220,10 +224,9 @@ __global__ __launch_bounds__(kRouteThreads) void route_global_kernel(
 // Multi-workgroup routing, step 1: the expert histogram of one chunk of ids.
 constexpr int kRouteCountThreads = 256;
 static_assert(kRouteChunk % kRouteCountThreads == 0, "a count thread takes a whole number of ids");
-__global__ __launch_bounds__(kRouteCountThreads) void route_count_kernel(const int32_t* __restrict__ ids, int n,
-                                                                         int E, int32_t* chunk_counts) {
-  extern __shared__ int hist[];   // [E]
-  const int tid = threadIdx.x, c = blockIdx.x;
+__device__ __forceinline__ void route_count_body(const int32_t* __restrict__ ids, int n, int E, int32_t* chunk_counts, int c,
+                                                 int* hist) {   // hist [E] in LDS
+  const int tid = threadIdx.x;
   for (int e = tid; e < E; e += kRouteCountThreads) hist[e] = 0;
   __syncthreads();
   const int lo = c * kRouteChunk, hi = min(n, lo + kRouteChunk);
@@ -239,6 +242,25 @@ __global__ __launch_bounds__(kRouteCountThreads) void route_count_kernel(const i
     if ((unsigned)ev[j] < (unsigned)E) atomicAdd(&hist[ev[j]], 1);
   __syncthreads();
   for (int e = tid; e < E; e += kRouteCountThreads) chunk_counts[(size_t)c * E + e] = hist[e];
+}
+__global__ __launch_bounds__(kRouteCountThreads) void route_count_kernel(const int32_t* __restrict__ ids, int n,
+                                                                         int E, int32_t* chunk_counts) {
+  extern __shared__ int hist[];
+  route_count_body(ids, n, E, chunk_counts, blockIdx.x, hist);
+}
+// The same, with the MXFP6 quantization of the hidden rows in the workgroups after the C chunks'.
+template <int ACT>
+__global__ __launch_bounds__(kRouteCountThreads) void route_count_mx_kernel(const int32_t* __restrict__ ids, int n, int E,
+                                                                            int32_t* chunk_counts, int C,
+                                                                            const uint16_t* __restrict__ x, int T, int H,
+                                                                            unsigned char* __restrict__ xq) {
+  extern __shared__ int hist[];
+  if ((int)blockIdx.x < C) {   // uniform
+    route_count_body(ids, n, E, chunk_counts, blockIdx.x, hist);
+    return;
+  }
+  mx_quant_rows<ACT>(x, T, H, xq, (int64_t)(blockIdx.x - C) * kRouteCountThreads + threadIdx.x,
+                     (int64_t)(gridDim.x - C) * kRouteCountThreads);
 }
 
 // Step 2 (one workgroup): totals over the C chunks, the outputs of
@@ -313,29 +335,72 @@ __global__ __launch_bounds__(kRouteThreads) void route_scatter_kernel(const int3
   route_seg_rank(lo, hi, K, nullptr, lane, mine, seg, tok, scat, tok_div);
 }
 
+// Steps 2 and 3 of the multi-workgroup routing.
+static hipError_t launch_route_scan_scatter(const int32_t* ids, int n, int K, int E, const RouteGlobal& rg, hipStream_t st,
+                                            int tok_div, int lpt) {
+  const int C = route_chunks(n);
+  hipLaunchKernelGGL(route_scan_kernel, dim3(1), dim3(kRouteThreads), (size_t)E * sizeof(int), st, rg.chunk,
+                     C, E, rg.counts, rg.starts, rg.active, rg.U, rg.tiles, rg.ntiles, lpt);
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return err;
+  hipLaunchKernelGGL(route_scatter_kernel, dim3(C), dim3(kRouteThreads), (size_t)kRouteWaves * E * sizeof(int),
+                     st, ids, n, K, E, rg.chunk, rg.tok, rg.scat, tok_div);
+  return hipGetLastError();
+}
+
 // tok_div = 0: tok[] holds pair indices t*K+k (fused kernels); 1: token ids.
-// lpt: row tiles heaviest first (route_finish).
+// lpt: order and size of the row tiles (route_finish).
 hipError_t launch_route_global(const int32_t* ids, int n, int K, int E, const RouteGlobal& rg,
                                hipStream_t st, int tok_div, int lpt) {
   if (n > kRouteMultiMin) {
     if (!rg.chunk) return hipErrorInvalidValue;   // the chunked routing needs its scratch
-    const int C = (n + kRouteChunk - 1) / kRouteChunk;
-    hipLaunchKernelGGL(route_count_kernel, dim3(C), dim3(kRouteCountThreads), (size_t)E * sizeof(int), st, ids,
-                       n, E, rg.chunk);
-    hipError_t err = hipGetLastError();
+    hipLaunchKernelGGL(route_count_kernel, dim3(route_chunks(n)), dim3(kRouteCountThreads), (size_t)E * sizeof(int), st,
+                       ids, n, E, rg.chunk);
+    const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
-    hipLaunchKernelGGL(route_scan_kernel, dim3(1), dim3(kRouteThreads), (size_t)E * sizeof(int), st, rg.chunk,
-                       C, E, rg.counts, rg.starts, rg.active, rg.U, rg.tiles, rg.ntiles, lpt);
-    err = hipGetLastError();
-    if (err != hipSuccess) return err;
-    hipLaunchKernelGGL(route_scatter_kernel, dim3(C), dim3(kRouteThreads), (size_t)kRouteWaves * E * sizeof(int),
-                       st, ids, n, K, E, rg.chunk, rg.tok, rg.scat, tok_div);
-    return hipGetLastError();
+    return launch_route_scan_scatter(ids, n, K, E, rg, st, tok_div, lpt);
   }
   const size_t lds = (size_t)(kRouteWaves + 1) * E * sizeof(int);
   hipLaunchKernelGGL(route_global_kernel, dim3(1), dim3(kRouteThreads), lds, st, ids, n, K, E,
                      rg.counts, rg.starts, rg.active, rg.tok, rg.scat, rg.U, tok_div, rg.tiles,
                      rg.ntiles, lpt);
+  return hipGetLastError();
+}
+
+// The single-workgroup routing (workgroup 0) and the MXFP6 quantization of
+// the hidden rows (the others): independent, in one launch.
+template <int ACT>
+__global__ __launch_bounds__(kRouteThreads) void route_mx_kernel(const int32_t* __restrict__ ids, int n, int K, int E,
+                                                                 RouteGlobal rg, int lpt, const uint16_t* __restrict__ x, int T,
+                                                                 int H, unsigned char* __restrict__ xq) {
+  extern __shared__ int lds[];
+  if (blockIdx.x == 0) {   // uniform
+    route_global_body(ids, n, K, E, rg.counts, rg.starts, rg.active, rg.tok, rg.scat, rg.U, 0, rg.tiles, rg.ntiles, lds, lpt);
+    return;
+  }
+  mx_quant_rows<ACT>(x, T, H, xq, (int64_t)(blockIdx.x - 1) * kRouteThreads + threadIdx.x,
+                     (int64_t)(gridDim.x - 1) * kRouteThreads);
+}
+
+// Routing with row tiles (lpt: route_finish) and the hidden rows as MXFP6 packets.
+hipError_t launch_route_mx(const void* x, int act, int T, int H, unsigned char* xq, const int32_t* ids, int n, int K, int E,
+                           const RouteGlobal& rg, hipStream_t st, int lpt) {
+  const int64_t blocks = (int64_t)T * 4 * mx_ktiles(H);
+  const uint16_t* xr = (const uint16_t*)x;
+  if (n > kRouteMultiMin) {
+    if (!rg.chunk) return hipErrorInvalidValue;
+    const int C = route_chunks(n);
+    const unsigned g = (unsigned)(C + std::min<int64_t>((blocks + kRouteCountThreads - 1) / kRouteCountThreads, 32768));
+    auto kern = act == 1 ? route_count_mx_kernel<1> : route_count_mx_kernel<0>;
+    hipLaunchKernelGGL(kern, dim3(g), dim3(kRouteCountThreads), (size_t)E * sizeof(int), st, ids, n, E, rg.chunk, C, xr, T, H, xq);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+    return launch_route_scan_scatter(ids, n, K, E, rg, st, 0, lpt);
+  }
+  const unsigned g = (unsigned)(1 + std::min<int64_t>((blocks + kRouteThreads - 1) / kRouteThreads, 1024));
+  auto kern = act == 1 ? route_mx_kernel<1> : route_mx_kernel<0>;
+  hipLaunchKernelGGL(kern, dim3(g), dim3(kRouteThreads), (size_t)(kRouteWaves + 1) * E * sizeof(int), st, ids, n, K, E, rg, lpt,
+                     xr, T, H, xq);
   return hipGetLastError();
 }
 

@@ -49,6 +49,9 @@ __host__ __device__ inline int64_t gemm_tiles_max(int64_t n, int E) {
   return n / kGemmRows + (n < E ? n : E);
 }
 
+// Row tiles of twice the rows (an order of route_finish).
+constexpr int kRouteBigTiles = 2;
+
 // Error reporting and shape rules shared by the C-ABI translation units:
 // api_fail records msg as the thread's last error and returns code;
 // check_dims applies the handle shape rules of mi_moe_create.
@@ -268,6 +271,11 @@ constexpr int kMxTileScaleBytes = 256;    // its scales: [64 lanes][4 tiles]
 constexpr int kMxPacketBytes = 32;        // an activation block: 24 B of codes, its scale byte
 __host__ __device__ constexpr size_t mx_row_bytes(int K) { return (size_t)mx_ktiles(K) * 4 * kMxPacketBytes; }
 
+// Rows per expert on average from which the grouped products (mx.hip) take
+// items of 128 rows.
+constexpr int kMxBigRows = 96;
+inline bool mx_big(int64_t n, int64_t E) { return n >= kMxBigRows * E; }
+
 struct MxArgs {
   const uint16_t* x;       // [T,H] act dtype bits
   uint16_t* y;             // [T,H]
@@ -281,8 +289,8 @@ struct MxArgs {
   const unsigned char* w2_s;
   unsigned char* xq;       // [T][mx_row_bytes(H)] quantized hidden rows
   unsigned char* act;      // [n][mx_row_bytes(I)] quantized intermediate, row = sorted position
-  int16_t* eout;           // [n][H] expert outputs, row = pair, 16-bit integers
-  float* eout_d;           // [n][H/64] their scales
+  int16_t* eout;           // [n][H] expert outputs, row = pair, 16-bit fixed point
+  unsigned char* eout_d;   // [n][H/64][4] their scales
   unsigned long long* tact;   // one-launch decode: tagged units [n][I/32][8] (within tagged_act_bytes(I))
 };
 

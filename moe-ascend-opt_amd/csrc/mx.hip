@@ -9,6 +9,8 @@
 // and run at the 4-bit rate, and its noise (2.8% of a Gaussian block, 2.6%
 // for E4M3) stays far below that of the 4-bit weights (11%).
 #pragma clang fp contract(off)
+#include <type_traits>
+
 #include "mx_device.hpp"
 
 namespace mimoe {
@@ -17,10 +19,6 @@ namespace {
 
 constexpr int kMxWaves = 8;
 constexpr int kMxThreads = kMxWaves * kWave;
-constexpr int kMxChunkK = 2;                              // k tiles staged at a time
-constexpr int kMxChunkRow = kMxChunkK * 4 * kMxPacketBytes;   // 256 B of a row
-constexpr int kMxStage = kGemmRows * kMxChunkRow;         // 16 KB
-
 __device__ __forceinline__ u32x4_t ld16(const void* p) { return *reinterpret_cast<const u32x4_t*>(p); }
 __device__ __forceinline__ void st16(void* p, const u32x4_t& v) { *reinterpret_cast<u32x4_t*>(p) = v; }
 
@@ -58,184 +56,237 @@ __device__ __forceinline__ bool mx_tile(const RouteGlobal& rg, int nblk, MxTile&
   return true;
 }
 
-// LDS position of 16-byte piece c of row r's chunk: pieces are permuted by
-// the row, so that the 16 rows of an operand read lie in different banks.
-__device__ __forceinline__ int mx_lds(int r, int c) { return r * kMxChunkRow + ((c ^ (r & 15)) << 4); }
+// The grouped products run one instance per number of 16-row subtiles of the
+// work item (rounded up to 1, 2, 4 or 8): without branches in the K loop the
+// loads of the next step stay in flight across it.
+// A step is S k tiles (S * 128 B of a row): enough products between barriers
+// to cover a load's latency, and a 16-byte piece for every thread.
+constexpr int mx_step(int nsub) { return nsub == 1 ? 4 : 2; }
+constexpr int mx_stage_bytes(int nsub) { return nsub * 16 * mx_step(nsub) * 128; }
 
 // acc[t][s] = tile t of the wave's weight unit times the rows of subtile s,
-// over all kt k tiles.  src: this thread's row of packets (row tid / 8) and
-// part (tid % 8) of every chunk; w, ws: the unit's codes and scales, at this
-// lane.  live: the wave has a unit (uniform); every wave stages.
-__device__ __forceinline__ void mx_gemm_core(unsigned char* smem, const unsigned char* src, int kt, const unsigned char* w,
-                                             const unsigned char* ws, int nsub, bool live, f32x4_t (&acc)[4][4]) {
-  const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, r = lane & 15, srow = tid >> 3, part = tid & 7;
-  const int nc = (kt + kMxChunkK - 1) / kMxChunkK, last = 4 * kt - 1;
-  const bool stager = srow < 16 * nsub;
-  auto stage_load = [&](int c, u32x4_t (&v)[2]) {
-    const unsigned char* p = src + (size_t)min(8 * c + part, last) * kMxPacketBytes;
-    v[0] = ld16(p);
-    v[1] = ld16(p + 16);
+// over all kt k tiles.  row(i): the packets of row i of the item; w, ws: the
+// unit's codes and scales, at this lane.
+// Rows are staged in LDS, double-buffered, through registers; a wave's weights
+// go straight to its registers, each k tile's replaced as soon as it is used.
+// LDS pieces of 16 B are permuted by the row, so that the 16 rows of an
+// operand read lie in different banks.
+template <int NSUB, class Row>
+__device__ __forceinline__ void mx_gemm_core(unsigned char* smem, Row row, int kt, const unsigned char* w, const unsigned char* ws,
+                                             f32x4_t (&acc)[4][NSUB]) {
+  constexpr int S = mx_step(NSUB), STRIDE = S * 128, BYTES = mx_stage_bytes(NSUB);
+  constexpr bool PART = BYTES < kMxThreads * 16;            // not every thread stages
+  constexpr int NP = PART ? 1 : BYTES / (kMxThreads * 16);  // pieces of a thread, STEP rows apart
+  constexpr int STEP = kMxThreads / (8 * S);
+  const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, r = lane & 15;
+  const int piece = tid % (8 * S), last = 8 * kt - 1, row0 = PART ? min(tid / (8 * S), 16 * NSUB - 1) : tid / (8 * S);
+  const unsigned char* src[NP];
+  int dst[NP];
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    src[p] = row(row0 + STEP * p);
+    dst[p] = (row0 + STEP * p) * STRIDE + ((piece ^ ((row0 + STEP * p) & 15)) << 4);
+  }
+  const bool stager = !PART || tid < BYTES / 16;
+  u32x4_t sv[NP], wv[S][4];
+  uint32_t sc[S];
+  auto stage_load = [&](int c) {
+    const int o = min(8 * S * c + piece, last) << 4;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) sv[p] = ld16(src[p] + o);
   };
-  u32x4_t sv[2], wv[kMxChunkK][4];
-  uint32_t sc[kMxChunkK];
+  auto stage_store = [&](unsigned char* buf) {
+    if (stager)
+#pragma unroll
+      for (int p = 0; p < NP; ++p) st16(buf + dst[p], sv[p]);
+  };
   auto weights = [&](int k, u32x4_t (&v)[4], uint32_t& s) {
     const int kk = min(k, kt - 1);
 #pragma unroll
     for (int t = 0; t < 4; ++t) v[t] = ld16(w + (size_t)kk * kMxTileBytes + t * 1024);
     s = *reinterpret_cast<const uint32_t*>(ws + (size_t)kk * kMxTileScaleBytes);
   };
-  stage_load(0, sv);
+  const int rd = r * STRIDE + (((2 * q) ^ r) << 4);
+  auto products = [&](const unsigned char* buf, int k) {
+    const int a0 = rd ^ (k << 7), a1 = a0 ^ 16;
 #pragma unroll
-  for (int k = 0; k < kMxChunkK; ++k) weights(k, wv[k], sc[k]);
+    for (int s = 0; s < NSUB; ++s) {
+      const u32x4_t lo = ld16(buf + a0 + s * 16 * STRIDE), hi = ld16(buf + a1 + s * 16 * STRIDE);
+      acc[0][s] = mx_mfma<0>(wv[k][0], sc[k], lo, hi, acc[0][s]);
+      acc[1][s] = mx_mfma<1>(wv[k][1], sc[k], lo, hi, acc[1][s]);
+      acc[2][s] = mx_mfma<2>(wv[k][2], sc[k], lo, hi, acc[2][s]);
+      acc[3][s] = mx_mfma<3>(wv[k][3], sc[k], lo, hi, acc[3][s]);
+    }
+  };
+  stage_load(0);
+#pragma unroll
+  for (int k = 0; k < S; ++k) weights(k, wv[k], sc[k]);
 #pragma unroll
   for (int t = 0; t < 4; ++t)
 #pragma unroll
-    for (int s = 0; s < 4; ++s) acc[t][s] = f32x4_t{0, 0, 0, 0};
-  if (stager) {
-    st16(smem + mx_lds(srow, 2 * part), sv[0]);
-    st16(smem + mx_lds(srow, 2 * part + 1), sv[1]);
-  }
+    for (int s = 0; s < NSUB; ++s) acc[t][s] = f32x4_t{0, 0, 0, 0};
+  stage_store(smem);
   __syncthreads();
+  const int nc = kt / S, rest = kt - nc * S;
   for (int c = 0; c < nc; ++c) {
-    const unsigned char* buf = smem + (c & 1) * kMxStage;
-    if (c + 1 < nc) stage_load(c + 1, sv);
-    if (live) {
+    const unsigned char* buf = smem + (c & 1) * BYTES;
+    stage_load(c + 1);   // past the end: the last piece again
+    __builtin_amdgcn_sched_barrier(0);   // loads stay where they are: sunk below the products they would be waited for at once
 #pragma unroll
-      for (int k = 0; k < kMxChunkK; ++k) {
-        if (kMxChunkK * c + k < kt) {   // uniform
-#pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            if (s < nsub) {   // uniform
-              const int row = 16 * s + r;
-              const u32x4_t lo = ld16(buf + mx_lds(row, 2 * (4 * k + q))), hi = ld16(buf + mx_lds(row, 2 * (4 * k + q) + 1));
-              acc[0][s] = mx_mfma<0>(wv[k][0], sc[k], lo, hi, acc[0][s]);
-              acc[1][s] = mx_mfma<1>(wv[k][1], sc[k], lo, hi, acc[1][s]);
-              acc[2][s] = mx_mfma<2>(wv[k][2], sc[k], lo, hi, acc[2][s]);
-              acc[3][s] = mx_mfma<3>(wv[k][3], sc[k], lo, hi, acc[3][s]);
-            }
-          }
-          // the weights of the same place in the next chunk, into the registers just used
-          weights(kMxChunkK * (c + 1) + k, wv[k], sc[k]);
-        }
-      }
+    for (int k = 0; k < S; ++k) {
+      products(buf, k);
+      __builtin_amdgcn_sched_barrier(0);
+      weights(S * (c + 1) + k, wv[k], sc[k]);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (c + 1 < nc && stager) {
-      unsigned char* nb = smem + ((c + 1) & 1) * kMxStage;
-      st16(nb + mx_lds(srow, 2 * part), sv[0]);
-      st16(nb + mx_lds(srow, 2 * part + 1), sv[1]);
-    }
+    stage_store(smem + ((c + 1) & 1) * BYTES);
     __syncthreads();
   }
+#pragma unroll
+  for (int k = 0; k < S - 1; ++k)
+    if (k < rest) products(smem + (nc & 1) * BYTES, k);   // uniform
 }
 
-// gate_up + SiLU*mul + MXFP6: work item (row tile, 8 slices of 32 rows of I,
-// one per wave).  A wave's gate and up tiles hold the same rows of I, so the
-// product is in registers; a transpose between its lane rows leaves every
-// lane with the 32 values of one token's block.
-__global__ __launch_bounds__(kMxThreads) void mx_gemm13_kernel(MxArgs a) {
-  __shared__ __align__(16) unsigned char smem[2 * kMxStage];
-  const int NS = a.I >> 5, kt = mx_ktiles(a.H), NSP = 4 * mx_ktiles(a.I), nblk = (NSP + kMxWaves - 1) / kMxWaves;
-  MxTile t;
-  if (!mx_tile(a.rg, nblk, t)) return;   // uniform
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int slice = kMxWaves * t.blk + wave, nsub = (t.rows + 15) >> 4;
-  const bool live = slice < NS;
-  const int pair = a.rg.tok[t.row0 + min(tid >> 3, t.rows - 1)];
-  const size_t unit = ((size_t)t.e * NS + (live ? slice : 0)) * kt;
-  f32x4_t acc[4][4];
-  mx_gemm_core(smem, a.xq + (size_t)(pair / a.K) * mx_row_bytes(a.H), kt, a.w13 + unit * kMxTileBytes + lane * 16,
-               a.w13_s + unit * kMxTileScaleBytes + lane * 4, nsub, live, acc);
-  if (slice >= NSP) return;
-  float v[32];   // [q][tile][4] after the transpose
+// gate_up + SiLU*mul + MXFP6 of one work item: a unit is a slice of 32 rows of
+// I (its gate and up tiles hold the same rows, so the product is in
+// registers); a transpose between the wave's lane rows leaves every lane with
+// the 32 values of one token's block.
+template <int NSUB>
+__device__ __forceinline__ void mx_gate_up(const MxArgs& a, unsigned char* smem, int e, int row0, int rows, int slice) {
+  const int NS = a.I >> 5, kt = mx_ktiles(a.H), lane = threadIdx.x & 63;
+  const size_t unit = ((size_t)e * NS + min(slice, NS - 1)) * kt;
+  f32x4_t acc[4][NSUB];
+  mx_gemm_core<NSUB>(
+      smem, [&](int i) { return a.xq + (size_t)(a.rg.tok[row0 + min(i, rows - 1)] / a.K) * mx_row_bytes(a.H); }, kt,
+      a.w13 + unit * kMxTileBytes + lane * 16, a.w13_s + unit * kMxTileScaleBytes + lane * 4, acc);
+  if (slice >= 4 * mx_ktiles(a.I)) return;
 #pragma unroll
-  for (int p = 0; p < 2; ++p)
+  for (int g = 0; g < (NSUB + 3) / 4; ++g) {   // four subtiles at a time
+    float v[32];   // [tile][q][4] after the transpose
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float h[4];
+    for (int p = 0; p < 2; ++p)
 #pragma unroll
-      for (int s = 0; s < 4; ++s) h[s] = silu_mul_fast(acc[p][s][i], acc[2 + p][s][i]);
-      transpose4(h[0], h[1], h[2], h[3]);
+      for (int i = 0; i < 4; ++i) {
+        float h[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v[16 * p + 4 * q + i] = h[q];
-    }
-  MxPacket pk = {u32x4_t{0, 0, 0, 0}, u32x4_t{0, 0, 0, 0}};
-  if (live) {
+        for (int s = 0; s < 4; ++s) {
+          const int ss = 4 * g + s < NSUB ? 4 * g + s : 0;
+          h[s] = 4 * g + s < NSUB ? silu_mul_fast(acc[p][ss][i], acc[2 + p][ss][i]) : 0.0f;
+        }
+        transpose4(h[0], h[1], h[2], h[3]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[16 * p + 4 * q + i] = h[q];
+      }
     const int s = mx_scale_byte<kMxFp6>(mx_amax32(v));
-    pk = mx_packet(mx_fp6_codes32(v, s), s);
-  }
-  if (lane < t.rows) {   // lane = 16 subtile + row
-    unsigned char* o = a.act + (size_t)(t.row0 + lane) * mx_row_bytes(a.I) + slice * kMxPacketBytes;
-    st16(o, pk.lo);
-    st16(o + 16, pk.hi);
-  }
-}
-
-// Expert outputs between the down product and the combine: 16-bit integers
-// with a power-of-two scale per 64 columns.  Half of fp32's bytes, and the
-// rounding, at most 2^-15 of the 64 columns' largest, is far below that of
-// the 16-bit result (16-bit floats would add as much as the result's own).
-__device__ __forceinline__ float eout_scale(uint32_t amax_bits) {   // 2^(e - 14), NaN for NaN and infinity
-  if (amax_bits >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
-  const int e = (int)(amax_bits >> 23);   // biased
-  return __uint_as_float((uint32_t)(e > 15 ? e - 14 : 1) << 23);
-}
-
-// down: work item (row tile, 8 units of 64 rows of H, one per wave).
-__global__ __launch_bounds__(kMxThreads) void mx_gemm2_kernel(MxArgs a) {
-  __shared__ __align__(16) unsigned char smem[2 * kMxStage];
-  const int NQ = a.H >> 6, kt = mx_ktiles(a.I), nblk = (NQ + kMxWaves - 1) / kMxWaves;
-  MxTile t;
-  if (!mx_tile(a.rg, nblk, t)) return;   // uniform
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int m = kMxWaves * t.blk + wave, nsub = (t.rows + 15) >> 4;
-  const bool live = m < NQ;
-  const size_t unit = ((size_t)t.e * NQ + (live ? m : 0)) * kt;
-  f32x4_t acc[4][4];
-  mx_gemm_core(smem, a.act + (size_t)(t.row0 + min(tid >> 3, t.rows - 1)) * mx_row_bytes(a.I), kt,
-               a.w2 + unit * kMxTileBytes + lane * 16, a.w2_s + unit * kMxTileScaleBytes + lane * 4, nsub, live, acc);
-  if (!live) return;
-  float v[64];
-#pragma unroll
-  for (int p = 0; p < 4; ++p)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float h[4] = {acc[p][0][i], acc[p][1][i], acc[p][2][i], acc[p][3][i]};
-      transpose4(h[0], h[1], h[2], h[3]);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) v[16 * p + 4 * q + i] = h[q];
+    MxPacket pk = mx_packet(mx_fp6_codes32(v, s), s);
+    if (slice >= NS) pk = MxPacket{u32x4_t{0, 0, 0, 0}, u32x4_t{0, 0, 0, 0}};   // past I
+    const int i = 64 * g + lane;   // 16 subtile + row
+    if (lane < 16 * NSUB && i < rows) {
+      unsigned char* o = a.act + (size_t)(row0 + i) * mx_row_bytes(a.I) + slice * kMxPacketBytes;
+      st16(o, pk.lo);
+      st16(o + 16, pk.hi);
     }
-  if (lane >= t.rows) return;
+  }
+}
+
+// Expert outputs between the down product and the combine: 16-bit fixed point
+// with a power-of-two scale for every 16 columns.  Half of fp32's bytes; the
+// rounding, at most 2^-15 of the 16 columns' largest, is far below that of
+// the 16-bit result (16-bit floats would add as much as the result's own).
+// Stores 16 columns and returns their scale byte s: |values| < 2^(s-126),
+// 255: one of them is NaN or infinite.
+__device__ __forceinline__ uint32_t eout_store(int16_t* o, const float (&v)[16]) {
   uint32_t am = 0;
 #pragma unroll
-  for (int i = 0; i < 64; ++i) {
+  for (int i = 0; i < 16; ++i) {
     const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
     am = b > am ? b : am;
   }
-  const float d = eout_scale(am), id = 1.0f / d;   // powers of two
-  const int pair = a.rg.tok[t.row0 + lane];
-  int16_t* o = a.eout + (size_t)pair * a.H + 64 * m;
+  const uint32_t s = am >= 0x7f800000u ? 255 : am >= 0x00800000u ? am >> 23 : 1;
+  const float id = __builtin_ldexpf(1.0f, 126 - (int)s);
+  uint32_t w[8];
 #pragma unroll
-  for (int c = 0; c < 8; ++c) {
-    uint32_t w[4];
+  for (int i = 0; i < 8; ++i)
+    w[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_i16(v[2 * i] * id, v[2 * i + 1] * id));
+  st16(o, u32x4_t{w[0], w[1], w[2], w[3]});
+  st16(o + 8, u32x4_t{w[4], w[5], w[6], w[7]});
+  return s;
+}
+// the factor of a value's integer
+__device__ __forceinline__ float eout_scale(int s) {
+  return s == 255 ? __uint_as_float(0x7fc00000u) : __builtin_ldexpf(1.0f / 32767.0f, s - 126);
+}
+
+// down of one work item: a unit is 64 rows of H.  After a transpose between
+// its lane rows a lane stores a token's 64 columns, a whole cache line (in 8
+// byte pieces, without the transpose, T = 4096 takes 118 us, not 92).
+template <int NSUB>
+__device__ __forceinline__ void mx_down(const MxArgs& a, unsigned char* smem, int e, int row0, int rows, int m) {
+  const int NQ = a.H >> 6, kt = mx_ktiles(a.I), lane = threadIdx.x & 63;
+  const size_t unit = ((size_t)e * NQ + min(m, NQ - 1)) * kt;
+  f32x4_t acc[4][NSUB];
+  mx_gemm_core<NSUB>(
+      smem, [&](int i) { return a.act + (size_t)(row0 + min(i, rows - 1)) * mx_row_bytes(a.I); }, kt,
+      a.w2 + unit * kMxTileBytes + lane * 16, a.w2_s + unit * kMxTileScaleBytes + lane * 4, acc);
+  if (m >= NQ) return;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      int z[2];
+  for (int g = 0; g < (NSUB + 3) / 4; ++g) {   // four subtiles at a time
+    const int row = 64 * g + lane;   // 16 subtile + row
+    const int pair = a.rg.tok[row0 + min(row, rows - 1)];
+    int16_t* o = a.eout + (size_t)pair * a.H + 64 * m;
+    uint32_t s4 = 0;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int n = (int)__builtin_rintf(v[8 * c + 2 * j + k] * id);
-        z[k] = n > 32767 ? 32767 : n;   // the largest may round up to 2^15; -2^15 is there
+    for (int t = 0; t < 4; ++t) {
+      float v[16];   // [q][4]
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float h[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) h[s] = 4 * g + s < NSUB ? acc[t][4 * g + s < NSUB ? 4 * g + s : 0][i] : 0.0f;
+        transpose4(h[0], h[1], h[2], h[3]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[4 * q + i] = h[q];
       }
-      w[j] = ((uint32_t)z[0] & 0xffffu) | ((uint32_t)z[1] << 16);
+      if (row < rows) s4 |= eout_store(o + 16 * t, v) << (8 * t);
     }
-    st16(o + 8 * c, u32x4_t{w[0], w[1], w[2], w[3]});
+    if (row < rows) *reinterpret_cast<uint32_t*>(a.eout_d + ((size_t)pair * NQ + m) * 4) = s4;
   }
-  a.eout_d[(size_t)pair * NQ + m] = d;
+}
+
+// Work item: 8 units, one a wave, and a row tile of an expert: up to 64 rows,
+// or with BIG 128 (kRouteBigTiles).
+template <bool BIG, bool DOWN>
+__device__ __forceinline__ void mx_gemm_item(const MxArgs& a, unsigned char* smem) {
+  const int units = DOWN ? a.H >> 6 : 4 * mx_ktiles(a.I);
+  MxTile t;
+  if (!mx_tile(a.rg, (units + kMxWaves - 1) / kMxWaves, t)) return;   // uniform
+  const int nsub = (t.rows + 15) >> 4, unit = kMxWaves * t.blk + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  auto run = [&](auto n) {
+    if constexpr (DOWN) mx_down<decltype(n)::value>(a, smem, t.e, t.row0, t.rows, unit);
+    else mx_gate_up<decltype(n)::value>(a, smem, t.e, t.row0, t.rows, unit);
+  };
+  if (BIG && nsub > 4) run(std::integral_constant<int, BIG ? 8 : 4>{});
+  else if (nsub > 2) run(std::integral_constant<int, 4>{});
+  else if (nsub == 2) run(std::integral_constant<int, 2>{});
+  else run(std::integral_constant<int, 1>{});
+}
+
+// 64-row items at four waves per SIMD, 128-row items at two (twice the accumulators).
+template <bool DOWN>
+__global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(4))) void mx_gemm_kernel(MxArgs a) {
+  __shared__ __align__(16) unsigned char smem[2 * mx_stage_bytes(4)];
+  mx_gemm_item<false, DOWN>(a, smem);
+}
+template <bool DOWN>
+__global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(2))) void mx_gemm_big_kernel(MxArgs a) {
+  __shared__ __align__(16) unsigned char smem[2 * mx_stage_bytes(8)];
+  mx_gemm_item<true, DOWN>(a, smem);
 }
 
 // y[t,h] = cast(sum_k w[t,k] eout[t*K+k,h]) over the valid ids in k order, in
 // fp32; a token without a valid id gets 0.  One thread per (t, 8 columns).
 template <int ACT>
-__global__ void mx_combine_kernel(const int16_t* __restrict__ eout, const float* __restrict__ eout_d, const float* __restrict__ tw,
+__global__ void mx_combine_kernel(const int16_t* __restrict__ eout, const unsigned char* __restrict__ eout_d, const float* __restrict__ tw,
                                   const int32_t* __restrict__ ids, uint16_t* __restrict__ y, int T, int K, int E, int H) {
   const int HV = H >> 3, NQ = H >> 6;
   const int64_t total = (int64_t)T * HV;
@@ -245,23 +296,25 @@ __global__ void mx_combine_kernel(const int16_t* __restrict__ eout, const float*
     constexpr int kB = 8;   // pairs whose loads are issued together
     for (int k0 = 0; k0 < K; k0 += kB) {
       int ev[kB];
-      float wv[kB], dv[kB];
+      float wv[kB];
+      int dv[kB];   // scale bytes
       u32x4_t rv[kB];
 #pragma unroll
       for (int j = 0; j < kB; ++j) {
         const int i = t * K + min(k0 + j, K - 1);
         ev[j] = k0 + j < K ? ids[i] : -1;
         wv[j] = tw[i];
-        dv[j] = eout_d[(size_t)i * NQ + (h >> 6)];
+        dv[j] = eout_d[(size_t)i * NQ * 4 + (h >> 4)];
         rv[j] = ld16(eout + (size_t)i * H + h);
       }
 #pragma unroll
       for (int j = 0; j < kB; ++j) {
         if ((unsigned)ev[j] >= (unsigned)E) continue;
         const uint32_t u[4] = {rv[j].x, rv[j].y, rv[j].z, rv[j].w};
+        const float d = eout_scale(dv[j]);
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
-          const float lo = (float)(int16_t)(u[p] & 0xffffu) * dv[j], hi = (float)((int32_t)u[p] >> 16) * dv[j];   // exact
+          const float lo = (float)(int16_t)(u[p] & 0xffffu) * d, hi = (float)((int32_t)u[p] >> 16) * d;
           acc[2 * p] = acc[2 * p] + wv[j] * lo;
           acc[2 * p + 1] = acc[2 * p + 1] + wv[j] * hi;
         }
@@ -272,33 +325,6 @@ __global__ void mx_combine_kernel(const int16_t* __restrict__ eout, const float*
     for (int p = 0; p < 4; ++p)
       o[p] = from_f32<ACT>(acc[2 * p]) | ((uint32_t)from_f32<ACT>(acc[2 * p + 1]) << 16);
     st16(y + (size_t)t * H + h, u32x4_t{o[0], o[1], o[2], o[3]});
-  }
-}
-
-__device__ __forceinline__ void ld_words(const void* p, uint32_t (&w)[16]) {
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const u32x4_t v = ld16(reinterpret_cast<const unsigned char*>(p) + 16 * c);
-    w[4 * c] = v.x; w[4 * c + 1] = v.y; w[4 * c + 2] = v.z; w[4 * c + 3] = v.w;
-  }
-}
-
-// Hidden rows -> packets, one thread per block; blocks past H are zeros.
-template <int ACT>
-__global__ void mx_quant_rows_kernel(const uint16_t* __restrict__ x, int T, int H, unsigned char* __restrict__ xq) {
-  const int nb = H >> 5, nbp = 4 * mx_ktiles(H);
-  const int64_t total = (int64_t)T * nbp;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int t = (int)(i / nbp), b = (int)(i - (int64_t)t * nbp);
-    MxPacket pk = {u32x4_t{0, 0, 0, 0}, u32x4_t{0, 0, 0, 0}};
-    if (b < nb) {
-      uint32_t w[16];
-      ld_words(x + (size_t)t * H + 32 * b, w);
-      const int s = mx_scale_byte<kMxFp6>(mx_amax16<ACT>(w));
-      pk = mx_packet(mx_fp6_codes16<ACT>(w, s), s);
-    }
-    st16(xq + i * kMxPacketBytes, pk.lo);
-    st16(xq + i * kMxPacketBytes + 16, pk.hi);
   }
 }
 
@@ -313,7 +339,7 @@ __device__ __forceinline__ void ld_block(const void* x, size_t elem, float (&v)[
     }
   } else {
     uint32_t w[16];
-    ld_words(reinterpret_cast<const uint16_t*>(x) + elem, w);
+    mx_load_words(reinterpret_cast<const uint16_t*>(x) + elem, w);
     mx_unpack16<DT>(w, v);
   }
 }
@@ -438,22 +464,18 @@ unsigned blocks_for(int64_t items) {
 
 }  // namespace
 
-// The sorted path: the hidden rows quantized, both grouped products, the combine.
+// The sorted path behind the routing (launch_route_mx): both grouped products, the combine.
 hipError_t launch_mx_sorted(const MxArgs& a, int act, int tiles_max, hipStream_t st, hipEvent_t mid) {
-  const int64_t nbp = (int64_t)a.T * 4 * mx_ktiles(a.H);
-  if (act == 1)
-    hipLaunchKernelGGL(mx_quant_rows_kernel<1>, dim3(blocks_for(nbp)), dim3(256), 0, st, a.x, a.T, a.H, a.xq);
-  else
-    hipLaunchKernelGGL(mx_quant_rows_kernel<0>, dim3(blocks_for(nbp)), dim3(256), 0, st, a.x, a.T, a.H, a.xq);
-  hipError_t err = hipGetLastError();
-  if (err != hipSuccess) return err;
+  const bool big = mx_big(a.n, a.E);
   const int tg = (tiles_max + 7) / 8 * 8;   // an eighth for each XCD
   const int b13 = (4 * mx_ktiles(a.I) + kMxWaves - 1) / kMxWaves, b2 = ((a.H >> 6) + kMxWaves - 1) / kMxWaves;
-  hipLaunchKernelGGL(mx_gemm13_kernel, dim3(tg * b13), dim3(kMxThreads), 0, st, a);
-  err = hipGetLastError();
+  if (big) hipLaunchKernelGGL(mx_gemm_big_kernel<false>, dim3(tg * b13), dim3(kMxThreads), 0, st, a);
+  else hipLaunchKernelGGL(mx_gemm_kernel<false>, dim3(tg * b13), dim3(kMxThreads), 0, st, a);
+  hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
   if (mid && (err = hipEventRecord(mid, st)) != hipSuccess) return err;
-  hipLaunchKernelGGL(mx_gemm2_kernel, dim3(tg * b2), dim3(kMxThreads), 0, st, a);
+  if (big) hipLaunchKernelGGL(mx_gemm_big_kernel<true>, dim3(tg * b2), dim3(kMxThreads), 0, st, a);
+  else hipLaunchKernelGGL(mx_gemm_kernel<true>, dim3(tg * b2), dim3(kMxThreads), 0, st, a);
   err = hipGetLastError();
   if (err != hipSuccess) return err;
   const unsigned g = blocks_for((int64_t)a.T * (a.H >> 3));

@@ -124,6 +124,37 @@ __device__ __forceinline__ i32x8_t mx_operand(const u32x4_t& lo, const u32x4_t& 
   return i32x8_t{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
 }
 
+// 16 words (64 B) of row data.
+__device__ __forceinline__ void mx_load_words(const void* p, uint32_t (&w)[16]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(reinterpret_cast<const unsigned char*>(p) + 16 * c);
+    w[4 * c] = v.x; w[4 * c + 1] = v.y; w[4 * c + 2] = v.z; w[4 * c + 3] = v.w;
+  }
+}
+
+// Hidden rows [T][H] -> packets [T][mx_row_bytes(H)], a thread per block
+// (i0, i0 + step, ...); blocks past H are zeros.
+template <int ACT>
+__device__ __forceinline__ void mx_quant_rows(const uint16_t* __restrict__ x, int T, int H, unsigned char* __restrict__ xq,
+                                              int64_t i0, int64_t step) {
+  const int nb = H >> 5, nbp = 4 * mx_ktiles(H);
+  const int64_t total = (int64_t)T * nbp;
+  for (int64_t i = i0; i < total; i += step) {
+    const int t = (int)(i / nbp), b = (int)(i - (int64_t)t * nbp);
+    MxPacket pk = {u32x4_t{0, 0, 0, 0}, u32x4_t{0, 0, 0, 0}};
+    if (b < nb) {
+      uint32_t w[16];
+      mx_load_words(x + (size_t)t * H + 32 * b, w);
+      const int s = mx_scale_byte<kMxFp6>(mx_amax16<ACT>(w));
+      pk = mx_packet(mx_fp6_codes16<ACT>(w, s), s);
+    }
+    u32x4_t* o = reinterpret_cast<u32x4_t*>(xq + i * kMxPacketBytes);
+    o[0] = pk.lo;
+    o[1] = pk.hi;
+  }
+}
+
 // D += W (16 rows x 128, E2M1) * X (128 x 16 columns, E2M3), fp32.  Lane
 // 16 q + r holds block q of row r of W and of column r of X, and rows
 // 4 q .. 4 q + 3 of D's column r.  T: the byte of ws that holds W's scale.

@@ -48,7 +48,7 @@ hipError_t launch_qint_gemm(const QArgs&, int, int, int, hipStream_t);
 hipError_t launch_quant_route(const void*, int, int64_t, int64_t, int8_t*, float*, const int32_t*, int, int, int,
                               const RouteGlobal&, hipStream_t, int);
 hipError_t launch_topk_softmax(const void*, int, int, int, int, int, int32_t*, float*, hipStream_t);
-hipError_t launch_topk_scores(const void*, int, const float*, const ScoreArgs&, int32_t*, float*, hipStream_t);
+hipError_t launch_topk_scores(const void*, int, const float*, ScoreArgs, int32_t*, float*, hipStream_t);
 hipError_t launch_route_mx(const void*, int, int, int, unsigned char*, const int32_t*, int, int, int, const RouteGlobal&,
                            hipStream_t, int);
 hipError_t launch_mx_sorted(const MxArgs&, int, int, hipStream_t, hipEvent_t);
@@ -912,7 +912,7 @@ MI_API int mi_moe_topk_scores(const void* logits, int logits_dtype, int64_t T, i
   if (T == 0) return MI_MOE_OK;
   if (!logits || !topk_ids || !topk_w) return fail(MI_MOE_EINVAL, "null pointer");
   const ScoreArgs a = {(int)T, (int)E, (int)K, score == MI_MOE_SCORE_SIGMOID, (int)n_group, (int)topk_group, (int)group_top,
-                       renormalize != 0, (double)scale};
+                       renormalize != 0, (double)scale, 0};
   HIPCHK(launch_topk_scores(logits, logits_dtype, bias, a, topk_ids, topk_w, (hipStream_t)stream));
   return MI_MOE_OK;
 }

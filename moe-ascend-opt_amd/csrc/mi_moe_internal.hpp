@@ -253,6 +253,7 @@ struct ScoreArgs {
   int n_group, topk_group, group_top;
   int renorm;
   double scale;
+  int group_lanes;             // lanes that hold a group, 0: not whole lanes (set by the launcher)
 };
 
 // ---------------------------------------------------------------- MXFP4 layer (mx.hip)

@@ -20,23 +20,59 @@ namespace {
 
 constexpr int kScoreWaves = 4;
 constexpr int kScoreMaxE = 512;
-constexpr int kScoreMaxGroups = 64;
 
-__device__ __forceinline__ double shfl_xor_f64(double v, int m) {
-  const int lo = __shfl_xor(__double2loint(v), m), hi = __shfl_xor(__double2hiint(v), m);
-  return __hiloint2double(hi, lo);
+// A lane's value from another lane of its row of 16 (DPP: no trip through
+// LDS).  In this order the four controls leave every lane with the result
+// over groups of 2, 4, 8 and 16 lanes.
+constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kHalfMirror = 0x141, kMirror = 0x140;
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, false));
 }
-__device__ __forceinline__ double shfl_f64(double v, int l) {
-  return __hiloint2double(__shfl(__double2hiint(v), l), __shfl(__double2loint(v), l));
+template <int CTRL>
+__device__ __forceinline__ double dpp(double v) {
+  return __hiloint2double(__builtin_amdgcn_mov_dpp(__double2hiint(v), CTRL, 0xf, 0xf, false),
+                          __builtin_amdgcn_mov_dpp(__double2loint(v), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float lane_value(float v, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); }
+__device__ __forceinline__ double lane_value(double v, int l) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), l), __builtin_amdgcn_readlane(__double2loint(v), l));
+}
+template <class T>
+__device__ __forceinline__ T larger(T a, T b) { return a > b ? a : b; }
+template <class T>
+__device__ __forceinline__ T wave_max(T v) {
+  v = larger(v, dpp<kXor1>(v));
+  v = larger(v, dpp<kXor2>(v));
+  v = larger(v, dpp<kHalfMirror>(v));
+  v = larger(v, dpp<kMirror>(v));
+  return larger(larger(lane_value(v, 0), lane_value(v, 16)), larger(lane_value(v, 32), lane_value(v, 48)));
 }
 __device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) v += shfl_xor_f64(v, m);
-  return v;
+  v += dpp<kXor1>(v);
+  v += dpp<kXor2>(v);
+  v += dpp<kHalfMirror>(v);
+  v += dpp<kMirror>(v);
+  return (lane_value(v, 0) + lane_value(v, 16)) + (lane_value(v, 32) + lane_value(v, 48));
 }
 
-// One wave per token; lane l holds experts l, l + 64, ...
-template <int LDT, int NJ>   // logits: 0 fp16, 1 bf16, 2 fp32; NJ = ceil(E / 64)
+// The two largest of two sets, from each one's two largest.
+struct Top2 {
+  double a, b;
+};
+__device__ __forceinline__ void merge(Top2& x, double a, double b) {
+  const double lo = x.a > a ? a : x.a;
+  x.a = larger(x.a, a);
+  x.b = larger(lo, larger(x.b, b));
+}
+
+// One wave per token; lane l holds experts l NJ .. l NJ + NJ - 1, so that the
+// lower of two experts is in the lower lane.
+//
+// A pick is the wave's largest choice: a maximum of the choices rounded to
+// fp32 (a rounding keeps the order, so the largest is among those that reach
+// it), and only where several lanes reach it the 64-bit one among them.
+template <int LDT, int NJ>   // logits: 0 fp16, 1 bf16, 2 fp32; NJ = ceil(E / 64), a power of two
 __global__ __launch_bounds__(kScoreWaves * kWave) void topk_scores_kernel(const void* __restrict__ logits, const float* __restrict__ bias,
                                                                           ScoreArgs a, int32_t* __restrict__ ids_out,
                                                                           float* __restrict__ w_out) {
@@ -45,27 +81,30 @@ __global__ __launch_bounds__(kScoreWaves * kWave) void topk_scores_kernel(const 
   const int t = blockIdx.x * kScoreWaves + wave;
   if (t >= a.T) return;   // whole wave; no workgroup barrier follows
   const double ninf = -__builtin_inf();
-  float l[NJ];
+  const int e0 = lane * NJ;
+  float l[NJ], b[NJ];
   double s[NJ], c[NJ];
-  bool nan = false;
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
-    const int e = lane + kWave * j;
-    const size_t off = (size_t)t * a.E + (e < a.E ? e : a.E - 1);
+    const int e = min(e0 + j, a.E - 1);
+    const size_t off = (size_t)t * a.E + e;
     float v;
     if constexpr (LDT == 2) v = reinterpret_cast<const float*>(logits)[off];
     else v = to_f32<LDT>(reinterpret_cast<const uint16_t*>(logits)[off]);
-    l[j] = e < a.E ? v : -__builtin_inff();
+    l[j] = v;
+    b[j] = bias ? bias[e] : 0.0f;
   }
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+    if (e0 + j >= a.E) l[j] = -__builtin_inff();
   if (a.sigmoid) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) s[j] = 1.0 / (1.0 + exp(-(double)l[j]));
   } else {
     float m = l[0];
 #pragma unroll
-    for (int j = 1; j < NJ; ++j) m = fmaxf(m, l[j]);
-#pragma unroll
-    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    for (int j = 1; j < NJ; ++j) m = larger(m, l[j]);   // a NaN shows in the scores
+    m = wave_max(m);
     if (m == -__builtin_inff()) m = 0.0f;   // every expert masked
     double sum = 0.0;
 #pragma unroll
@@ -74,13 +113,14 @@ __global__ __launch_bounds__(kScoreWaves * kWave) void topk_scores_kernel(const 
       sum += s[j];
     }
     sum = wave_sum(sum);
+    const double inv = 1.0 / sum;   // a sum of 0: every score is 0, and every expert masked
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) s[j] = sum == 0.0 ? 0.0 : s[j] / sum;
+    for (int j = 0; j < NJ; ++j) s[j] = sum == 0.0 ? 0.0 : s[j] * inv;
   }
+  bool nan = false;
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
-    const int e = lane + kWave * j;
-    c[j] = bias && e < a.E ? s[j] + (double)bias[e] : s[j];
+    c[j] = s[j] + (double)b[j];
     nan |= c[j] != c[j];
     if (l[j] == -__builtin_inff()) c[j] = ninf;   // masked, or past E
   }
@@ -93,51 +133,70 @@ __global__ __launch_bounds__(kScoreWaves * kWave) void topk_scores_kernel(const 
     }
     return;
   }
-  if (a.topk_group < a.n_group) {
+  if (a.topk_group < a.n_group) {   // uniform
     const int gs = a.E / a.n_group;
-    double* cw = cs[wave];
+    if (a.group_lanes) {
+      // a group is 1, 2, 4, 8 or 16 whole lanes of a row
+      Top2 x = {c[0], ninf};
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) cw[lane + kWave * j] = c[j];
-    __builtin_amdgcn_wave_barrier();
-    double b1 = ninf, b2 = ninf;   // the group's two largest
-    if (lane < a.n_group)
-      for (int i = 0; i < gs; ++i) {
-        const double v = cw[lane * gs + i];
-        if (v > b1) { b2 = b1; b1 = v; }
-        else if (v > b2) b2 = v;
+      for (int j = 1; j < NJ; ++j) merge(x, c[j], ninf);
+      if (a.group_lanes > 1) merge(x, dpp<kXor1>(x.a), dpp<kXor1>(x.b));
+      if (a.group_lanes > 2) merge(x, dpp<kXor2>(x.a), dpp<kXor2>(x.b));
+      if (a.group_lanes > 4) merge(x, dpp<kHalfMirror>(x.a), dpp<kHalfMirror>(x.b));
+      if (a.group_lanes > 8) merge(x, dpp<kMirror>(x.a), dpp<kMirror>(x.b));
+      const double g = a.group_top == 1 ? x.a : x.b == ninf ? ninf : x.a + x.b;
+      const int mine = lane / a.group_lanes;
+      int ahead = 0;   // groups that come before this lane's
+      for (int i = 0; i < a.n_group; ++i) {
+        const double o = lane_value(g, i * a.group_lanes);
+        ahead += o > g || (o == g && i < mine);
       }
-    const double g = a.group_top == 1 ? b1 : b2 == ninf ? ninf : b1 + b2;
-    int ahead = 0;   // groups that come before this lane's
-    for (int i = 0; i < a.n_group; ++i) {
-      const double o = shfl_f64(g, i);
-      ahead += o > g || (o == g && i < lane);
-    }
-    const uint64_t open = __ballot(lane < a.n_group && ahead < a.topk_group);
+      if (ahead >= a.topk_group)
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const int e = lane + kWave * j;
-      if (e < a.E && !((open >> (e / gs)) & 1)) c[j] = ninf;
+        for (int j = 0; j < NJ; ++j) c[j] = ninf;
+    } else {
+      // any other size: a lane goes through its group in LDS
+      double* cw = cs[wave];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) cw[e0 + j] = c[j];
+      __builtin_amdgcn_wave_barrier();
+      Top2 x = {ninf, ninf};
+      if (lane < a.n_group)
+        for (int i = 0; i < gs; ++i) merge(x, cw[lane * gs + i], ninf);
+      const double g = a.group_top == 1 ? x.a : x.b == ninf ? ninf : x.a + x.b;
+      int ahead = 0;
+      for (int i = 0; i < a.n_group; ++i) {
+        const double o = lane_value(g, i);
+        ahead += o > g || (o == g && i < lane);
+      }
+      const uint64_t open = __ballot(lane < a.n_group && ahead < a.topk_group);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+        if (e0 + j < a.E && !((open >> ((e0 + j) / gs)) & 1)) c[j] = ninf;
     }
   }
   double mys = 0.0;
   int myid = -1;
   for (int k = 0; k < a.K; ++k) {
-    double bv = ninf, bs = 0.0;
-    int bi = 0x7fffffff;
+    double bv = c[0], bs = s[0];
+    int bi = e0;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
-      if (c[j] > bv) { bv = c[j]; bs = s[j]; bi = lane + kWave * j; }
-#pragma unroll
-    for (int m = 32; m; m >>= 1) {
-      const double ov = shfl_xor_f64(bv, m), os = shfl_xor_f64(bs, m);
-      const int oi = __shfl_xor(bi, m);
-      if (ov > bv || (ov == bv && oi < bi)) { bv = ov; bs = os; bi = oi; }
+    for (int j = 1; j < NJ; ++j)
+      if (c[j] > bv) { bv = c[j]; bs = s[j]; bi = e0 + j; }
+    const float bf = (float)bv, m = wave_max(bf);
+    if (m == -__builtin_inff()) break;   // uniform: only masked experts are left
+    uint64_t at = __ballot(bf == m);
+    if (at & (at - 1)) {   // uniform
+      const double top = wave_max(bf == m ? bv : ninf);
+      at = __ballot(bv == top);
     }
-    if (bi == 0x7fffffff) break;   // uniform: only masked experts are left
+    const int w = __ffsll((long long)at) - 1;
+    const int id = __builtin_amdgcn_readlane(bi, w);
+    const double ps = lane_value(bs, w);
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
-      if (bi == lane + kWave * j) c[j] = ninf;
-    if (lane == k) { mys = bs; myid = bi; }
+      if (e0 + j == id) c[j] = ninf;
+    if (lane == k) { mys = ps; myid = id; }
   }
   const double sum = wave_sum(lane < a.K ? mys : 0.0);
   if (a.renorm) mys = sum > 0.0 ? mys / sum : 0.0;
@@ -158,9 +217,12 @@ void launch_t(const void* logits, const float* bias, const ScoreArgs& a, int32_t
 
 }  // namespace
 
-hipError_t launch_topk_scores(const void* logits, int ldt, const float* bias, const ScoreArgs& a, int32_t* ids, float* w,
+hipError_t launch_topk_scores(const void* logits, int ldt, const float* bias, ScoreArgs a, int32_t* ids, float* w,
                               hipStream_t st) {
   if (a.T == 0) return hipSuccess;
+  if (a.E > kScoreMaxE) return hipErrorInvalidValue;
+  const int nj = a.E <= 64 ? 1 : a.E <= 128 ? 2 : a.E <= 256 ? 4 : 8, gs = a.E / a.n_group, gl = gs / nj;
+  a.group_lanes = gs % nj == 0 && gl <= 16 && (gl & (gl - 1)) == 0 ? gl : 0;
   if (ldt == 2) launch_t<2>(logits, bias, a, ids, w, st);
   else if (ldt == 1) launch_t<1>(logits, bias, a, ids, w, st);
   else launch_t<0>(logits, bias, a, ids, w, st);

@@ -38,8 +38,45 @@ __device__ __forceinline__ float lane_value(float v, int l) { return __int_as_fl
 __device__ __forceinline__ double lane_value(double v, int l) {
   return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), l), __builtin_amdgcn_readlane(__double2loint(v), l));
 }
-template <class T>
-__device__ __forceinline__ T larger(T a, T b) { return a > b ? a : b; }
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_fmaxf(a, b); }
+__device__ __forceinline__ double larger(double a, double b) { return __builtin_fmax(a, b); }
+
+// exp(x) for x <= 0, in 64 bits: x = n log 2 + r, |r| <= log(2) / 2, the
+// Taylor series of exp(r) to r^13 (4e-18 left), scaled by 2^n.  NaN stays NaN.
+__device__ __forceinline__ double exp_neg(double x) {
+  x = x < -750.0 ? -750.0 : x;   // 0 after the scaling
+  const double n = __builtin_rint(x * 1.4426950408889634);
+  double r = __builtin_fma(n, -0x1.62e42fefa0000p-1, x);   // log 2 in two parts: n times the first, of 36 bits, is exact
+  r = __builtin_fma(n, -0x1.cf79abc9e3b3ap-40, r);
+  double p = 1.0 / 6227020800.0;
+  p = __builtin_fma(p, r, 1.0 / 479001600.0);
+  p = __builtin_fma(p, r, 1.0 / 39916800.0);
+  p = __builtin_fma(p, r, 1.0 / 3628800.0);
+  p = __builtin_fma(p, r, 1.0 / 362880.0);
+  p = __builtin_fma(p, r, 1.0 / 40320.0);
+  p = __builtin_fma(p, r, 1.0 / 5040.0);
+  p = __builtin_fma(p, r, 1.0 / 720.0);
+  p = __builtin_fma(p, r, 1.0 / 120.0);
+  p = __builtin_fma(p, r, 1.0 / 24.0);
+  p = __builtin_fma(p, r, 1.0 / 6.0);
+  p = __builtin_fma(p, r, 0.5);
+  p = __builtin_fma(p, r, 1.0);
+  p = __builtin_fma(p, r, 1.0);
+  return __builtin_amdgcn_ldexp(p, (int)n);
+}
+// 1 / x for 1 <= x <= 2 or any other x of ordinary size: the hardware's
+// estimate and two Newton steps.
+__device__ __forceinline__ double reciprocal(double x) {
+  double y = __builtin_amdgcn_rcp(x);
+  y = __builtin_fma(__builtin_fma(-x, y, 1.0), y, y);
+  return __builtin_fma(__builtin_fma(-x, y, 1.0), y, y);
+}
+// 1 / (1 + exp(-l)), from the exponential of -|l|, which cannot overflow
+__device__ __forceinline__ double sigmoid(float l) {
+  const double e = exp_neg(-__builtin_fabs((double)l)), y = reciprocal(1.0 + e);
+  return l < 0.0f ? e * y : y;
+}
+
 template <class T>
 __device__ __forceinline__ T wave_max(T v) {
   v = larger(v, dpp<kXor1>(v));
@@ -61,7 +98,7 @@ struct Top2 {
   double a, b;
 };
 __device__ __forceinline__ void merge(Top2& x, double a, double b) {
-  const double lo = x.a > a ? a : x.a;
+  const double lo = __builtin_fmin(x.a, a);
   x.a = larger(x.a, a);
   x.b = larger(lo, larger(x.b, b));
 }
@@ -69,9 +106,9 @@ __device__ __forceinline__ void merge(Top2& x, double a, double b) {
 // One wave per token; lane l holds experts l NJ .. l NJ + NJ - 1, so that the
 // lower of two experts is in the lower lane.
 //
-// A pick is the wave's largest choice: a maximum of the choices rounded to
-// fp32 (a rounding keeps the order, so the largest is among those that reach
-// it), and only where several lanes reach it the 64-bit one among them.
+// A pick is the largest choice: found as a maximum of the choices rounded to
+// fp32 (rounding keeps the order, so the largest is among those that reach
+// it), and only where several experts reach it in 64 bits among them.
 template <int LDT, int NJ>   // logits: 0 fp16, 1 bf16, 2 fp32; NJ = ceil(E / 64), a power of two
 __global__ __launch_bounds__(kScoreWaves * kWave) void topk_scores_kernel(const void* __restrict__ logits, const float* __restrict__ bias,
                                                                           ScoreArgs a, int32_t* __restrict__ ids_out,
@@ -99,21 +136,21 @@ __global__ __launch_bounds__(kScoreWaves * kWave) void topk_scores_kernel(const 
     if (e0 + j >= a.E) l[j] = -__builtin_inff();
   if (a.sigmoid) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) s[j] = 1.0 / (1.0 + exp(-(double)l[j]));
+    for (int j = 0; j < NJ; ++j) s[j] = sigmoid(l[j]);
   } else {
     float m = l[0];
 #pragma unroll
-    for (int j = 1; j < NJ; ++j) m = larger(m, l[j]);   // a NaN shows in the scores
+    for (int j = 1; j < NJ; ++j) m = larger(m, l[j]);   // drops NaN, which shows in the scores
     m = wave_max(m);
     if (m == -__builtin_inff()) m = 0.0f;   // every expert masked
     double sum = 0.0;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-      s[j] = exp((double)l[j] - (double)m);
+      s[j] = exp_neg((double)l[j] - (double)m);
       sum += s[j];
     }
     sum = wave_sum(sum);
-    const double inv = 1.0 / sum;   // a sum of 0: every score is 0, and every expert masked
+    const double inv = reciprocal(sum);   // 1 <= sum <= E; a sum of 0: every score is 0, and every expert masked
 #pragma unroll
     for (int j = 0; j < NJ; ++j) s[j] = sum == 0.0 ? 0.0 : s[j] * inv;
   }
@@ -175,28 +212,48 @@ __global__ __launch_bounds__(kScoreWaves * kWave) void topk_scores_kernel(const 
         if (e0 + j < a.E && !((open >> ((e0 + j) / gs)) & 1)) c[j] = ninf;
     }
   }
-  double mys = 0.0;
+  float f[NJ];   // the choices left, rounded to fp32
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) f[j] = (float)c[j];
   int myid = -1;
   for (int k = 0; k < a.K; ++k) {
-    double bv = c[0], bs = s[0];
-    int bi = e0;
+    float m = f[0];
 #pragma unroll
-    for (int j = 1; j < NJ; ++j)
-      if (c[j] > bv) { bv = c[j]; bs = s[j]; bi = e0 + j; }
-    const float bf = (float)bv, m = wave_max(bf);
+    for (int j = 1; j < NJ; ++j) m = larger(m, f[j]);
+    m = wave_max(m);
     if (m == -__builtin_inff()) break;   // uniform: only masked experts are left
-    uint64_t at = __ballot(bf == m);
-    if (at & (at - 1)) {   // uniform
-      const double top = wave_max(bf == m ? bv : ninf);
-      at = __ballot(bv == top);
+    int reach = 0, id = 0;               // experts that reach it, and the (one) expert
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const uint64_t at = __ballot(f[j] == m);
+      reach += __popcll(at);
+      if (at) id = (__ffsll((long long)at) - 1) * NJ + j;   // uniform
     }
-    const int w = __ffsll((long long)at) - 1;
-    const int id = __builtin_amdgcn_readlane(bi, w);
-    const double ps = lane_value(bs, w);
+    if (reach > 1) {   // uniform: the 64-bit choices decide, then the lower expert
+      double top = ninf;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) top = f[j] == m ? larger(top, c[j]) : top;
+      top = wave_max(top);
+      id = kScoreMaxE;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const uint64_t at = __ballot(f[j] == m && c[j] == top);
+        const int lo = at ? (__ffsll((long long)at) - 1) * NJ + j : kScoreMaxE;
+        id = lo < id ? lo : id;
+      }
+    }
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
-      if (e0 + j == id) c[j] = ninf;
-    if (lane == k) { mys = ps; myid = id; }
+      if (e0 + j == id) f[j] = -__builtin_inff();
+    if (lane == k) myid = id;
+  }
+  // lane k fetches the score of pick k
+  double mys = 0.0;
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    const int from = myid < 0 ? 0 : myid / NJ;
+    const double v = __hiloint2double(__shfl(__double2hiint(s[j]), from), __shfl(__double2loint(s[j]), from));
+    if (myid >= 0 && myid % NJ == j) mys = v;
   }
   const double sum = wave_sum(lane < a.K ? mys : 0.0);
   if (a.renorm) mys = sum > 0.0 ? mys / sum : 0.0;

@@ -273,8 +273,11 @@ constexpr int kMxPacketBytes = 32;        // an activation block: 24 B of codes,
 __host__ __device__ constexpr size_t mx_row_bytes(int K) { return (size_t)mx_ktiles(K) * 4 * kMxPacketBytes; }
 
 // Rows per expert on average from which the grouped products (mx.hip) take
-// items of 128 rows.
-constexpr int kMxBigRows = 96;
+// items of 128 rows.  us a call, 64-row / 128-row items, H=2048 I=768 E=128
+// top-8: 9 rows 75 / 79, 16 rows 78 / 81, 32 rows 103 / 88, 94 rows 147 / 124;
+// 12 rows Zipf-routed 86 / 78; H=4096 I=768 E=16 top-2: 11 rows 32 / 33,
+// Zipf-routed 55 / 37 (an expert's many rows read its weights half as often).
+constexpr int kMxBigRows = 10;
 inline bool mx_big(int64_t n, int64_t E) { return n >= kMxBigRows * E; }
 
 struct MxArgs {

@@ -3,11 +3,10 @@
 // combine in the down product.
 //
 // gate_up item (pair, slice of 32 rows of I): serves its expert iff the pair
-// is the expert's first (wave ballots over all ids).  The 8 waves split K.  A
-// lane of the matrix operand holds one whole block of one token, so it loads
-// the 32 hidden values, finds their scale and converts them in registers,
-// while the weights are on their way; nothing is staged.  The waves' sums
-// meet in LDS, and one lane per token makes the slice's MXFP6 block.
+// is the expert's first (wave ballots over all ids).  The 8 waves split K.
+// While the weights are on their way to registers, the tokens' rows are
+// quantized into LDS, a lane per block.  The waves' sums meet in LDS, and one
+// lane per token makes the slice's MXFP6 block.
 //
 // down item (token, 16 rows of H): wave k takes routed expert k over all of
 // I; y = cast(sum_k w_k out_k) in k order.
@@ -30,18 +29,34 @@ constexpr int kUnitsPerBlock = 8;
 constexpr int kUnitBatch = 4;        // units per lane loaded together by a down wave
 constexpr int kRedBytes = kDecWaves * 4 * 64 * 16;   // partial sums [wave][tile][lane][4]
 constexpr int kHiddenStride = 33;    // floats of a token's slice in LDS
-constexpr int kGateUpLds = kRedBytes + 16 * kHiddenStride * 4;
 
+// Keeps loads in the order they are written in.
+__device__ __forceinline__ void issue_order_fence() { asm volatile("" ::: "memory"); }
 __device__ __forceinline__ u32x4_t ld16(const void* p) { return *reinterpret_cast<const u32x4_t*>(p); }
 __device__ __forceinline__ void st16(void* p, const u32x4_t& v) { *reinterpret_cast<u32x4_t*>(p) = v; }
 
 // ---------------------------------------------------------------- gate_up
-// NB: k tiles whose loads a wave issues together.
+// The columns (tokens of the expert) of a pass lie in LDS as packets, 16
+// bytes apart from whole lines, so that 16 columns' packets of one block
+// spread over the banks.  As many at a time as fit beside nothing (at least
+// one, at most the matrix operand's 16).
+__host__ __device__ inline int col_bytes(int H) { return (int)mx_row_bytes(H) + 16; }
+__host__ __device__ inline int pass_cols(int H) {
+  const int p = kRedBytes / col_bytes(H);
+  return p < 1 ? 1 : p > 16 ? 16 : p;
+}
+// packets, then (the same memory) the partial sums; the slice's values
+__host__ __device__ inline int gate_up_lds(int H) {
+  const int p = pass_cols(H) * col_bytes(H);
+  return (p > kRedBytes ? p : kRedBytes) + 16 * kHiddenStride * 4;
+}
+
+// NB: k tiles whose weights a wave has on their way together.
 template <int ACT, int NB, bool FUSED>
 __device__ __forceinline__ void gate_up_item(const MxArgs& a, int item, int js, unsigned char* smem) {
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int q = lane >> 4, r = lane & 15;
-  const int NS = a.I >> 5, kt = mx_ktiles(a.H), nb = a.H >> 5;
+  const int NS = a.I >> 5, kt = mx_ktiles(a.H), nb = a.H >> 5, cb = col_bytes(a.H), P = pass_cols(a.H);
   SchedArgs c;
   c.ids = a.ids; c.n = a.n; c.E = a.E;
   const BallotCols cl = ballot_cols(c, item, lane);
@@ -53,43 +68,63 @@ __device__ __forceinline__ void gate_up_item(const MxArgs& a, int item, int js, 
   const unsigned char* ws = a.w13_s + unit * kMxTileScaleBytes + lane * 4;
   const int k0 = kt * wave / kDecWaves, k1 = kt * (wave + 1) / kDecWaves;
   f32x4_t* red = reinterpret_cast<f32x4_t*>(smem);
-  float* hid = reinterpret_cast<float*>(smem + kRedBytes);
-  for (int c0 = 0; c0 < cnt; c0 += 16) {
-    const int ncol = min(16, cnt - c0);
-    const int pair = __shfl(cl.colpair, c0 + min(r, ncol - 1));
-    const uint16_t* x = a.x + (size_t)div_small(pair, rk) * a.H;
-    f32x4_t acc[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) acc[t] = f32x4_t{0, 0, 0, 0};
-    for (int kb = k0; kb < k1; kb += NB) {
-      u32x4_t wv[NB][4];
-      uint32_t sc[NB], xv[NB][16];
+  float* hid = reinterpret_cast<float*>(smem + gate_up_lds(a.H) - 16 * kHiddenStride * 4);
+  for (int c0 = 0; c0 < cnt; c0 += P) {
+    const int ncol = min(P, cnt - c0);
+    u32x4_t wv[NB][4];
+    uint32_t sc[NB];
+    auto weights = [&](int kb) {
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        const int k = min(kb + i, k1 - 1);
+        const int k = max(min(kb + i, k1 - 1), 0);
 #pragma unroll
         for (int t = 0; t < 4; ++t) wv[i][t] = ld16(w + (size_t)k * kMxTileBytes + t * 1024);
         sc[i] = *reinterpret_cast<const uint32_t*>(ws + (size_t)k * kMxTileScaleBytes);
-        const uint16_t* p = x + 32 * min(4 * k + q, nb - 1);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const u32x4_t v = ld16(p + 8 * j);
-          xv[i][4 * j] = v.x; xv[i][4 * j + 1] = v.y; xv[i][4 * j + 2] = v.z; xv[i][4 * j + 3] = v.w;
-        }
       }
+    };
+    // The hidden rows: a wave takes a column, a lane a block.  The first
+    // blocks' loads go out before the weights' (loads return in order), which
+    // are on their way during the quantization.
+    uint32_t xv[16];
+    auto row = [&](int col) { return a.x + (size_t)div_small(__shfl(cl.colpair, c0 + col), rk) * a.H; };
+    if (wave < ncol) mx_load_words(row(wave) + 32 * min(lane, nb - 1), xv);   // uniform
+    issue_order_fence();
+    weights(k0);
+    issue_order_fence();
+    for (int col = wave; col < ncol; col += kDecWaves) {   // uniform
+      const uint16_t* x = row(col);
+      for (int b = lane; b < 4 * kt; b += 64) {
+        if (col != wave || b != lane) mx_load_words(x + 32 * min(b, nb - 1), xv);
+        MxPacket pk = {u32x4_t{0, 0, 0, 0}, u32x4_t{0, 0, 0, 0}};   // past H
+        if (b < nb) {
+          const int s = mx_scale_byte<kMxFp6>(mx_amax16<ACT>(xv));
+          pk = mx_packet(mx_fp6_codes16<ACT>(xv, s), s);
+        }
+        st16(smem + col * cb + b * kMxPacketBytes, pk.lo);
+        st16(smem + col * cb + b * kMxPacketBytes + 16, pk.hi);
+      }
+    }
+    __syncthreads();
+    f32x4_t acc[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) acc[t] = f32x4_t{0, 0, 0, 0};
+    const unsigned char* cp = smem + min(r, ncol - 1) * cb + q * kMxPacketBytes;
+    for (int kb = k0; kb < k1; kb += NB) {
+      if (kb > k0) weights(kb);
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         if (kb + i < k1) {   // uniform
-          const int s = mx_scale_byte<kMxFp6>(mx_amax16<ACT>(xv[i]));
-          MxPacket pk = mx_packet(mx_fp6_codes16<ACT>(xv[i], s), s);
-          if (4 * (kb + i) + q >= nb) pk = MxPacket{u32x4_t{0, 0, 0, 0}, u32x4_t{0, 0, 0, 0}};   // past H
-          acc[0] = mx_mfma<0>(wv[i][0], sc[i], pk.lo, pk.hi, acc[0]);
-          acc[1] = mx_mfma<1>(wv[i][1], sc[i], pk.lo, pk.hi, acc[1]);
-          acc[2] = mx_mfma<2>(wv[i][2], sc[i], pk.lo, pk.hi, acc[2]);
-          acc[3] = mx_mfma<3>(wv[i][3], sc[i], pk.lo, pk.hi, acc[3]);
+          const unsigned char* p = cp + (kb + i) * 4 * kMxPacketBytes;
+          const u32x4_t lo = ld16(p), hi = ld16(p + 16);
+          acc[0] = mx_mfma<0>(wv[i][0], sc[i], lo, hi, acc[0]);
+          acc[1] = mx_mfma<1>(wv[i][1], sc[i], lo, hi, acc[1]);
+          acc[2] = mx_mfma<2>(wv[i][2], sc[i], lo, hi, acc[2]);
+          acc[3] = mx_mfma<3>(wv[i][3], sc[i], lo, hi, acc[3]);
         }
       }
     }
+    const int pair = __shfl(cl.colpair, c0 + min(lane, ncol - 1));   // of column lane
+    __syncthreads();   // the packets are read: the sums take their place
 #pragma unroll
     for (int t = 0; t < 4; ++t) red[(wave * 4 + t) * 64 + lane] = acc[t];
     __syncthreads();
@@ -123,9 +158,9 @@ __device__ __forceinline__ void gate_up_item(const MxArgs& a, int item, int js, 
         st16(o + 16, pk.hi);
       }
     }
-    // the next pass writes red after every wave has read it (the barrier
-    // above) and hid after its own first barrier, which wave 0 reaches only
-    // with its reads of hid done
+    // The next pass's packets take the place of the sums, which are read (the
+    // barrier above); hid is written again behind two more barriers, which
+    // wave 0 reaches with its reads of it done.
   }
 }
 
@@ -272,12 +307,12 @@ template <int ACT, int NB1, int NB2>
 hipError_t launch_decode_t(const MxArgs& a, hipStream_t st, hipEvent_t mid) {
   const int NS = a.I >> 5, nt = a.H >> 4;
   if (mx_decode_fused(a.n, a.K, a.I)) {
-    const size_t dl = down_lds(a.K, a.I, true), lds = dl > kGateUpLds ? dl : kGateUpLds;
+    const size_t dl = down_lds(a.K, a.I, true), gl = gate_up_lds(a.H), lds = dl > gl ? dl : gl;
     hipLaunchKernelGGL((mx_decode_kernel<ACT, NB1, NB2>), dim3(a.n * NS + a.T * nt), dim3(kDecWaves * kWave), lds, st,
                        a.ids, a.x, a.w13, a.w13_s, a.w2, a.w2_s, a.n * NS, NS, a);
     return hipGetLastError();
   }
-  hipLaunchKernelGGL((mx_gate_up_kernel<ACT, NB1>), dim3(NS, a.n), dim3(kDecWaves * kWave), kGateUpLds, st, a.ids, a.x,
+  hipLaunchKernelGGL((mx_gate_up_kernel<ACT, NB1>), dim3(NS, a.n), dim3(kDecWaves * kWave), gate_up_lds(a.H), st, a.ids, a.x,
                      a.w13, a.w13_s, a);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;

@@ -475,7 +475,7 @@ int mx_alloc_weights(mi_moe_handle* h) {
 int forward_mx(mi_moe_handle* h, const void* x, void* y, const float* tw, const int32_t* ids, int64_t T, int64_t K,
                int act, bool noalloc, hipStream_t st) {
   const int64_t n = T * K;
-  const bool decode = mx_decode_ok(n, K), fused = mx_decode_fused(n, K, (int)h->I);
+  const bool decode = mx_decode_ok(n, K, h->E, h->H, h->I), fused = decode && mx_decode_fused(K, h->I);
   Work w;
   const int rc = get_work(h, T, n, !decode, noalloc, st, w);
   if (rc) return rc;

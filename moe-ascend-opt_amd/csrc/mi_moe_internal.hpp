@@ -301,7 +301,15 @@ struct MxArgs {
 // Decode calls (mx_decode.hip): up to 64 routed pairs (a wave's ballot), a
 // wave of the down workgroup per routed expert; in one launch where its
 // workgroups' 8 waves hold the top-k and the handle has a hand-over buffer.
-inline bool mx_decode_ok(int64_t n, int64_t K) { return n <= 64 && K <= 16; }
-inline bool mx_decode_fused(int64_t n, int64_t K, int I) { return mx_decode_ok(n, K) && K <= 8 && I <= kTagActMaxI; }
+// A token's down workgroups read their experts' weights for themselves, the
+// sorted path reads an expert's once: with more pairs than experts the bytes
+// read again decide.  us a call, decode / sorted: H=4096 I=1408 E=16 top-2,
+// 32 pairs (49 MB read again) 50 / 53, 64 pairs (147 MB) 81 / 54; H=2048 I=768
+// E=16 top-4, 64 pairs (40 MB) 20 / 25; E=128 top-8, 64 pairs (0) 31 / 43.
+constexpr int64_t kMxDecodeAgain = 64 << 20;
+inline bool mx_decode_ok(int64_t n, int64_t K, int64_t E, int64_t H, int64_t I) {
+  return n <= 64 && K <= 16 && (n <= E || (n - E) * (H * I / 32 * 17) <= kMxDecodeAgain);
+}
+inline bool mx_decode_fused(int64_t K, int64_t I) { return K <= 8 && I <= kTagActMaxI; }
 
 }  // namespace mimoe

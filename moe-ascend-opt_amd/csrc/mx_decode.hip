@@ -306,7 +306,7 @@ __global__ __launch_bounds__(kMaxDecodeK * kWave) void mx_down_kernel(const int3
 template <int ACT, int NB1, int NB2>
 hipError_t launch_decode_t(const MxArgs& a, hipStream_t st, hipEvent_t mid) {
   const int NS = a.I >> 5, nt = a.H >> 4;
-  if (mx_decode_fused(a.n, a.K, a.I)) {
+  if (mx_decode_fused(a.K, a.I)) {
     const size_t dl = down_lds(a.K, a.I, true), gl = gate_up_lds(a.H), lds = dl > gl ? dl : gl;
     hipLaunchKernelGGL((mx_decode_kernel<ACT, NB1, NB2>), dim3(a.n * NS + a.T * nt), dim3(kDecWaves * kWave), lds, st,
                        a.ids, a.x, a.w13, a.w13_s, a.w2, a.w2_s, a.n * NS, NS, a);
@@ -327,7 +327,7 @@ hipError_t launch_decode_t(const MxArgs& a, hipStream_t st, hipEvent_t mid) {
 // Decode calls: a.tact for the one-launch form (mx_decode_fused), a.act ([n]
 // rows, row = pair) for the other.
 hipError_t launch_mx_decode(const MxArgs& a, int act, hipStream_t st, hipEvent_t mid) {
-  if (!mx_decode_ok(a.n, a.K)) return hipErrorInvalidValue;
+  if (!mx_decode_ok(a.n, a.K, a.E, a.H, a.I)) return hipErrorInvalidValue;
   const int nb2 = mx_ktiles(a.I) <= 2 ? 2 : mx_ktiles(a.I) <= 4 ? 4 : 6;
   if (act == 1)
     return nb2 == 2 ? launch_decode_t<1, 2, 2>(a, st, mid) : nb2 == 4 ? launch_decode_t<1, 2, 4>(a, st, mid) : launch_decode_t<1, 2, 6>(a, st, mid);

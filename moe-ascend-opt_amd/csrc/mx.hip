@@ -9,6 +9,7 @@
 // and run at the 4-bit rate, and its noise (2.8% of a Gaussian block, 2.6%
 // for E4M3) stays far below that of the 4-bit weights (11%).
 #pragma clang fp contract(off)
+#include <algorithm>
 #include <type_traits>
 
 #include "mx_device.hpp"
@@ -284,14 +285,16 @@ __global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(2)))
 }
 
 // y[t,h] = cast(sum_k w[t,k] eout[t*K+k,h]) over the valid ids in k order, in
-// fp32; a token without a valid id gets 0.  One thread per (t, 8 columns).
+// fp32; a token without a valid id gets 0.  A workgroup takes (part of) a
+// token, a thread 8 columns.
+constexpr int kMxCombineThreads = 256;
 template <int ACT>
-__global__ void mx_combine_kernel(const int16_t* __restrict__ eout, const unsigned char* __restrict__ eout_d, const float* __restrict__ tw,
-                                  const int32_t* __restrict__ ids, uint16_t* __restrict__ y, int T, int K, int E, int H) {
-  const int HV = H >> 3, NQ = H >> 6;
-  const int64_t total = (int64_t)T * HV;
-  for (int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; idx < total; idx += (int64_t)gridDim.x * blockDim.x) {
-    const int t = (int)(idx / HV), h = (int)(idx - (int64_t)t * HV) * 8;
+__global__ __launch_bounds__(kMxCombineThreads) void mx_combine_kernel(const int16_t* __restrict__ eout, const unsigned char* __restrict__ eout_d,
+                                                                       const float* __restrict__ tw, const int32_t* __restrict__ ids,
+                                                                       uint16_t* __restrict__ y, int T, int parts, int K, int E, int H) {
+  for (unsigned b = blockIdx.x; b < (unsigned)T * parts; b += gridDim.x) {
+    const int t = b / parts, h = ((b - t * parts) * kMxCombineThreads + threadIdx.x) * 8;
+    if (h >= H) continue;
     float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     constexpr int kB = 8;   // pairs whose loads are issued together
     for (int k0 = 0; k0 < K; k0 += kB) {
@@ -301,15 +304,15 @@ __global__ void mx_combine_kernel(const int16_t* __restrict__ eout, const unsign
       u32x4_t rv[kB];
 #pragma unroll
       for (int j = 0; j < kB; ++j) {
-        const int i = t * K + min(k0 + j, K - 1);
+        const size_t i = (size_t)t * K + min(k0 + j, K - 1);
         ev[j] = k0 + j < K ? ids[i] : -1;
         wv[j] = tw[i];
-        dv[j] = eout_d[(size_t)i * NQ * 4 + (h >> 4)];
-        rv[j] = ld16(eout + (size_t)i * H + h);
+        dv[j] = eout_d[i * (H >> 4) + (h >> 4)];
+        rv[j] = ld16(eout + i * H + h);
       }
 #pragma unroll
       for (int j = 0; j < kB; ++j) {
-        if ((unsigned)ev[j] >= (unsigned)E) continue;
+        if ((unsigned)ev[j] >= (unsigned)E) continue;   // uniform
         const uint32_t u[4] = {rv[j].x, rv[j].y, rv[j].z, rv[j].w};
         const float d = eout_scale(dv[j]);
 #pragma unroll
@@ -322,8 +325,7 @@ __global__ void mx_combine_kernel(const int16_t* __restrict__ eout, const unsign
     }
     uint32_t o[4];
 #pragma unroll
-    for (int p = 0; p < 4; ++p)
-      o[p] = from_f32<ACT>(acc[2 * p]) | ((uint32_t)from_f32<ACT>(acc[2 * p + 1]) << 16);
+    for (int p = 0; p < 4; ++p) o[p] = from_f32<ACT>(acc[2 * p]) | ((uint32_t)from_f32<ACT>(acc[2 * p + 1]) << 16);
     st16(y + (size_t)t * H + h, u32x4_t{o[0], o[1], o[2], o[3]});
   }
 }
@@ -474,11 +476,10 @@ hipError_t launch_mx_sorted(const MxArgs& a, int act, int tiles_max, hipStream_t
   else hipLaunchKernelGGL(mx_gemm_kernel<true>, dim3(tg * b2), dim3(kMxThreads), 0, st, a);
   err = hipGetLastError();
   if (err != hipSuccess) return err;
-  const unsigned g = blocks_for((int64_t)a.T * (a.H >> 3));
-  if (act == 1)
-    hipLaunchKernelGGL(mx_combine_kernel<1>, dim3(g), dim3(256), 0, st, a.eout, a.eout_d, a.tw, a.ids, a.y, a.T, a.K, a.E, a.H);
-  else
-    hipLaunchKernelGGL(mx_combine_kernel<0>, dim3(g), dim3(256), 0, st, a.eout, a.eout_d, a.tw, a.ids, a.y, a.T, a.K, a.E, a.H);
+  const int parts = ((a.H >> 3) + kMxCombineThreads - 1) / kMxCombineThreads;   // at most 32: T parts < 2^30
+  auto kern = act == 1 ? mx_combine_kernel<1> : mx_combine_kernel<0>;
+  const unsigned g = (unsigned)std::min<int64_t>((int64_t)a.T * parts, 1 << 20);
+  hipLaunchKernelGGL(kern, dim3(g), dim3(kMxCombineThreads), 0, st, a.eout, a.eout_d, a.tw, a.ids, a.y, a.T, parts, a.K, a.E, a.H);
   return hipGetLastError();
 }
 

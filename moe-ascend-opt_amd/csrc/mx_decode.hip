@@ -308,10 +308,16 @@ hipError_t launch_decode_t(const MxArgs& a, hipStream_t st, hipEvent_t mid) {
   const int NS = a.I >> 5, nt = a.H >> 4;
   if (mx_decode_fused(a.K, a.I)) {
     const size_t dl = down_lds(a.K, a.I, true), gl = gate_up_lds(a.H), lds = dl > gl ? dl : gl;
+    if (lds > kMaxLds)   // H near its limit
+      (void)hipFuncSetAttribute(reinterpret_cast<const void*>(mx_decode_kernel<ACT, NB1, NB2>),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     hipLaunchKernelGGL((mx_decode_kernel<ACT, NB1, NB2>), dim3(a.n * NS + a.T * nt), dim3(kDecWaves * kWave), lds, st,
                        a.ids, a.x, a.w13, a.w13_s, a.w2, a.w2_s, a.n * NS, NS, a);
     return hipGetLastError();
   }
+  if (gate_up_lds(a.H) > (int)kMaxLds)
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(mx_gate_up_kernel<ACT, NB1>),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, gate_up_lds(a.H));
   hipLaunchKernelGGL((mx_gate_up_kernel<ACT, NB1>), dim3(NS, a.n), dim3(kDecWaves * kWave), gate_up_lds(a.H), st, a.ids, a.x,
                      a.w13, a.w13_s, a);
   hipError_t err = hipGetLastError();

@@ -111,6 +111,18 @@ def test_layer(cuda, E, H, I, T):
     _check(h, w13, w2, x, ids, tw, cuda)
 
 
+@pytest.mark.parametrize("E,H,I", [(1, 65536, 64), (2, 64, 65536), (2, 64, 4096), (2, 64, 4128), (2, 17472, 32)])
+@pytest.mark.parametrize("T,K", [(1, 1), (5, 2), (3, 9), (70, 2)])
+def test_layer_long_rows(cuda, E, H, I, T, K):
+    """The largest rows, and the largest and the next intermediate on either side of the one-launch decode kernel."""
+    h, w13, w2 = _handle(E, H, I, H + I, cuda)
+    g = torch.Generator().manual_seed(T)
+    ids = torch.randint(0, E, (T, K), generator=g, dtype=torch.int32)
+    tw = torch.rand(T, K, generator=g)
+    x = torch.randn(T, H, generator=g).to(torch.bfloat16)
+    _check(h, w13, w2, x, ids, tw, cuda)
+
+
 @pytest.mark.parametrize("K", [1, 8, 10, 16, 40, 64])
 @pytest.mark.parametrize("T", [1, 4, 9])
 def test_layer_top_k(cuda, K, T):

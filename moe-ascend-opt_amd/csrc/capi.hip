@@ -469,6 +469,7 @@ int mx_alloc_weights(mi_moe_handle* h) {
   HIPCHK(h->w2_s.alloc(t2 * kMxTileScaleBytes));
   // zeros stay where K is no multiple of 128, and in what has not been stored
   for (DevBuf* b : {&h->w13, &h->w13_s, &h->w2, &h->w2_s}) HIPCHK(hipMemset(b->p, 0, b->bytes));
+  HIPCHK(hipStreamSynchronize(nullptr));   // before the caller's stream, which may not wait for the default one
   return MI_MOE_OK;
 }
 

@@ -319,6 +319,7 @@ std::tuple<at::Tensor, at::Tensor> moe_topk_scores_hip(const at::Tensor& logits,
                                                        int64_t n_group, int64_t topk_group, int64_t group_top,
                                                        bool renormalize, double scale) {
   check_scores(logits, top_k);
+  TORCH_CHECK(logits.is_cuda(), "moe_topk_scores: bias and logits must be on one device");
   c10::hip::HIPGuard guard(logits.get_device());
   at::Tensor x = contig(logits), b = score_bias(bias, logits);
   const int64_t T = x.size(0), E = x.size(1);

@@ -76,11 +76,10 @@ template <int NSUB, class Row>
 __device__ __forceinline__ void mx_gemm_core(unsigned char* smem, Row row, int kt, const unsigned char* w, const unsigned char* ws,
                                              f32x4_t (&acc)[4][NSUB]) {
   constexpr int S = mx_step(NSUB), STRIDE = S * 128, BYTES = mx_stage_bytes(NSUB);
-  constexpr bool PART = BYTES < kMxThreads * 16;            // not every thread stages
-  constexpr int NP = PART ? 1 : BYTES / (kMxThreads * 16);  // pieces of a thread, STEP rows apart
-  constexpr int STEP = kMxThreads / (8 * S);
+  constexpr int NP = BYTES / (kMxThreads * 16), STEP = kMxThreads / (8 * S);   // pieces of a thread, STEP rows apart
+  static_assert(NP >= 1 && NP * STEP == 16 * NSUB, "every thread stages whole pieces");
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, r = lane & 15;
-  const int piece = tid % (8 * S), last = 8 * kt - 1, row0 = PART ? min(tid / (8 * S), 16 * NSUB - 1) : tid / (8 * S);
+  const int piece = tid % (8 * S), last = 8 * kt - 1, row0 = tid / (8 * S);
   const unsigned char* src[NP];
   int dst[NP];
 #pragma unroll
@@ -88,7 +87,6 @@ __device__ __forceinline__ void mx_gemm_core(unsigned char* smem, Row row, int k
     src[p] = row(row0 + STEP * p);
     dst[p] = (row0 + STEP * p) * STRIDE + ((piece ^ ((row0 + STEP * p) & 15)) << 4);
   }
-  const bool stager = !PART || tid < BYTES / 16;
   u32x4_t sv[NP], wv[S][4];
   uint32_t sc[S];
   auto stage_load = [&](int c) {
@@ -97,9 +95,8 @@ __device__ __forceinline__ void mx_gemm_core(unsigned char* smem, Row row, int k
     for (int p = 0; p < NP; ++p) sv[p] = ld16(src[p] + o);
   };
   auto stage_store = [&](unsigned char* buf) {
-    if (stager)
 #pragma unroll
-      for (int p = 0; p < NP; ++p) st16(buf + dst[p], sv[p]);
+    for (int p = 0; p < NP; ++p) st16(buf + dst[p], sv[p]);
   };
   auto weights = [&](int k, u32x4_t (&v)[4], uint32_t& s) {
     const int kk = min(k, kt - 1);

@@ -269,6 +269,41 @@ def test_layer_other_stream(cuda):
     assert torch.equal(q.cpu().float(), fmt.mx_dequant(*fmt.mx_quantize(x.cpu(), "mxfp6"), "mxfp6"))
 
 
+def test_two_handles_at_once(cuda):
+    """Decode and sorted calls of two layers on two streams, queued without waiting: each as alone."""
+    E, H, I, K = 16, 512, 256, 4
+    hs = [_handle(E, H, I, s, cuda)[0] for s in (11, 12)]
+    streams = [torch.cuda.Stream() for _ in hs]
+    g = torch.Generator().manual_seed(8)
+    calls = []
+    for T in (1, 8, 16, 100, 400):
+        ids, tw = (t.to(cuda) for t in topk_routing(T, E, K, seed=T))
+        x = torch.randn(T, H, generator=g).to(torch.bfloat16).to(cuda)
+        calls.append((x, ids, tw, [torch.ops.nanovllm.moe_forward(x, ids, tw, h) for h in hs]))
+    torch.cuda.synchronize()
+    got = []
+    for rep in range(6):
+        for x, ids, tw, _ in calls:
+            for h, s in zip(hs, streams):
+                with torch.cuda.stream(s):
+                    got.append(torch.ops.nanovllm.moe_forward(x, ids, tw, h))
+    torch.cuda.synchronize()
+    want = [y for _ in range(6) for c in calls for y in c[3]]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_layer_timing(cuda):
+    E, H, I = 8, 256, 128
+    h, _, _ = _handle(E, H, I, 13, cuda)
+    assert h.get_last_run_time_ms() < 0
+    h.set_timing(True)
+    for T, K, phases in ((2, 4, 1), (2, 8, 1), (100, 4, 2)):   # one launch; sorted
+        ids, tw = (t.to(cuda) for t in topk_routing(T, E, K, seed=T))
+        torch.ops.nanovllm.moe_forward(torch.zeros(T, H, dtype=torch.bfloat16, device=cuda), ids, tw, h)
+        ms = h.get_last_phase_times_ms()
+        assert len(ms) == phases and all(v > 0 for v in ms) and h.get_last_run_time_ms() > 0
+
+
 def test_layer_refusals(cuda):
     E, H, I, K = 4, 128, 64, 2
     h = torch.classes.nanovllm.MoEInfer(E, H, I, 3)
@@ -290,6 +325,17 @@ def test_layer_refusals(cuda):
     h.store_mxfp4_repack(*a, *b)
     with pytest.raises(RuntimeError, match="float16 or bfloat16"):
         torch.ops.nanovllm.moe_forward(x.float(), ids, tw, h)
+    f, lg = torch.ops.nanovllm.moe_forward_scores, torch.zeros(2, E, device=cuda)
+    for args, word in (((x, lg[:1], 2), "T,H"), ((x, lg[:, :3], 2), "experts"), ((x[:, :64], lg, 2), "hidden size"),
+                       ((x, lg, 5), "top_k"), ((x, lg.cpu(), 2), "one device"), ((x.float(), lg, 2), "float16 or bfloat16")):
+        with pytest.raises(RuntimeError, match=word):
+            f(*args, None, "softmax", 1, 1, 1, True, 1.0, h)
+    with pytest.raises(RuntimeError, match="one device"):
+        f(x, lg, 2, torch.zeros(E), "softmax", 1, 1, 1, True, 1.0, h)
+    with pytest.raises(RuntimeError, match="one device"):
+        torch.ops.nanovllm.moe_topk_scores(lg.cpu(), 2, torch.zeros(E, device=cuda))
+    assert f(x[:0], lg[:0], 2, None, "softmax", 1, 1, 1, True, 1.0, h).shape == (0, H)
+    assert torch.ops.nanovllm.moe_forward(x[:0], ids[:0], tw[:0], h).shape == (0, H)
     with pytest.raises(RuntimeError, match="HIP tensors only"):
         torch.ops.nanovllm.moe_forward(x.cpu(), ids.cpu(), tw.cpu(), h)
 

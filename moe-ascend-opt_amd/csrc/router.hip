@@ -109,6 +109,10 @@ __device__ __forceinline__ void merge(Top2& x, double a, double b) {
 // A pick is the largest choice: found as a maximum of the choices rounded to
 // fp32 (rounding keeps the order, so the largest is among those that reach
 // it), and only where several experts reach it in 64 bits among them.
+//
+// Bound by vector issue, of the 64-bit scores and of K dependent maxima:
+// T = 16384 E = 256 top-8 bf16 in 8 groups 27 us (reading its 8 MB: 2 us);
+// T = 1 4.4 us, a launch and that chain.
 template <int LDT, int NJ>   // logits: 0 fp16, 1 bf16, 2 fp32; NJ = ceil(E / 64), a power of two
 __global__ __launch_bounds__(kScoreWaves * kWave) void topk_scores_kernel(const void* __restrict__ logits, const float* __restrict__ bias,
                                                                           ScoreArgs a, int32_t* __restrict__ ids_out,

@@ -253,6 +253,40 @@ def test_layer_graph(cuda, T):
         torch.ops.nanovllm.moe_forward(big, bi, bw, h)
 
 
+@pytest.mark.parametrize("T", [1, 8, 70])
+def test_ops_in_a_graph(cuda, T):
+    """Router, layer and quantizers captured once, replayed over new inputs: as called eagerly."""
+    E, H, I, K = 16, 512, 256, 8
+    h, _, _ = _handle(E, H, I, 14, cuda)
+    g = torch.Generator().manual_seed(T)
+    x = torch.randn(T, H, generator=g).to(torch.bfloat16).to(cuda)
+    logits = torch.randn(T, E, generator=g).to(cuda)
+    bias = (torch.randn(E, generator=g) * 0.1).to(cuda)
+    ops = torch.ops.nanovllm
+
+    def run():
+        args = (K, bias, "sigmoid", 4, 2, 2, True, 2.5)
+        y = ops.moe_forward_scores(x, logits, *args, h)
+        codes, scales = ops.mx_quantize(y, "mxfp6")
+        return y, *ops.moe_topk_scores(logits, *args), codes, scales, ops.mx_dequantize(codes, scales, "mxfp6", torch.bfloat16)
+
+    run()   # the handle's buffers
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for i in range(4):
+        x.copy_(torch.randn(T, H, generator=g).to(torch.bfloat16))
+        logits.copy_(torch.randn(T, E, generator=g))
+        logits[0, i:i + 9] = -float("inf")
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        assert all(torch.equal(a, b) for a, b in zip(got, run()))
+        n = 200 * (i + 1)   # an eager call that outgrows the buffers
+        ops.moe_forward_scores(x[:1].expand(n, H), logits[:1].expand(n, E), K, None, "softmax", 1, 1, 1, True, 1.0, h)
+
+
 def test_layer_other_stream(cuda):
     E, H, I, K, T = 8, 256, 128, 4, 33
     h, _, _ = _handle(E, H, I, 7, cuda)

@@ -260,7 +260,6 @@ struct ScoreArgs {
 // Element formats of the MX blocks (mx_device.hpp): the wire codes of
 // mi_moe_mx_quantize.
 constexpr int kMxFp4 = 0, kMxFp6 = 1;
-__host__ __device__ constexpr int mx_block_bytes(int fmt) { return fmt == kMxFp4 ? 16 : 24; }
 
 // K runs in tiles of 128 (4 blocks); rows whose length is no multiple end in
 // blocks of zeros.  Weights are stored in units of 64 rows, four 16-row

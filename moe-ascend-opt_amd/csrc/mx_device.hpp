@@ -101,7 +101,7 @@ __device__ __forceinline__ u32x4_t mx_fp4_codes32(const float (&v)[32], int s) {
   return o;
 }
 
-// Two adjacent elements of row data of type DT (0 fp16, 1 bf16, 2 fp32) as floats.
+// 32 16-bit values (DT 0 fp16, 1 bf16) in 16 words as floats.
 template <int DT>
 __device__ __forceinline__ void mx_unpack16(const uint32_t (&w)[16], float (&v)[32]) {
 #pragma unroll

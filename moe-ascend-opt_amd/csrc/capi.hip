@@ -913,7 +913,7 @@ MI_API int mi_moe_topk_scores(const void* logits, int logits_dtype, int64_t T, i
   if (T == 0) return MI_MOE_OK;
   if (!logits || !topk_ids || !topk_w) return fail(MI_MOE_EINVAL, "null pointer");
   const ScoreArgs a = {(int)T, (int)E, (int)K, score == MI_MOE_SCORE_SIGMOID, (int)n_group, (int)topk_group, (int)group_top,
-                       renormalize != 0, (double)scale, 0};
+                       renormalize != 0, (double)scale, 0, 0};
   HIPCHK(launch_topk_scores(logits, logits_dtype, bias, a, topk_ids, topk_w, (hipStream_t)stream));
   return MI_MOE_OK;
 }

@@ -254,6 +254,7 @@ struct ScoreArgs {
   int renorm;
   double scale;
   int group_lanes;             // lanes that hold a group, 0: not whole lanes (set by the launcher)
+  int wide;                    // wave per token: rows and bias load in pieces (set by the launcher)
 };
 
 // ---------------------------------------------------------------- MXFP4 layer (mx.hip)

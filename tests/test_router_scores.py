@@ -133,6 +133,39 @@ def test_c_refusals():
     assert rc == 1 and "null handle" in L.mi_moe_last_error().decode()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("E,K,groups", [(64, 6, (1, 1, 1)), (60, 16, (1, 1, 1)), (128, 8, (16, 4, 2)), (128, 12, (8, 8, 1)),
+                                        (256, 8, (8, 4, 2)), (160, 6, (10, 3, 1)), (240, 1, (15, 2, 2)), (16, 4, (4, 2, 2)),
+                                        (256, 20, (8, 4, 2)), (250, 5, (1, 1, 1))])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+def test_many_tokens(E, K, groups, dt):
+    """A call of many tokens gives each the bits of a call of few, from unaligned rows as well."""
+    nanovllm_moe.load()
+    T, f, inf = 4001, torch.ops.nanovllm.moe_topk_scores, float("inf")
+    g = torch.Generator().manual_seed(E + K)
+    flat = (torch.randn(T * E + 1, generator=g) * 2).to(dt)
+    x = flat[:T * E].view(T, E)
+    x[5], x[6, 3:], x[7, ::2], x[8, 1] = -inf, -inf, -inf, float("nan")
+    x[9], x[10], x[11] = 0.0, torch.finfo(dt).min, x[11].round()     # ties
+    x[12, 2], x[3999, 1], x[4000, -1] = inf, -inf, float("nan")
+    x[20:400] = x[20:400].round()
+    flat = flat.cuda()
+    x = flat[:T * E].view(T, E)
+    bias = (torch.randn(E + 1, generator=g) * 0.1).cuda()
+    for score in ("softmax", "sigmoid"):
+        for b in (None, bias[:E]):
+            args = (b, score, *groups, True, 2.5)
+            ids, w = f(x, K, *args)
+            parts = [f(x[i:i + 500], K, *args) for i in range(0, T, 500)]
+            assert torch.equal(ids, torch.cat([p[0] for p in parts]))
+            assert torch.equal(w.nan_to_num(nan=-1.0), torch.cat([p[1] for p in parts]).nan_to_num(nan=-1.0))
+            hi, hw = f(x[:600].cpu(), K, None if b is None else b.cpu(), score, *groups, True, 2.5)
+            assert torch.equal(ids[:600].cpu(), hi) and torch.equal(w[:600].cpu().isnan(), hw.isnan())
+    y, b = flat[1:].view(T, E), bias[1:]
+    for p, q in zip(f(y, K, b, "sigmoid", *groups, False, 1.0), f(y.clone(), K, b.clone(), "sigmoid", *groups, False, 1.0)):
+        assert torch.equal(p.nan_to_num(nan=-1.0), q.nan_to_num(nan=-1.0))
+
+
 def test_forward_scores_on_host(monkeypatch):
     """The host layer behind the host router: as its two steps."""
     monkeypatch.setenv("MIMOE_HOST_WEIGHTS", "1")

@@ -148,8 +148,8 @@ int mi_moe_store_mxfp4(mi_moe_handle* h, const uint8_t* gate_up_codes,
  * MXFP4 handles quantize x and the intermediate silu(gate) * up to MXFP6
  * blocks (mi_moe_mx_quantize's rounding) and sum exact products in fp32; they
  * use the workspace at every size (reserve it before a capture).  A NaN or an
- * infinity in x makes its token's y NaN; an expert output beyond the fp32
- * range makes 16 columns of it NaN, or stays infinite in small calls. */
+ * infinity in x makes its token's y NaN.  Expert outputs are held in fp32 at
+ * every size. */
 int mi_moe_forward(mi_moe_handle* h, const void* x, void* y,
                    const float* topk_w, const int32_t* topk_ids, int64_t T,
                    int64_t K, int act_dtype, void* stream);

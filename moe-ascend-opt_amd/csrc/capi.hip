@@ -51,7 +51,7 @@ hipError_t launch_topk_softmax(const void*, int, int, int, int, int, int32_t*, f
 hipError_t launch_topk_scores(const void*, int, const float*, ScoreArgs, int32_t*, float*, hipStream_t);
 hipError_t launch_route_mx(const void*, int, int, int, unsigned char*, const int32_t*, int, int, int, const RouteGlobal&,
                            hipStream_t, int);
-hipError_t launch_mx_sorted(const MxArgs&, int, int, hipStream_t, hipEvent_t);
+hipError_t launch_mx_gemm(const MxArgs&, int, hipStream_t, hipEvent_t);
 hipError_t launch_mx_decode(const MxArgs&, int, hipStream_t, hipEvent_t);
 hipError_t launch_mx_quantize(const void*, int, int64_t, int, int64_t, int, unsigned char*, unsigned char*, hipStream_t);
 hipError_t launch_mx_dequantize(const unsigned char*, const unsigned char*, int64_t, int, void*, int, hipStream_t);
@@ -492,8 +492,7 @@ int forward_mx(mi_moe_handle* h, const void* x, void* y, const float* tw, const 
   a.w2 = (const unsigned char*)h->w2.p; a.w2_s = (const unsigned char*)h->w2_s.p;
   a.xq = (unsigned char*)w.xq;
   a.act = (unsigned char*)w.act;
-  a.eout = (int16_t*)w.eout;   // the fp32 rows' room holds both
-  a.eout_d = (unsigned char*)w.eout + (size_t)n * h->H * 2;
+  a.eout = w.eout;
   a.tact = w.tact;
   hipEvent_t mid = h->timing && !noalloc && !fused ? h->evmid : nullptr;
   if (decode) {
@@ -503,8 +502,9 @@ int forward_mx(mi_moe_handle* h, const void* x, void* y, const float* tw, const 
   }
   const bool big = mx_big(n, h->E);
   HIPCHK(launch_route_mx(x, act, a.T, a.H, a.xq, ids, a.n, a.K, a.E, a.rg, st, big ? kRouteBigTiles : 0));
-  HIPCHK(launch_mx_sorted(a, act, (int)(big ? n / (2 * kGemmRows) + h->E : gemm_tiles_max(n, (int)h->E)), st, mid));
+  HIPCHK(launch_mx_gemm(a, (int)(big ? n / (2 * kGemmRows) + h->E : gemm_tiles_max(n, (int)h->E)), st, mid));
   if (!noalloc) h->mid_recorded = mid != nullptr;
+  HIPCHK(launch_combine(a.eout, tw, ids, y, a.T, a.K, a.E, a.H, act, st, false));
   return MI_MOE_OK;
 }
 

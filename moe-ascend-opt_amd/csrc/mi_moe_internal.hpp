@@ -293,8 +293,7 @@ struct MxArgs {
   const unsigned char* w2_s;
   unsigned char* xq;       // [T][mx_row_bytes(H)] quantized hidden rows
   unsigned char* act;      // [n][mx_row_bytes(I)] quantized intermediate, row = sorted position
-  int16_t* eout;           // [n][H] expert outputs, row = pair, 16-bit fixed point
-  unsigned char* eout_d;   // [n][H/64][4] their scales
+  float* eout;             // [n][H] expert outputs, row = pair
   unsigned long long* tact;   // one-launch decode: tagged units [n][I/32][8] (within tagged_act_bytes(I))
 };
 

@@ -188,39 +188,12 @@ __device__ __forceinline__ void mx_gate_up(const MxArgs& a, unsigned char* smem,
   }
 }
 
-// Expert outputs between the down product and the combine: 16-bit fixed point
-// with a power-of-two scale for every 16 columns.  Half of fp32's bytes; the
-// rounding, at most 2^-15 of the 16 columns' largest, is far below that of
-// the 16-bit result (16-bit floats would add as much as the result's own)
-// unless one column is some hundred times its neighbours: at a thousand times
-// it is up to 3% of them, still a part of the 4-bit weights' 11%.
-// Stores 16 columns and returns their scale byte s: |values| < 2^(s-126),
-// 255: one of them is NaN or infinite.
-__device__ __forceinline__ uint32_t eout_store(int16_t* o, const float (&v)[16]) {
-  uint32_t am = 0;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
-    am = b > am ? b : am;
-  }
-  const uint32_t s = am >= 0x7f800000u ? 255 : am >= 0x00800000u ? am >> 23 : 1;
-  const float id = __builtin_ldexpf(1.0f, 126 - (int)s);
-  uint32_t w[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    w[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_i16(v[2 * i] * id, v[2 * i + 1] * id));
-  st16(o, u32x4_t{w[0], w[1], w[2], w[3]});
-  st16(o + 8, u32x4_t{w[4], w[5], w[6], w[7]});
-  return s;
-}
-// the factor of a value's integer
-__device__ __forceinline__ float eout_scale(int s) {
-  return s == 255 ? __uint_as_float(0x7fc00000u) : __builtin_ldexpf(1.0f / 32767.0f, s - 126);
-}
-
-// down of one work item: a unit is 64 rows of H.  After a transpose between
-// its lane rows a lane stores a token's 64 columns, a whole cache line (in 8
-// byte pieces, without the transpose, T = 4096 takes 118 us, not 92).
+// down of one work item: a unit is 64 rows of H.  Expert outputs are fp32 up
+// to the combine, as in decode calls: a column may be a thousand times its
+// neighbours, so none shares a scale with them.  Lanes store where the
+// products leave the values, four lanes 64 bytes of a token's row (T = 4096
+// H=2048 top-8: 268 MB, the call 258 us; with a transpose, a lane per token's
+// row, 271).
 template <int NSUB>
 __device__ __forceinline__ void mx_down(const MxArgs& a, unsigned char* smem, int e, int row0, int rows, int m) {
   const int NQ = a.H >> 6, kt = mx_ktiles(a.I), lane = threadIdx.x & 63;
@@ -230,27 +203,16 @@ __device__ __forceinline__ void mx_down(const MxArgs& a, unsigned char* smem, in
       smem, [&](int i) { return a.act + (size_t)(row0 + min(i, rows - 1)) * mx_row_bytes(a.I); }, kt,
       a.w2 + unit * kMxTileBytes + lane * 16, a.w2_s + unit * kMxTileScaleBytes + lane * 4, acc);
   if (m >= NQ) return;
+  int pair[NSUB];
 #pragma unroll
-  for (int g = 0; g < (NSUB + 3) / 4; ++g) {   // four subtiles at a time
-    const int row = 64 * g + lane;   // 16 subtile + row
-    const int pair = a.rg.tok[row0 + min(row, rows - 1)];
-    int16_t* o = a.eout + (size_t)pair * a.H + 64 * m;
-    uint32_t s4 = 0;
+  for (int s = 0; s < NSUB; ++s) pair[s] = a.rg.tok[row0 + min(16 * s + (lane & 15), rows - 1)];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      float v[16];   // [q][4]
+  for (int s = 0; s < NSUB; ++s) {
+    if (16 * s + (lane & 15) < rows) {
+      float* o = a.eout + (size_t)pair[s] * a.H + 64 * m + 4 * (lane >> 4);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float h[4];
-#pragma unroll
-        for (int s = 0; s < 4; ++s) h[s] = 4 * g + s < NSUB ? acc[t][4 * g + s < NSUB ? 4 * g + s : 0][i] : 0.0f;
-        transpose4(h[0], h[1], h[2], h[3]);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[4 * q + i] = h[q];
-      }
-      if (row < rows) s4 |= eout_store(o + 16 * t, v) << (8 * t);
+      for (int t = 0; t < 4; ++t) *reinterpret_cast<f32x4_t*>(o + 16 * t) = acc[t][s];
     }
-    if (row < rows) *reinterpret_cast<uint32_t*>(a.eout_d + ((size_t)pair * NQ + m) * 4) = s4;
   }
 }
 
@@ -275,9 +237,9 @@ __device__ __forceinline__ void mx_gemm_item(const MxArgs& a, unsigned char* sme
 // 64-row items at four waves per SIMD, 128-row items at two (twice the accumulators).
 //
 // gate_up / down, H=2048 I=768 E=128 top-8: T = 333 skewed 43 / 30 us, 5.0 /
-// 3.6 TB/s of weights, the memory rate; T = 4096 96 / 92 us, 2.1 / 1.1 PFLOP/s:
+// 3.6 TB/s of weights, the memory rate; T = 4096 95 / 118 us, 2.2 / 0.9 PFLOP/s:
 // the K loop alone runs at 5 (the instruction in registers at 5.9), the items'
-// first loads and their epilogues, gate_up's quantization and down's 138 MB
+// first loads and their epilogues, gate_up's quantization and down's 268 MB
 // of expert outputs, take the rest.
 template <bool DOWN>
 __global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(4))) void mx_gemm_kernel(MxArgs a) {
@@ -288,53 +250,6 @@ template <bool DOWN>
 __global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(2))) void mx_gemm_big_kernel(MxArgs a) {
   __shared__ __align__(16) unsigned char smem[2 * mx_stage_bytes(8)];
   mx_gemm_item<true, DOWN>(a, smem);
-}
-
-// y[t,h] = cast(sum_k w[t,k] eout[t*K+k,h]) over the valid ids in k order, in
-// fp32; a token without a valid id gets 0.  A workgroup takes (part of) a
-// token, a thread 8 columns.  Bound by reading: T = 4096 H=2048 top-8, 155 MB
-// in 25 us (part of it from the caches).
-constexpr int kMxCombineThreads = 256;
-template <int ACT>
-__global__ __launch_bounds__(kMxCombineThreads) void mx_combine_kernel(const int16_t* __restrict__ eout, const unsigned char* __restrict__ eout_d,
-                                                                       const float* __restrict__ tw, const int32_t* __restrict__ ids,
-                                                                       uint16_t* __restrict__ y, int T, int parts, int K, int E, int H) {
-  for (unsigned b = blockIdx.x; b < (unsigned)T * parts; b += gridDim.x) {
-    const int t = b / parts, h = ((b - t * parts) * kMxCombineThreads + threadIdx.x) * 8;
-    if (h >= H) continue;
-    float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    constexpr int kB = 8;   // pairs whose loads are issued together
-    for (int k0 = 0; k0 < K; k0 += kB) {
-      int ev[kB];
-      float wv[kB];
-      int dv[kB];   // scale bytes
-      u32x4_t rv[kB];
-#pragma unroll
-      for (int j = 0; j < kB; ++j) {
-        const size_t i = (size_t)t * K + min(k0 + j, K - 1);
-        ev[j] = k0 + j < K ? ids[i] : -1;
-        wv[j] = tw[i];
-        dv[j] = eout_d[i * (H >> 4) + (h >> 4)];
-        rv[j] = ld16(eout + i * H + h);
-      }
-#pragma unroll
-      for (int j = 0; j < kB; ++j) {
-        if ((unsigned)ev[j] >= (unsigned)E) continue;   // uniform
-        const uint32_t u[4] = {rv[j].x, rv[j].y, rv[j].z, rv[j].w};
-        const float d = eout_scale(dv[j]);
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const float lo = (float)(int16_t)(u[p] & 0xffffu) * d, hi = (float)((int32_t)u[p] >> 16) * d;
-          acc[2 * p] = acc[2 * p] + wv[j] * lo;
-          acc[2 * p + 1] = acc[2 * p + 1] + wv[j] * hi;
-        }
-      }
-    }
-    uint32_t o[4];
-#pragma unroll
-    for (int p = 0; p < 4; ++p) o[p] = from_f32<ACT>(acc[2 * p]) | ((uint32_t)from_f32<ACT>(acc[2 * p + 1]) << 16);
-    st16(y + (size_t)t * H + h, u32x4_t{o[0], o[1], o[2], o[3]});
-  }
 }
 
 // One block of 32 elements of type DT (0 fp16, 1 bf16, 2 fp32) as floats.
@@ -471,8 +386,8 @@ unsigned blocks_for(int64_t items) {
 
 }  // namespace
 
-// The sorted path behind the routing (launch_route_mx): both grouped products, the combine.
-hipError_t launch_mx_sorted(const MxArgs& a, int act, int tiles_max, hipStream_t st, hipEvent_t mid) {
+// The grouped products of the sorted path, behind the routing (launch_route_mx).
+hipError_t launch_mx_gemm(const MxArgs& a, int tiles_max, hipStream_t st, hipEvent_t mid) {
   const bool big = mx_big(a.n, a.E);
   const int tg = (tiles_max + 7) / 8 * 8;   // an eighth for each XCD
   const int b13 = (4 * mx_ktiles(a.I) + kMxWaves - 1) / kMxWaves, b2 = ((a.H >> 6) + kMxWaves - 1) / kMxWaves;
@@ -483,12 +398,6 @@ hipError_t launch_mx_sorted(const MxArgs& a, int act, int tiles_max, hipStream_t
   if (mid && (err = hipEventRecord(mid, st)) != hipSuccess) return err;
   if (big) hipLaunchKernelGGL(mx_gemm_big_kernel<true>, dim3(tg * b2), dim3(kMxThreads), 0, st, a);
   else hipLaunchKernelGGL(mx_gemm_kernel<true>, dim3(tg * b2), dim3(kMxThreads), 0, st, a);
-  err = hipGetLastError();
-  if (err != hipSuccess) return err;
-  const int parts = ((a.H >> 3) + kMxCombineThreads - 1) / kMxCombineThreads;   // at most 32: T parts < 2^30
-  auto kern = act == 1 ? mx_combine_kernel<1> : mx_combine_kernel<0>;
-  const unsigned g = (unsigned)std::min<int64_t>((int64_t)a.T * parts, 1 << 20);
-  hipLaunchKernelGGL(kern, dim3(g), dim3(kMxCombineThreads), 0, st, a.eout, a.eout_d, a.tw, a.ids, a.y, a.T, parts, a.K, a.E, a.H);
   return hipGetLastError();
 }
 

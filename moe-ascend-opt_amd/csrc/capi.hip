@@ -14,6 +14,7 @@
 #include <cstdlib>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <string>
 #include <vector>
 
@@ -113,6 +114,24 @@ struct DevBuf {
     return e;
   }
 };
+
+struct BufBytes {
+  DevBuf* buf;
+  size_t bytes;
+};
+// All of the buffers or, where one cannot be had, none: callers take a buffer
+// that is there as a sign that its fellows are.
+hipError_t alloc_all(std::initializer_list<BufBytes> bufs, bool cleared) {
+  hipError_t e = hipSuccess;
+  for (const BufBytes& b : bufs) {
+    e = b.buf->alloc(b.bytes);
+    if (e == hipSuccess && cleared) e = hipMemset(b.buf->p, 0, b.buf->bytes);
+    if (e != hipSuccess) break;
+  }
+  if (e != hipSuccess)
+    for (const BufBytes& b : bufs) b.buf->release();
+  return e;
+}
 
 // Scoped temporary device copy of a caller buffer (host or device source).
 struct Staged {
@@ -400,14 +419,10 @@ int forward_w4a16(mi_moe_handle* h, const void* x, void* y, const float* tw, con
 int q_alloc_weights(mi_moe_handle* h) {
   const int64_t E = h->E, H = h->H, I = h->I;
   const int64_t bb = h->quant == MI_MOE_Q8_0 ? 2048 : 1024;  // bytes per (tile, block)
-  HIPCHK(h->w13.alloc((size_t)E * (I / 32) * (H / 32) * bb));
-  HIPCHK(h->w13_s.alloc((size_t)E * (I / 32) * (H / 32) * 64 * 2));
-  HIPCHK(h->w2.alloc((size_t)E * (H / 64) * (I / 32) * bb));
-  HIPCHK(h->w2_s.alloc((size_t)E * (H / 64) * (I / 32) * 64 * 2));
-  HIPCHK(hipMemset(h->w13.p, 0, h->w13.bytes));
-  HIPCHK(hipMemset(h->w13_s.p, 0, h->w13_s.bytes));
-  HIPCHK(hipMemset(h->w2.p, 0, h->w2.bytes));
-  HIPCHK(hipMemset(h->w2_s.p, 0, h->w2_s.bytes));
+  HIPCHK(alloc_all({{&h->w13, (size_t)E * (I / 32) * (H / 32) * bb},
+                    {&h->w13_s, (size_t)E * (I / 32) * (H / 32) * 64 * 2},
+                    {&h->w2, (size_t)E * (H / 64) * (I / 32) * bb},
+                    {&h->w2_s, (size_t)E * (H / 64) * (I / 32) * 64 * 2}}, true));
   return MI_MOE_OK;
 }
 
@@ -463,12 +478,9 @@ int forward_q(mi_moe_handle* h, const void* x, void* y, const float* tw, const i
 
 int mx_alloc_weights(mi_moe_handle* h) {
   const size_t E = (size_t)h->E, t13 = E * (h->I / 32) * mx_ktiles((int)h->H), t2 = E * (h->H / 64) * mx_ktiles((int)h->I);
-  HIPCHK(h->w13.alloc(t13 * kMxTileBytes));
-  HIPCHK(h->w13_s.alloc(t13 * kMxTileScaleBytes));
-  HIPCHK(h->w2.alloc(t2 * kMxTileBytes));
-  HIPCHK(h->w2_s.alloc(t2 * kMxTileScaleBytes));
   // zeros stay where K is no multiple of 128, and in what has not been stored
-  for (DevBuf* b : {&h->w13, &h->w13_s, &h->w2, &h->w2_s}) HIPCHK(hipMemset(b->p, 0, b->bytes));
+  HIPCHK(alloc_all({{&h->w13, t13 * kMxTileBytes}, {&h->w13_s, t13 * kMxTileScaleBytes},
+                    {&h->w2, t2 * kMxTileBytes}, {&h->w2_s, t2 * kMxTileScaleBytes}}, true));
   HIPCHK(hipStreamSynchronize(nullptr));   // before the caller's stream, which may not wait for the default one
   return MI_MOE_OK;
 }
@@ -686,10 +698,14 @@ MI_API int mi_moe_store_awq(mi_moe_handle* h, const int32_t* w13_q, const int32_
   HIPCHK(e.stage(w2_z, z2, src_on_device, st));
   HIPCHK(f.stage(w2_s, s2, src_on_device, st));
   const int64_t NT13 = 2 * (I / 16), G1 = H / 128, CH = I / 32, MQ = H / 64, G2 = I / 128;
-  HIPCHK(h->w13.alloc((size_t)E * NT13 * G1 * 1024));
-  HIPCHK(h->w13_s.alloc((size_t)E * (I / 16) * 80 * G1));    // metadata blocks
-  HIPCHK(h->w2.alloc((size_t)E * CH * MQ * 1024));
-  HIPCHK(h->w2_s.alloc((size_t)E * MQ * 4 * w2_meta_sec_bytes((int)G2)));   // metadata sections
+  if (!h->w13.p) {
+    HIPCHK(alloc_all({{&h->w13, (size_t)E * NT13 * G1 * 1024},
+                      {&h->w13_s, (size_t)E * (I / 16) * 80 * G1},   // metadata blocks
+                      {&h->w2, (size_t)E * CH * MQ * 1024},
+                      {&h->w2_s, (size_t)E * MQ * 4 * w2_meta_sec_bytes((int)G2)}}, false));   // metadata sections
+  } else {
+    HIPCHK(hipDeviceSynchronize());   // the weights that are replaced may be in use on any stream
+  }
   HIPCHK(launch_awq_repack_all((const int32_t*)a.ptr, (const int32_t*)b.ptr, (const uint16_t*)c.ptr,
                                (const int32_t*)d.ptr, (const int32_t*)e.ptr, (const uint16_t*)f.ptr,
                                h->w13.p, (unsigned char*)h->w13_s.p, h->w2.p, (unsigned char*)h->w2_s.p,

@@ -1,0 +1,126 @@
+"""Checks of libmimoe.so's host code against a HIP runtime of host memory (cpp/fake_hip.cpp), in which allocations can
+fail and kernels are counted, not run.  A program of its own, without torch: the runtime has to be loaded before the
+library.  Usage: fake_device.py <fake runtime> <library> <check>; prints ok."""
+import ctypes
+import sys
+
+P, I64, I, F = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
+Q8_0, Q4_0, W4A16, MXFP4 = range(4)
+BF16, F32 = 1, 2
+EHIP = 4
+STREAM = P(1 << 20)      # a stream of the caller's, which does not wait for the default one
+DATA = ctypes.create_string_buffer(1 << 22)   # what every argument points to; only host sources are read
+AT = P((ctypes.addressof(DATA) + 255) & ~255)
+SHAPE = {Q8_0: (4, 128, 64), Q4_0: (4, 128, 64), W4A16: (2, 512, 128), MXFP4: (4, 192, 96)}
+
+ARGS = {
+    "mi_moe_create": [I64, I64, I64, I, ctypes.POINTER(P)], "mi_moe_destroy": [P], "mi_moe_reserve": [P, I64, I64, P],
+    "mi_moe_store_mxfp4": [P, P, P, P, P, I, P], "mi_moe_store_quantized": [P, P, P, P, P, I, I, P],
+    "mi_moe_store_awq": [P, P, P, P, P, P, P, I64, I, I, P],
+    "mi_moe_quantize_and_store_expert": [P, I64, I, P, I, I, P],
+    "mi_moe_forward": [P, P, P, P, P, I64, I64, I, P],
+    "mi_moe_forward_logits": [P, P, P, P, I, I64, I64, I, I, P, P, P],
+    "mi_moe_forward_scores": [P, P, P, P, I, I64, I64, P, I, I64, I64, I64, I, F, I, P, P, P],
+}
+
+
+class Device:
+    def __init__(self, fake, lib):
+        self.f = ctypes.CDLL(fake, mode=ctypes.RTLD_GLOBAL)
+        self.f.fake_mallocs.restype = self.f.fake_launches.restype = self.f.fake_live.restype = ctypes.c_long
+        self.f.fake_fail_at.argtypes = [ctypes.c_long]
+        self.lib = ctypes.CDLL(lib)
+        self.lib.mi_moe_last_error.restype = ctypes.c_char_p
+        for name, args in ARGS.items():
+            getattr(self.lib, name).argtypes = args
+
+    def call(self, name, *args):
+        return getattr(self.lib, "mi_moe_" + name)(*args)
+
+    def ok(self, name, *args):
+        rc = self.call(name, *args)
+        assert rc == 0, (name, rc, self.lib.mi_moe_last_error())
+
+    def handle(self, quant):
+        h = P()
+        self.ok("create", *SHAPE[quant], quant, ctypes.byref(h))
+        return h
+
+    def live(self):
+        """The sizes of all allocations, and which were cleared as a whole."""
+        sizes, cleared = (ctypes.c_size_t * 256)(), (I * 256)()
+        n = self.f.fake_live(sizes, cleared, 256)
+        return sorted((sizes[i], cleared[i]) for i in range(n))
+
+    # calls of each kind, the same for every handle
+    def store(self, h, quant):
+        if quant == MXFP4:
+            return self.call("store_mxfp4", h, AT, AT, AT, AT, 1, STREAM)
+        if quant == W4A16:
+            return self.call("store_awq", h, *[AT] * 6, 128, BF16, 1, STREAM)
+        return self.call("store_quantized", h, AT, AT, AT, AT, BF16, 1, STREAM)
+
+    def online(self, h, quant):
+        return self.call("quantize_and_store_expert", h, 1, 2, AT, F32, 1, STREAM)
+
+    def forward(self, h, T, K=2):
+        return self.call("forward", h, AT, AT, AT, AT, T, K, BF16, STREAM)
+
+
+def retried(d, quant, before, call, after):
+    """call fails at each of its allocations in turn; `after` on such a handle leaves what it leaves on one where the
+    call was never made."""
+    def run(fail):
+        h = d.handle(quant)
+        before(h)
+        n = None
+        if fail is not None:
+            d.f.fake_fail_at(fail)
+            rc = call(h)
+            n = d.f.fake_mallocs()
+            d.f.fake_fail_at(-1)
+            if n <= fail:            # it has no allocation of that number
+                assert rc == 0
+                d.ok("destroy", h)
+                return None
+            assert rc == EHIP, rc
+        rc = after(h)
+        assert rc == 0, (fail, rc, d.lib.mi_moe_last_error())
+        left = d.live()
+        d.ok("destroy", h)
+        assert d.live() == [], "allocations left behind a handle"
+        return left
+    want, tried = run(None), 0
+    while True:
+        got = run(tried)
+        if got is None:
+            break
+        assert got == want, (tried, got, want)
+        tried += 1
+    return tried
+
+
+def weights(d):
+    for quant in (Q8_0, Q4_0, W4A16, MXFP4):
+        store = lambda h: d.store(h, quant)
+        assert retried(d, quant, lambda h: None, store, store) == 4, quant
+        if quant in (Q8_0, MXFP4):
+            online = lambda h: d.online(h, quant)
+            assert retried(d, quant, lambda h: None, online, online) == 4, quant
+    # weights stored a second time, with no memory to be had: the handle serves on
+    for quant in (Q8_0, Q4_0, W4A16, MXFP4):
+        h = d.handle(quant)
+        assert d.store(h, quant) == 0
+        have = d.live()
+        d.f.fake_fail_at(0)
+        assert d.store(h, quant) == 0 and d.f.fake_mallocs() == 0, quant
+        d.f.fake_fail_at(-1)
+        assert d.live() == have
+        d.ok("destroy", h)
+
+
+CHECKS = {f.__name__: f for f in (weights,)}
+
+if __name__ == "__main__":
+    CHECKS[sys.argv[3]](Device(sys.argv[1], sys.argv[2]))
+    print("ok")

@@ -1,0 +1,31 @@
+"""The library's host code when memory runs out or calls are refused, on a HIP runtime of host memory
+(cpp/fake_hip.cpp, fake_device.py): a failed allocation leaves a handle that later calls can use."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+import nanovllm_moe
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+
+@pytest.fixture(scope="module")
+def fake(tmp_path_factory):
+    so = str(tmp_path_factory.mktemp("fake") / "libfake_hip.so")
+    build = subprocess.run(["g++", "-O1", "-std=c++17", "-fPIC", "-shared", os.path.join(HERE, "cpp", "fake_hip.cpp"), "-o", so],
+                           stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    assert build.returncode == 0, build.stdout
+    return so
+
+
+def _run(fake, check):
+    run = subprocess.run([sys.executable, os.path.join(HERE, "fake_device.py"), fake, nanovllm_moe.LIB_PATH, check],
+                         stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=120)
+    assert run.returncode == 0 and run.stdout.strip().endswith("ok"), run.stdout
+
+
+def test_weights(fake):
+    """Storing weights: all buffers or none, whichever allocation fails."""
+    _run(fake, "weights")

@@ -119,11 +119,12 @@ struct BufBytes {
   DevBuf* buf;
   size_t bytes;
 };
-// All of the buffers or, where one cannot be had, none: callers take a buffer
-// that is there as a sign that its fellows are.
+// All of the buffers (those of 0 bytes are left out) or, where one cannot be
+// had, none: callers take a buffer that is there as a sign that its fellows are.
 hipError_t alloc_all(std::initializer_list<BufBytes> bufs, bool cleared) {
   hipError_t e = hipSuccess;
   for (const BufBytes& b : bufs) {
+    if (!b.bytes) continue;
     e = b.buf->alloc(b.bytes);
     if (e == hipSuccess && cleared) e = hipMemset(b.buf->p, 0, b.buf->bytes);
     if (e != hipSuccess) break;
@@ -202,11 +203,9 @@ size_t xq_row_bytes(const mi_moe_handle* h) { return h->quant == MI_MOE_MXFP4 ? 
 
 int ensure_workspace(mi_moe_handle* h, int64_t T, int64_t n, hipStream_t st) {
   if (h->r_U.p == nullptr) {
-    HIPCHK(h->r_counts.alloc((size_t)h->E * sizeof(int32_t)));
-    HIPCHK(h->r_starts.alloc((size_t)(h->E + 1) * sizeof(int32_t)));
-    HIPCHK(h->r_active.alloc((size_t)h->E * sizeof(int32_t)));
-    HIPCHK(h->r_U.alloc(sizeof(int32_t)));
-    HIPCHK(h->r_ntiles.alloc(sizeof(int32_t)));
+    HIPCHK(alloc_all({{&h->r_counts, (size_t)h->E * sizeof(int32_t)}, {&h->r_starts, (size_t)(h->E + 1) * sizeof(int32_t)},
+                      {&h->r_active, (size_t)h->E * sizeof(int32_t)}, {&h->r_U, sizeof(int32_t)},
+                      {&h->r_ntiles, sizeof(int32_t)}}, false));
   }
   if (T <= h->cap_T && n <= h->cap_n) return MI_MOE_OK;
   int64_t capT = h->cap_T ? h->cap_T : 16;
@@ -219,17 +218,17 @@ int ensure_workspace(mi_moe_handle* h, int64_t T, int64_t n, hipStream_t st) {
     for (DevBuf* b : {&h->act, &h->act_d, &h->eout, &h->r_tok, &h->r_scat, &h->r_tiles, &h->r_chunk, &h->xq, &h->xd})
       b->retire(h->retired);
   }
-  HIPCHK(h->act.alloc((size_t)capn * act_row_bytes(h)));
-  HIPCHK(h->act_d.alloc((size_t)capn * (h->I / 32) * sizeof(float)));
-  HIPCHK(h->eout.alloc((size_t)capn * h->H * sizeof(float)));
-  HIPCHK(h->r_tok.alloc((size_t)capn * sizeof(int32_t)));
-  HIPCHK(h->r_scat.alloc((size_t)capn * sizeof(int32_t)));
-  HIPCHK(h->r_tiles.alloc((size_t)gemm_tiles_max(capn, (int)h->E) * 4 * sizeof(int32_t)));
-  HIPCHK(h->r_chunk.alloc((size_t)route_chunks((int)capn) * h->E * sizeof(int32_t)));
-  if (h->quant != MI_MOE_W4A16) {
-    HIPCHK(h->xq.alloc((size_t)capT * xq_row_bytes(h)));
-    HIPCHK(h->xd.alloc((size_t)capT * (h->H / 32) * sizeof(float)));
-  }
+  h->cap_T = h->cap_n = 0;   // until every buffer is there
+  const bool xq = h->quant != MI_MOE_W4A16;
+  HIPCHK(alloc_all({{&h->act, (size_t)capn * act_row_bytes(h)},
+                    {&h->act_d, (size_t)capn * (h->I / 32) * sizeof(float)},
+                    {&h->eout, (size_t)capn * h->H * sizeof(float)},
+                    {&h->r_tok, (size_t)capn * sizeof(int32_t)},
+                    {&h->r_scat, (size_t)capn * sizeof(int32_t)},
+                    {&h->r_tiles, (size_t)gemm_tiles_max(capn, (int)h->E) * 4 * sizeof(int32_t)},
+                    {&h->r_chunk, (size_t)route_chunks((int)capn) * h->E * sizeof(int32_t)},
+                    {&h->xq, xq ? (size_t)capT * xq_row_bytes(h) : 0},
+                    {&h->xd, xq ? (size_t)capT * (h->H / 32) * sizeof(float) : 0}}, false));
   h->cap_T = capT;
   h->cap_n = capn;
   return MI_MOE_OK;

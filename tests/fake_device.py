@@ -119,7 +119,18 @@ def weights(d):
         d.ok("destroy", h)
 
 
-CHECKS = {f.__name__: f for f in (weights,)}
+def workspace(d):
+    for quant in (Q8_0, Q4_0, W4A16, MXFP4):
+        for first in (None, 1, 20):       # calls before the one that fails
+            def before(h):
+                assert d.store(h, quant) == 0
+                if first:
+                    assert d.forward(h, first) == 0
+            tried = retried(d, quant, before, lambda h: d.forward(h, 400), lambda h: d.forward(h, first or 1))
+            assert tried >= 7, (quant, first, tried)
+
+
+CHECKS = {f.__name__: f for f in (weights, workspace)}
 
 if __name__ == "__main__":
     CHECKS[sys.argv[3]](Device(sys.argv[1], sys.argv[2]))

@@ -29,3 +29,8 @@ def _run(fake, check):
 def test_weights(fake):
     """Storing weights: all buffers or none, whichever allocation fails."""
     _run(fake, "weights")
+
+
+def test_workspace(fake):
+    """A call that cannot grow the workspace: the next, smaller one finds one that fits it, not parts of two."""
+    _run(fake, "workspace")

@@ -284,6 +284,15 @@ int grow(mi_moe_hybrid* hh, int64_t T, int64_t n, hipStream_t st) {
   return MI_MOE_OK;
 }
 
+// The hot experts' wire arrays on the device, between a store call's copy and
+// the device handle's repack (which ends before its store returns).
+struct HotArrays {
+  std::vector<DBuf> arr;
+  ~HotArrays() {
+    for (DBuf& b : arr) b.release();
+  }
+};
+
 // Split caller arrays [E, ...] (host or device memory) into the compacted hot
 // arrays (device, slot order) and the cold experts' host copies.
 int split_arrays(mi_moe_hybrid* hh, const void* const* src, int narr, int src_on_device, hipStream_t st,
@@ -407,7 +416,8 @@ MI_API int mi_moe_hybrid_store_quantized(mi_moe_hybrid* hh, const void* gate_up_
     return hfail(MI_MOE_EINVAL, "gate_up_d must be float16 or bfloat16");
   hipStream_t st = (hipStream_t)stream;
   const void* src[4] = {gate_up_qs, gate_up_d, down_qs, down_d};
-  std::vector<DBuf> hot;
+  HotArrays ha;
+  std::vector<DBuf>& hot = ha.arr;
   rc = split_arrays(hh, src, 4, src_on_device, st, hot);
   if (rc) return rc;
   if (hh->dev) {
@@ -440,7 +450,8 @@ MI_API int mi_moe_hybrid_store_awq(mi_moe_hybrid* hh, const int32_t* w13_qweight
     return hfail(MI_MOE_EINVAL, "scale dtype must be fp16 or bf16");
   hipStream_t st = (hipStream_t)stream;
   const void* src[6] = {w13_qweight, w13_qzeros, w13_scales, w2_qweight, w2_qzeros, w2_scales};
-  std::vector<DBuf> hot;
+  HotArrays ha;
+  std::vector<DBuf>& hot = ha.arr;
   rc = split_arrays(hh, src, 6, src_on_device, st, hot);
   if (rc) return rc;
   if (hh->dev) {

@@ -47,6 +47,12 @@ int hipFree(void* p) {
   std::free(p);
   return 0;
 }
+int hipHostMalloc(void** p, size_t bytes, unsigned) {
+  const int e = hipMalloc(p, bytes);
+  if (!e) std::memset(*p, 0, bytes);
+  return e;
+}
+int hipHostFree(void* p) { return hipFree(p); }
 int hipMemset(void* p, int v, size_t bytes) {
   std::memset(p, v, bytes);
   const auto it = live.find(p);
@@ -55,10 +61,16 @@ int hipMemset(void* p, int v, size_t bytes) {
   return 0;
 }
 int hipMemcpyAsync(void* d, const void* s, size_t bytes, int, void*) { std::memcpy(d, s, bytes); return 0; }
+int hipMemcpy(void* d, const void* s, size_t bytes, int) { std::memcpy(d, s, bytes); return 0; }
+int hipStreamCreateWithFlags(void** s, unsigned) { *s = std::malloc(1); return 0; }
+int hipStreamDestroy(void* s) { std::free(s); return 0; }
+int hipStreamWaitEvent(void*, void*, unsigned) { return 0; }
+int hipLaunchHostFunc(void*, void (*fn)(void*), void* data) { fn(data); return 0; }
 int hipStreamSynchronize(void* s) { ++syncs; if (!s) clearing = false; return 0; }
 int hipDeviceSynchronize() { clearing = false; return 0; }
 int hipStreamIsCapturing(void*, int* s) { *s = 0; return 0; }
 int hipEventCreate(void** e) { *e = std::malloc(1); return 0; }
+int hipEventCreateWithFlags(void** e, unsigned) { return hipEventCreate(e); }
 int hipEventDestroy(void* e) { std::free(e); return 0; }
 int hipEventRecord(void*, void*) { return 0; }
 int hipEventSynchronize(void*) { return 0; }

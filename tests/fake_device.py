@@ -18,6 +18,8 @@ ARGS = {
     "mi_moe_store_mxfp4": [P, P, P, P, P, I, P], "mi_moe_store_quantized": [P, P, P, P, P, I, I, P],
     "mi_moe_store_awq": [P, P, P, P, P, P, P, I64, I, I, P],
     "mi_moe_quantize_and_store_expert": [P, I64, I, P, I, I, P],
+    "mi_moe_hybrid_create": [I64, I64, I64, I, P, I, ctypes.POINTER(P)], "mi_moe_hybrid_destroy": [P],
+    "mi_moe_hybrid_store_quantized": [P, P, P, P, P, I, I, P], "mi_moe_hybrid_forward": [P, P, P, P, P, I64, I64, I, P],
     "mi_moe_forward": [P, P, P, P, P, I64, I64, I, P],
     "mi_moe_forward_logits": [P, P, P, P, I, I64, I64, I, I, P, P, P],
     "mi_moe_forward_scores": [P, P, P, P, I, I64, I64, P, I, I64, I64, I64, I, F, I, P, P, P],
@@ -130,7 +132,20 @@ def workspace(d):
             assert tried >= 7, (quant, first, tried)
 
 
-CHECKS = {f.__name__: f for f in (weights, workspace)}
+def hybrid_handle(d, quant=Q4_0):
+    mask, h = (ctypes.c_uint8 * 4)(1, 0, 1, 0), P()
+    d.ok("hybrid_create", *SHAPE[quant], quant, mask, 1, ctypes.byref(h))
+    d.ok("hybrid_store_quantized", h, AT, AT, AT, AT, BF16, 0, STREAM)
+    return h
+
+
+def hybrid_leaves_nothing(d):
+    for quant in (Q8_0, Q4_0):
+        d.ok("hybrid_destroy", hybrid_handle(d, quant))
+        assert d.live() == [], d.live()
+
+
+CHECKS = {f.__name__: f for f in (weights, workspace, hybrid_leaves_nothing)}
 
 if __name__ == "__main__":
     CHECKS[sys.argv[3]](Device(sys.argv[1], sys.argv[2]))

@@ -34,3 +34,8 @@ def test_weights(fake):
 def test_workspace(fake):
     """A call that cannot grow the workspace: the next, smaller one finds one that fits it, not parts of two."""
     _run(fake, "workspace")
+
+
+def test_hybrid_leaves_nothing(fake):
+    """The offload executor's handle gives back every allocation, those of its store call too."""
+    _run(fake, "hybrid_leaves_nothing")

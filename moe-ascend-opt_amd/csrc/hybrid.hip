@@ -274,6 +274,7 @@ int grow(mi_moe_hybrid* hh, int64_t T, int64_t n, hipStream_t st) {
     for (PinBuf* b : {&hh->x_h, &hh->part_h, &hh->ids_h, &hh->w_h}) b->retire(hh->retired_pin);
     hh->ids_dev.retire(hh->retired_dev);
   }
+  hh->cap_T = hh->cap_n = 0;   // until every buffer is there
   HCHK(hh->x_h.alloc((size_t)capT * hh->H * 2));
   HCHK(hh->part_h.alloc((size_t)capT * hh->H * sizeof(float)));
   HCHK(hh->ids_h.alloc((size_t)capn * sizeof(int32_t)));

@@ -145,7 +145,26 @@ def hybrid_leaves_nothing(d):
         assert d.live() == [], d.live()
 
 
-CHECKS = {f.__name__: f for f in (weights, workspace, hybrid_leaves_nothing)}
+def hybrid_staging(d):
+    forward = lambda h, T: d.call("hybrid_forward", h, AT, AT, AT, AT, T, 2, BF16, STREAM)
+
+    def left(fail):   # a call, one that fails to grow, and one that fits what the first left
+        h = hybrid_handle(d)
+        assert forward(h, 1) == 0
+        d.f.fake_fail_at(fail)
+        assert fail < 0 or forward(h, 400) == EHIP
+        d.f.fake_fail_at(-1)
+        assert forward(h, 1) == 0
+        sizes = d.live()
+        d.ok("hybrid_destroy", h)
+        return sizes
+    want = left(-1)
+    for fail in range(5):   # the staging buffers; the device handle's workspace is not reached
+        got = left(fail)
+        assert got == want, (fail, got, want)
+
+
+CHECKS = {f.__name__: f for f in (weights, workspace, hybrid_leaves_nothing, hybrid_staging)}
 
 if __name__ == "__main__":
     CHECKS[sys.argv[3]](Device(sys.argv[1], sys.argv[2]))

@@ -39,3 +39,8 @@ def test_workspace(fake):
 def test_hybrid_leaves_nothing(fake):
     """The offload executor's handle gives back every allocation, those of its store call too."""
     _run(fake, "hybrid_leaves_nothing")
+
+
+def test_hybrid_staging(fake):
+    """The executor's staging buffers after a call that could not grow them."""
+    _run(fake, "hybrid_staging")

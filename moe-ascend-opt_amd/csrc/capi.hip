@@ -907,8 +907,8 @@ int picks_buffer(mi_moe_handle* h, int64_t need, hipStream_t st, int32_t*& ids, 
       h->r_rids.retire(h->retired);
       h->r_rw.retire(h->retired);
     }
-    HIPCHK(h->r_rids.alloc((size_t)cap * sizeof(int32_t)));
-    HIPCHK(h->r_rw.alloc((size_t)cap * sizeof(float)));
+    h->cap_r = 0;   // until both are there
+    HIPCHK(alloc_all({{&h->r_rids, (size_t)cap * sizeof(int32_t)}, {&h->r_rw, (size_t)cap * sizeof(float)}}, false));
     h->cap_r = cap;
   }
   ids = (int32_t*)h->r_rids.p;

@@ -65,13 +65,19 @@ class Device:
     def online(self, h, quant):
         return self.call("quantize_and_store_expert", h, 1, 2, AT, F32, 1, STREAM)
 
+    def logits(self, h, T, K=2, ldt=F32, act=BF16, x=AT, y=AT, logits=AT):
+        return self.call("forward_logits", h, x, y, logits, ldt, T, K, 1, act, None, None, STREAM)
+
+    def scores(self, h, T, K=2, ldt=F32, act=BF16, x=AT, y=AT, logits=AT):
+        return self.call("forward_scores", h, x, y, logits, ldt, T, K, None, 1, 1, 1, 1, 1, 1.0, act, None, None, STREAM)
+
     def forward(self, h, T, K=2):
         return self.call("forward", h, AT, AT, AT, AT, T, K, BF16, STREAM)
 
 
-def retried(d, quant, before, call, after):
+def retried(d, quant, before, call, after, first=None):
     """call fails at each of its allocations in turn; `after` on such a handle leaves what it leaves on one where the
-    call was never made."""
+    call was never made.  first: only so many allocations."""
     def run(fail):
         h = d.handle(quant)
         before(h)
@@ -93,7 +99,7 @@ def retried(d, quant, before, call, after):
         assert d.live() == [], "allocations left behind a handle"
         return left
     want, tried = run(None), 0
-    while True:
+    while tried != first:
         got = run(tried)
         if got is None:
             break
@@ -132,6 +138,14 @@ def workspace(d):
             assert tried >= 7, (quant, first, tried)
 
 
+def picks(d):
+    for quant in (Q4_0, W4A16, MXFP4):
+        for call in (d.logits, d.scores):
+            def before(h):
+                assert d.store(h, quant) == 0 and call(h, 1) == 0
+            assert retried(d, quant, before, lambda h: call(h, 2000), lambda h: call(h, 1), first=2) == 2
+
+
 def hybrid_handle(d, quant=Q4_0):
     mask, h = (ctypes.c_uint8 * 4)(1, 0, 1, 0), P()
     d.ok("hybrid_create", *SHAPE[quant], quant, mask, 1, ctypes.byref(h))
@@ -164,7 +178,7 @@ def hybrid_staging(d):
         assert got == want, (fail, got, want)
 
 
-CHECKS = {f.__name__: f for f in (weights, workspace, hybrid_leaves_nothing, hybrid_staging)}
+CHECKS = {f.__name__: f for f in (weights, workspace, picks, hybrid_leaves_nothing, hybrid_staging)}
 
 if __name__ == "__main__":
     CHECKS[sys.argv[3]](Device(sys.argv[1], sys.argv[2]))

@@ -36,6 +36,11 @@ def test_workspace(fake):
     _run(fake, "workspace")
 
 
+def test_picks(fake):
+    """The buffer of a call's router picks after a failed growth."""
+    _run(fake, "picks")
+
+
 def test_hybrid_leaves_nothing(fake):
     """The offload executor's handle gives back every allocation, those of its store call too."""
     _run(fake, "hybrid_leaves_nothing")

@@ -519,9 +519,8 @@ int forward_mx(mi_moe_handle* h, const void* x, void* y, const float* tw, const 
   return MI_MOE_OK;
 }
 
-// Argument checks shared by mi_moe_forward and mi_moe_forward_noalloc.
-int check_forward_args(mi_moe_handle* h, const void* x, void* y, const float* topk_w, const int32_t* topk_ids,
-                       int64_t T, int64_t K, int act_dtype) {
+// Argument checks shared by the forward entry points, all but those of the ids and weights.
+int check_forward_call(mi_moe_handle* h, const void* x, void* y, int64_t T, int64_t K, int act_dtype) {
   int rc = check_handle(h);
   if (rc) return rc;
   if (!h->loaded) return fail(MI_MOE_ENOTLOADED, "weights not stored");
@@ -530,8 +529,32 @@ int check_forward_args(mi_moe_handle* h, const void* x, void* y, const float* to
   if (T < 0 || K < 1 || K > 64) return fail(MI_MOE_EINVAL, "bad T=%lld / top_k=%lld", (long long)T, (long long)K);
   if (T == 0) return MI_MOE_OK;
   if ((int64_t)T * K > (int64_t)1 << 24) return fail(MI_MOE_EINVAL, "T*top_k too large");
-  if (!x || !y || !topk_w || !topk_ids) return fail(MI_MOE_EINVAL, "null data pointer");
+  if (!x || !y) return fail(MI_MOE_EINVAL, "null data pointer");
   if (!aligned16(x) || !aligned16(y)) return fail(MI_MOE_EINVAL, "hidden/out must be 16-byte aligned");
+  return MI_MOE_OK;
+}
+
+// Argument checks shared by mi_moe_forward and mi_moe_forward_noalloc.
+int check_forward_args(mi_moe_handle* h, const void* x, void* y, const float* topk_w, const int32_t* topk_ids,
+                       int64_t T, int64_t K, int act_dtype) {
+  const int rc = check_forward_call(h, x, y, T, K, act_dtype);
+  if (rc || T == 0) return rc;
+  if (!topk_w || !topk_ids) return fail(MI_MOE_EINVAL, "null data pointer");
+  return MI_MOE_OK;
+}
+
+// The logits' dtype of both routers, and the sizes of mi_moe_topk_softmax.
+int check_logits_dtype(int logits_dtype) {
+  if (logits_dtype != MI_MOE_F16 && logits_dtype != MI_MOE_BF16 && logits_dtype != MI_MOE_F32)
+    return fail(MI_MOE_EINVAL, "logits dtype must be fp16, bf16 or fp32");
+  return MI_MOE_OK;
+}
+int check_topk_softmax(int logits_dtype, int64_t T, int64_t E, int64_t K) {
+  const int rc = check_logits_dtype(logits_dtype);
+  if (rc) return rc;
+  if (T < 0 || E < 1 || E > 512) return fail(MI_MOE_EINVAL, "bad T=%lld / E=%lld (E <= 512)", (long long)T, (long long)E);
+  if (K < 1 || K > E || K > 64) return fail(MI_MOE_EINVAL, "top_k=%lld must be in [1, min(E, 64)]", (long long)K);
+  if (T > ((int64_t)1 << 24)) return fail(MI_MOE_EINVAL, "T too large");
   return MI_MOE_OK;
 }
 
@@ -881,12 +904,8 @@ MI_API int mi_moe_forward_noalloc(mi_moe_handle* h, const void* x, void* y, cons
 
 MI_API int mi_moe_topk_softmax(const void* logits, int logits_dtype, int64_t T, int64_t E, int64_t K,
                                int renormalize, int32_t* topk_ids, float* topk_w, void* stream) {
-  if (logits_dtype != MI_MOE_F16 && logits_dtype != MI_MOE_BF16 && logits_dtype != MI_MOE_F32)
-    return fail(MI_MOE_EINVAL, "logits dtype must be fp16, bf16 or fp32");
-  if (T < 0 || E < 1 || E > 512) return fail(MI_MOE_EINVAL, "bad T=%lld / E=%lld (E <= 512)", (long long)T, (long long)E);
-  if (K < 1 || K > E || K > 64) return fail(MI_MOE_EINVAL, "top_k=%lld must be in [1, min(E, 64)]", (long long)K);
-  if (T > ((int64_t)1 << 24)) return fail(MI_MOE_EINVAL, "T too large");
-  if (T == 0) return MI_MOE_OK;
+  const int rc = check_topk_softmax(logits_dtype, T, E, K);
+  if (rc || T == 0) return rc;
   if (!logits || !topk_ids || !topk_w) return fail(MI_MOE_EINVAL, "null pointer");
   HIPCHK(launch_topk_softmax(logits, logits_dtype, (int)T, (int)E, (int)K, renormalize ? 1 : 0, topk_ids, topk_w,
                              (hipStream_t)stream));
@@ -921,8 +940,8 @@ int picks_buffer(mi_moe_handle* h, int64_t need, hipStream_t st, int32_t*& ids, 
 MI_API int mi_moe_topk_scores(const void* logits, int logits_dtype, int64_t T, int64_t E, int64_t K, const float* bias,
                               int score, int64_t n_group, int64_t topk_group, int64_t group_top, int renormalize,
                               float scale, int32_t* topk_ids, float* topk_w, void* stream) {
-  if (logits_dtype != MI_MOE_F16 && logits_dtype != MI_MOE_BF16 && logits_dtype != MI_MOE_F32)
-    return fail(MI_MOE_EINVAL, "logits dtype must be fp16, bf16 or fp32");
+  const int rc = check_logits_dtype(logits_dtype);
+  if (rc) return rc;
   const char* bad = score_args_error(T, E, K, score, n_group, topk_group, group_top);
   if (bad) return fail(MI_MOE_EINVAL, "%s", bad);
   if (T == 0) return MI_MOE_OK;
@@ -945,11 +964,14 @@ MI_API int mi_moe_forward_scores(mi_moe_handle* h, const void* x, void* y, const
   if ((topk_ids_out == nullptr) != (topk_w_out == nullptr))
     return fail(MI_MOE_EINVAL, "topk_ids_out and topk_w_out must both be given or both be null");
   if (!router_logits) return fail(MI_MOE_EINVAL, "null router logits");
+  // nothing is allocated or launched for a call that is refused
+  rc = check_logits_dtype(logits_dtype);
+  if (rc) return rc;
+  rc = check_forward_call(h, x, y, T, K, act_dtype);
+  if (rc) return rc;
   int32_t* ids = topk_ids_out;
   float* w = topk_w_out;
   rc = picks_buffer(h, T * K, (hipStream_t)stream, ids, w);
-  if (rc) return rc;
-  rc = check_forward_args(h, x, y, w, ids, T, K, act_dtype);   // nothing is launched for a call that cannot end
   if (rc) return rc;
   rc = mi_moe_topk_scores(router_logits, logits_dtype, T, h->E, K, bias, score, n_group, topk_group, group_top,
                           renormalize, scale, ids, w, stream);
@@ -1002,6 +1024,11 @@ MI_API int mi_moe_forward_logits(mi_moe_handle* h, const void* x, void* y, const
   if (T == 0) return MI_MOE_OK;
   if ((topk_ids_out == nullptr) != (topk_w_out == nullptr))
     return fail(MI_MOE_EINVAL, "topk_ids_out and topk_w_out must both be given or both be null");
+  if (!router_logits) return fail(MI_MOE_EINVAL, "null router logits");
+  rc = check_topk_softmax(logits_dtype, T, h->E, K);
+  if (rc) return rc;
+  rc = check_forward_call(h, x, y, T, K, act_dtype);
+  if (rc) return rc;
   int32_t* ids = topk_ids_out;
   float* w = topk_w_out;
   rc = picks_buffer(h, T * K, (hipStream_t)stream, ids, w);

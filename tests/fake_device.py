@@ -146,6 +146,32 @@ def picks(d):
             assert retried(d, quant, before, lambda h: call(h, 2000), lambda h: call(h, 1), first=2) == 2
 
 
+def refused(d):
+    odd = P(AT.value + 8)
+    for quant in (Q4_0, W4A16, MXFP4):
+        for call in (d.logits, d.scores):
+            h = d.handle(quant)
+            have, done = d.live(), (d.f.fake_launches(), d.f.fake_syncs())
+            assert call(h, 4096) == 2, "weights not stored"
+
+            def nothing_done(rc, word):
+                assert rc == 1 and word in d.lib.mi_moe_last_error(), (quant, rc, d.lib.mi_moe_last_error())
+                assert d.live() == have and (d.f.fake_launches(), d.f.fake_syncs()) == done, (quant, word)
+            assert d.live() == have and (d.f.fake_launches(), d.f.fake_syncs()) == done
+            assert d.store(h, quant) == 0
+            have, done = d.live(), (d.f.fake_launches(), d.f.fake_syncs())
+            nothing_done(call(h, 1 << 24), b"too large")
+            nothing_done(call(h, 4096, act=7), b"fp16 or bf16")
+            nothing_done(call(h, 4096, ldt=7), b"logits dtype")
+            nothing_done(call(h, 4096, K=SHAPE[quant][0] + 1), b"top_k")
+            nothing_done(call(h, 4096, logits=None), b"null")
+            nothing_done(call(h, 4096, x=None), b"null")
+            nothing_done(call(h, 4096, y=None), b"null")
+            nothing_done(call(h, 4096, x=odd), b"aligned")
+            assert call(h, 0) == 0 and call(h, 4096) == 0
+            d.ok("destroy", h)
+
+
 def hybrid_handle(d, quant=Q4_0):
     mask, h = (ctypes.c_uint8 * 4)(1, 0, 1, 0), P()
     d.ok("hybrid_create", *SHAPE[quant], quant, mask, 1, ctypes.byref(h))
@@ -178,7 +204,7 @@ def hybrid_staging(d):
         assert got == want, (fail, got, want)
 
 
-CHECKS = {f.__name__: f for f in (weights, workspace, picks, hybrid_leaves_nothing, hybrid_staging)}
+CHECKS = {f.__name__: f for f in (weights, workspace, picks, refused, hybrid_leaves_nothing, hybrid_staging)}
 
 if __name__ == "__main__":
     CHECKS[sys.argv[3]](Device(sys.argv[1], sys.argv[2]))

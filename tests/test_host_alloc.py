@@ -41,6 +41,11 @@ def test_picks(fake):
     _run(fake, "picks")
 
 
+def test_refused(fake):
+    """A call behind a router that is refused allocates, launches and waits for nothing."""
+    _run(fake, "refused")
+
+
 def test_hybrid_leaves_nothing(fake):
     """The offload executor's handle gives back every allocation, those of its store call too."""
     _run(fake, "hybrid_leaves_nothing")

@@ -121,6 +121,8 @@ struct BufBytes {
 };
 // All of the buffers (those of 0 bytes are left out) or, where one cannot be
 // had, none: callers take a buffer that is there as a sign that its fellows are.
+// Clears have ended on return, since a caller's stream may not wait for the
+// default one.
 hipError_t alloc_all(std::initializer_list<BufBytes> bufs, bool cleared) {
   hipError_t e = hipSuccess;
   for (const BufBytes& b : bufs) {
@@ -129,6 +131,7 @@ hipError_t alloc_all(std::initializer_list<BufBytes> bufs, bool cleared) {
     if (e == hipSuccess && cleared) e = hipMemset(b.buf->p, 0, b.buf->bytes);
     if (e != hipSuccess) break;
   }
+  if (e == hipSuccess && cleared) e = hipStreamSynchronize(nullptr);
   if (e != hipSuccess)
     for (const BufBytes& b : bufs) b.buf->release();
   return e;
@@ -286,7 +289,8 @@ int init_scratch(int dev) {
   if (e != hipSuccess || p == nullptr)
     return fail(MI_MOE_EHIP, "hipGetSymbolAddress(scratch) failed on device %d: %s", dev, hipGetErrorString(e));
   // the one-launch decode units at the head start zeroed (no dispatch has tag 0)
-  const hipError_t ez = hipMemset(p, 0, tagged_act_bytes(kTagActMaxI));
+  hipError_t ez = hipMemset(p, 0, tagged_act_bytes(kTagActMaxI));
+  if (ez == hipSuccess) ez = hipStreamSynchronize(nullptr);
   if (ez != hipSuccess)
     return fail(MI_MOE_EHIP, "clearing the no-alloc scratch head failed on device %d: %s", dev, hipGetErrorString(ez));
   g_scratch_ptr[dev] = p;
@@ -480,7 +484,6 @@ int mx_alloc_weights(mi_moe_handle* h) {
   // zeros stay where K is no multiple of 128, and in what has not been stored
   HIPCHK(alloc_all({{&h->w13, t13 * kMxTileBytes}, {&h->w13_s, t13 * kMxTileScaleBytes},
                     {&h->w2, t2 * kMxTileBytes}, {&h->w2_s, t2 * kMxTileScaleBytes}}, true));
-  HIPCHK(hipStreamSynchronize(nullptr));   // before the caller's stream, which may not wait for the default one
   return MI_MOE_OK;
 }
 
@@ -632,8 +635,7 @@ MI_API int mi_moe_create(int64_t E, int64_t H, int64_t I, int quant_type, mi_moe
   }
   // the one-launch decode units (zeroed: no dispatch has tag 0)
   if (I <= kTagActMaxI &&
-      (h->tact.alloc(tagged_act_bytes((int)I)) != hipSuccess ||
-       hipMemset(h->tact.p, 0, tagged_act_bytes((int)I)) != hipSuccess)) {
+      alloc_all({{&h->tact, tagged_act_bytes((int)I)}}, true) != hipSuccess) {
     mi_moe_destroy(h);
     return fail(MI_MOE_EHIP, "allocating the decode hand-over buffer failed");
   }

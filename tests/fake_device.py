@@ -172,6 +172,19 @@ def refused(d):
             d.ok("destroy", h)
 
 
+def clears(d):
+    """fake_unordered counts launches while a clear on the default stream may still be running."""
+    for quant in (Q8_0, Q4_0, W4A16, MXFP4):
+        h = d.handle(quant)
+        assert d.store(h, quant) == 0 and d.f.fake_unordered() == 0, ("stored", quant)
+        assert d.forward(h, 1) == 0 and d.f.fake_unordered() == 0, ("forward", quant)
+        d.ok("destroy", h)
+        if quant in (Q8_0, MXFP4):
+            h = d.handle(quant)
+            assert d.online(h, quant) == 0 and d.f.fake_unordered() == 0, ("online", quant)
+            d.ok("destroy", h)
+
+
 def hybrid_handle(d, quant=Q4_0):
     mask, h = (ctypes.c_uint8 * 4)(1, 0, 1, 0), P()
     d.ok("hybrid_create", *SHAPE[quant], quant, mask, 1, ctypes.byref(h))
@@ -204,7 +217,7 @@ def hybrid_staging(d):
         assert got == want, (fail, got, want)
 
 
-CHECKS = {f.__name__: f for f in (weights, workspace, picks, refused, hybrid_leaves_nothing, hybrid_staging)}
+CHECKS = {f.__name__: f for f in (weights, workspace, picks, refused, clears, hybrid_leaves_nothing, hybrid_staging)}
 
 if __name__ == "__main__":
     CHECKS[sys.argv[3]](Device(sys.argv[1], sys.argv[2]))

@@ -46,6 +46,11 @@ def test_refused(fake):
     _run(fake, "refused")
 
 
+def test_clears(fake):
+    """New buffers are clear before the caller's stream, which may not wait for the default one, stores into them."""
+    _run(fake, "clears")
+
+
 def test_hybrid_leaves_nothing(fake):
     """The offload executor's handle gives back every allocation, those of its store call too."""
     _run(fake, "hybrid_leaves_nothing")

@@ -395,7 +395,12 @@ void topk_scores(const float* logits, int64_t T, int64_t E, int64_t K, const flo
     int32_t* oi = ids + t * K;
     float* ow = w + t * K;
     if (sigmoid) {
-      for (int64_t e = 0; e < E; ++e) s[e] = 1.0 / (1.0 + std::exp(-(double)l[e]));
+      // from the exponential of -|l|, which cannot overflow: 1 + exp(-l) would
+      // leave a score of 0 where it is a number below 2^-1022
+      for (int64_t e = 0; e < E; ++e) {
+        const double x = std::exp(-std::fabs((double)l[e])), y = 1.0 / (1.0 + x);
+        s[e] = l[e] < 0.0f ? x * y : y;
+      }
     } else {
       float m = -INFINITY;
       for (int64_t e = 0; e < E; ++e) m = l[e] > m ? l[e] : m;

@@ -277,9 +277,11 @@ int mi_moe_cpu_topk_softmax(const float* logits, int64_t T, int64_t E, int64_t K
  *   topk_w = scale * s, with renormalize scale * s / (sum of the picks' s), 0
  *   where that sum is 0.  The bias only decides the choice.
  * Scores, choices and sums are in 64 bits; topk_w is rounded once.  An expert
- * whose logit (or bias) is -infinity is masked: never picked, -infinity in its
- * group's sum; where fewer than K experts are left the remaining ids are -1,
- * which mi_moe_forward drops, with weight 0.  A token with a NaN score (a NaN
+ * whose logit (or bias) is -infinity is masked: never picked and no part of its
+ * group's sum, which is that of the experts it has left (-infinity of none), so
+ * that a token with an expert left is always routed to one; where fewer than K
+ * experts are left in the chosen groups the remaining ids are -1, which
+ * mi_moe_forward drops, with weight 0.  A token with a NaN score (a NaN
  * logit or bias; an infinite logit under softmax) gets ids 0 .. K-1 and NaN
  * weights.  E <= 512, n_group <= 64, K <= 64.  Stream-ordered, no workspace. */
 int mi_moe_topk_scores(const void* logits, int logits_dtype, int64_t T, int64_t E,

@@ -433,7 +433,7 @@ void topk_scores(const float* logits, int64_t T, int64_t E, int64_t K, const flo
           if (c[e] > b1) { b2 = b1; b1 = c[e]; }
           else if (c[e] > b2) b2 = c[e];
         }
-        g[i] = group_top == 1 ? b1 : b2 == ninf ? ninf : b1 + b2;
+        g[i] = group_top == 1 || b2 == ninf ? b1 : b1 + b2;   // masked experts are no part of it
       }
       for (int64_t i = 0; i < n_group; ++i) {
         int64_t ahead = 0;

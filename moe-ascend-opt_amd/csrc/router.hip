@@ -3,7 +3,8 @@
 // renormalized and scaled weights.
 //
 //   s_e = sigmoid(l_e) or softmax(l)_e,  c_e = s_e + b_e
-//   group score = the sum of the group's group_top largest c (1 or 2)
+//   group score = the sum of the group's group_top largest c (1 or 2), of
+//   the one that is left where the others are masked, -infinity of none
 //   the topk_group groups of the largest scores, in them the K largest c
 //   w_k = scale * s_k / sum of the picks' s  (renormalize), or scale * s_k
 //
@@ -232,7 +233,7 @@ __global__ __launch_bounds__(kScoreWaves * kWave) void topk_scores_kernel(const 
       if (a.group_lanes > 2) merge(x, dpp<kXor2>(x.a), dpp<kXor2>(x.b));
       if (a.group_lanes > 4) merge(x, dpp<kHalfMirror>(x.a), dpp<kHalfMirror>(x.b));
       if (a.group_lanes > 8) merge(x, dpp<kMirror>(x.a), dpp<kMirror>(x.b));
-      const double g = a.group_top == 1 ? x.a : x.b == ninf ? ninf : x.a + x.b;
+      const double g = a.group_top == 1 || x.b == ninf ? x.a : x.a + x.b;
       const int mine = lane / a.group_lanes;
       int ahead = 0;   // groups that come before this lane's
       for (int i = 0; i < a.n_group; ++i) {
@@ -251,7 +252,7 @@ __global__ __launch_bounds__(kScoreWaves * kWave) void topk_scores_kernel(const 
       Top2 x = {ninf, ninf};
       if (lane < a.n_group)
         for (int i = 0; i < gs; ++i) merge(x, cw[lane * gs + i], ninf);
-      const double g = a.group_top == 1 ? x.a : x.b == ninf ? ninf : x.a + x.b;
+      const double g = a.group_top == 1 || x.b == ninf ? x.a : x.a + x.b;
       int ahead = 0;
       for (int i = 0; i < a.n_group; ++i) {
         const double o = lane_value(g, i);
@@ -384,7 +385,7 @@ __global__ __launch_bounds__(kScoreWaves * kWave) void topk_scores_rows_kernel(c
     if (a.group_lanes > 2) merge(x, dpp<kXor2>(x.a), dpp<kXor2>(x.b));
     if (a.group_lanes > 4) merge(x, dpp<kHalfMirror>(x.a), dpp<kHalfMirror>(x.b));
     if (a.group_lanes > 8) merge(x, dpp<kMirror>(x.a), dpp<kMirror>(x.b));
-    const double g = a.group_top == 1 ? x.a : x.b == ninf ? ninf : x.a + x.b;
+    const double g = a.group_top == 1 || x.b == ninf ? x.a : x.a + x.b;
     const int mine = lane / a.group_lanes;
     int ahead = 0;
     for (int i = 0; i < a.n_group; ++i) {

@@ -25,7 +25,8 @@ def route(logits, bias, K, sigmoid, n_group, topk_group, group_top, renorm, scal
         best = []
         for g in range(n_group):
             top = sorted(c[g * n:(g + 1) * n], reverse=True)[:group_top]
-            best.append(-math.inf if -math.inf in top else sum(top))
+            top = [v for v in top if v > -math.inf]   # masked experts are no part of a group's sum
+            best.append(sum(top) if top else -math.inf)
         open_ = sorted(range(n_group), key=lambda g: (-best[g], g))[:topk_group]
         c = [v if e // n in open_ else -math.inf for e, v in enumerate(c)]
     ids = [e for e in sorted(range(E), key=lambda e: (-c[e], e)) if c[e] > -math.inf][:K]

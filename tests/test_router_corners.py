@@ -40,3 +40,43 @@ def test_sigmoid_of_very_low_logits(dev, T):
     x[:, :5] = x[:, 7:] = -750.0
     ids, w = _scores(x.to(dev), 3, None, "sigmoid", 1, 1, 1, True, 2.5)
     assert all(i == [5, 0, 1] for i in ids) and all(v == [2.5, 0.0, 0.0] for v in w), (ids[0], w[0])
+
+
+@pytest.mark.parametrize("T", [1, 3001])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_group_with_one_expert_left(dev, score, T):
+    """A masked expert is out of its group's sum; the group goes on with those it has left."""
+    x = torch.full((T, 64), -INF)
+    x[:, 41] = 0.5
+    for groups, top in ((8, 1), (8, 3), (16, 2), (16, 1), (4, 3)):
+        ids, w = _scores(x.to(dev), 4, None, score, groups, top, 2, True, 1.0)
+        assert all(i == [41, -1, -1, -1] for i in ids) and all(v == [1.0, 0.0, 0.0, 0.0] for v in w), (groups, ids[0])
+    x[:, 0], x[:, 1], x[:, 41] = -9.0, -9.0, 9.0    # two small choices in one group, a large one alone in another
+    ids, _ = _scores(x.to(dev), 2, None, score, 8, 1, 2, False, 1.0)
+    assert all(i == [41, -1] for i in ids), ids[0]
+    x[:, 0], x[:, 1], x[:, 41] = 1.0, 1.0, 1.1      # two that outweigh one a little larger
+    ids, _ = _scores(x.to(dev), 2, None, score, 8, 1, 2, False, 1.0)
+    assert all(i == [0, 1] for i in ids), ids[0]
+
+
+@pytest.mark.parametrize("E,groups,top,K", [(64, 8, 1, 4), (64, 8, 3, 4), (60, 4, 1, 3), (250, 5, 2, 6), (256, 8, 4, 8),
+                                            (128, 16, 4, 8), (512, 64, 9, 10), (511, 7, 1, 3)])
+@pytest.mark.parametrize("T", [40, 3200])
+def test_nothing_routed_to_nothing(dev, E, groups, top, K, T):
+    """A token with an expert left is routed to one, and never to a masked one."""
+    g = torch.Generator().manual_seed(E + groups)
+    x = torch.randn(T, E, generator=g)
+    left = torch.randint(1, 5, (T, 1), generator=g)              # experts left in a row
+    x[torch.rand(T, E, generator=g).argsort(1).argsort(1) >= left] = -INF
+    for score in ("softmax", "sigmoid"):
+        for bias in (None, torch.randn(E, generator=g), torch.full((E,), -3.0)):
+            for group_top in (1, 2):
+                ids, _ = torch.ops.nanovllm.moe_topk_scores(x.to(dev), K, None if bias is None else bias.to(dev), score,
+                                                            groups, top, group_top, True, 1.0)
+                ids = ids.cpu().long()
+                n = (ids >= 0).sum(1)
+                assert bool((n >= 1).all()), (score, group_top, int((n == 0).sum()))
+                assert bool((ids[:, 0] >= 0).all())
+                assert bool(torch.gather(x, 1, ids.clamp_min(0))[ids >= 0].isfinite().all())
+                groups_left = (x.reshape(T, groups, -1) > -INF).any(-1).sum(1)
+                assert bool((n >= torch.minimum(groups_left, torch.tensor(min(top, K)))).all())   # one at least of each group

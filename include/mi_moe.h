@@ -283,7 +283,8 @@ int mi_moe_cpu_topk_softmax(const float* logits, int64_t T, int64_t E, int64_t K
  * experts are left in the chosen groups the remaining ids are -1, which
  * mi_moe_forward drops, with weight 0.  A token with a NaN score (a NaN
  * logit or bias; an infinite logit under softmax) gets ids 0 .. K-1 and NaN
- * weights.  E <= 512, n_group <= 64, K <= 64.  Stream-ordered, no workspace. */
+ * weights.  E <= 512, n_group <= 64, K <= 64; group_top has no meaning where
+ * topk_group is n_group.  Stream-ordered, no workspace. */
 int mi_moe_topk_scores(const void* logits, int logits_dtype, int64_t T, int64_t E,
                        int64_t K, const float* bias, int score, int64_t n_group,
                        int64_t topk_group, int64_t group_top, int renormalize,

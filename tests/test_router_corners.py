@@ -80,3 +80,15 @@ def test_nothing_routed_to_nothing(dev, E, groups, top, K, T):
                 assert bool(torch.gather(x, 1, ids.clamp_min(0))[ids >= 0].isfinite().all())
                 groups_left = (x.reshape(T, groups, -1) > -INF).any(-1).sum(1)
                 assert bool((n >= torch.minimum(groups_left, torch.tensor(min(top, K)))).all())   # one at least of each group
+
+
+def test_group_top_without_groups_to_drop(dev):
+    """Where every group is taken, group_top has no meaning and no limit but its own: groups of one expert run as they are."""
+    f, x = torch.ops.nanovllm.moe_topk_scores, torch.tensor([[0.5, 2.0, -1.0, 1.0]], device=dev)
+    ids, w = f(x[:, :1], 1)
+    assert ids.tolist() == [[0]] and w.tolist() == [[1.0]]
+    for args in ((None, "softmax", 4, 4), (None, "softmax", 4, 4, 1), (None, "softmax")):
+        assert f(x, 3, *args)[0].tolist() == [[1, 3, 0]]
+    for args in ((None, "softmax", 4, 3), (None, "softmax", 4, 4, 3), (None, "softmax", 4, 4, 0)):
+        with pytest.raises(RuntimeError, match="group_top"):
+            f(x, 3, *args)

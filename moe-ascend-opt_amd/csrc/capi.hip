@@ -222,16 +222,16 @@ int ensure_workspace(mi_moe_handle* h, int64_t T, int64_t n, hipStream_t st) {
       b->retire(h->retired);
   }
   h->cap_T = h->cap_n = 0;   // until every buffer is there
-  const bool xq = h->quant != MI_MOE_W4A16;
+  const bool xq = h->quant != MI_MOE_W4A16, mx = h->quant == MI_MOE_MXFP4;   // MX packets hold their scales
   HIPCHK(alloc_all({{&h->act, (size_t)capn * act_row_bytes(h)},
-                    {&h->act_d, (size_t)capn * (h->I / 32) * sizeof(float)},
+                    {&h->act_d, mx ? 0 : (size_t)capn * (h->I / 32) * sizeof(float)},
                     {&h->eout, (size_t)capn * h->H * sizeof(float)},
                     {&h->r_tok, (size_t)capn * sizeof(int32_t)},
                     {&h->r_scat, (size_t)capn * sizeof(int32_t)},
                     {&h->r_tiles, (size_t)gemm_tiles_max(capn, (int)h->E) * 4 * sizeof(int32_t)},
                     {&h->r_chunk, (size_t)route_chunks((int)capn) * h->E * sizeof(int32_t)},
                     {&h->xq, xq ? (size_t)capT * xq_row_bytes(h) : 0},
-                    {&h->xd, xq ? (size_t)capT * (h->H / 32) * sizeof(float) : 0}}, false));
+                    {&h->xd, xq && !mx ? (size_t)capT * (h->H / 32) * sizeof(float) : 0}}, false));
   h->cap_T = capT;
   h->cap_n = capn;
   return MI_MOE_OK;
@@ -324,11 +324,12 @@ size_t carve_work(unsigned char* base, const mi_moe_handle* h, int64_t T, int64_
   w.rg.tiles = (int32_t*)take((size_t)gemm_tiles_max(n, (int)E) * 16);
   w.rg.chunk = (int32_t*)take((size_t)route_chunks((int)n) * E * 4);
   w.act = take((size_t)n * act_row_bytes(h));
-  w.act_d = (float*)take((size_t)n * (I / 32) * 4);
+  const bool mx = h->quant == MI_MOE_MXFP4;   // MX packets hold their scales
+  if (!mx) w.act_d = (float*)take((size_t)n * (I / 32) * 4);
   w.eout = need_eout ? (float*)take((size_t)n * H * 4) : nullptr;
   if (h->quant != MI_MOE_W4A16) {
     w.xq = (int8_t*)take((size_t)T * xq_row_bytes(h));
-    w.xd = (float*)take((size_t)T * (H / 32) * 4);
+    if (!mx) w.xd = (float*)take((size_t)T * (H / 32) * 4);
   }
   return off;
 }

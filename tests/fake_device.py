@@ -20,6 +20,7 @@ ARGS = {
     "mi_moe_quantize_and_store_expert": [P, I64, I, P, I, I, P],
     "mi_moe_hybrid_create": [I64, I64, I64, I, P, I, ctypes.POINTER(P)], "mi_moe_hybrid_destroy": [P],
     "mi_moe_hybrid_store_quantized": [P, P, P, P, P, I, I, P], "mi_moe_hybrid_forward": [P, P, P, P, P, I64, I64, I, P],
+    "mi_moe_forward_noalloc": [P, P, P, P, P, I64, I64, I, P],
     "mi_moe_forward": [P, P, P, P, P, I64, I64, I, P],
     "mi_moe_forward_logits": [P, P, P, P, I, I64, I64, I, I, P, P, P],
     "mi_moe_forward_scores": [P, P, P, P, I, I64, I64, P, I, I64, I64, I64, I, F, I, P, P, P],
@@ -185,6 +186,30 @@ def clears(d):
             d.ok("destroy", h)
 
 
+def mx_workspace(d):
+    """What an MXFP4 layer reads: packets of 32 bytes a block (rows in whole 128s), fp32 outputs, routing; no block
+    scales beside them."""
+    E, H, I_ = SHAPE[MXFP4]
+    h = d.handle(MXFP4)
+    assert d.store(h, MXFP4) == 0
+    have = d.live()
+    d.ok("reserve", h, 512, 2, STREAM)
+    new = d.live()
+    for b in have:
+        new.remove(b)
+    big = sorted(b[0] for b in new if b[0] > 8192)
+    assert big == sorted([1024 * 128, 512 * 256, 1024 * H * 4]), big   # intermediate, hidden rows, outputs
+    assert not any(b[0] in (1024 * I_ // 32 * 4, 512 * H // 32 * 4) for b in new), new
+    d.ok("destroy", h)
+    # 7000 rows of I = 4096 fit the array of the call without allocation: 4096 + 256 + 128 bytes each, and routing
+    h = P()
+    d.ok("create", 2, 64, 4096, MXFP4, ctypes.byref(h))
+    assert d.store(h, MXFP4) == 0
+    assert d.call("forward_noalloc", h, AT, AT, AT, AT, 7000, 1, BF16, STREAM) == 0, d.lib.mi_moe_last_error()
+    assert d.call("forward_noalloc", h, AT, AT, AT, AT, 7600, 1, BF16, STREAM) == 1
+    d.ok("destroy", h)
+
+
 def hybrid_handle(d, quant=Q4_0):
     mask, h = (ctypes.c_uint8 * 4)(1, 0, 1, 0), P()
     d.ok("hybrid_create", *SHAPE[quant], quant, mask, 1, ctypes.byref(h))
@@ -217,7 +242,7 @@ def hybrid_staging(d):
         assert got == want, (fail, got, want)
 
 
-CHECKS = {f.__name__: f for f in (weights, workspace, picks, refused, clears, hybrid_leaves_nothing, hybrid_staging)}
+CHECKS = {f.__name__: f for f in (weights, workspace, picks, refused, clears, mx_workspace, hybrid_leaves_nothing, hybrid_staging)}
 
 if __name__ == "__main__":
     CHECKS[sys.argv[3]](Device(sys.argv[1], sys.argv[2]))

@@ -51,6 +51,11 @@ def test_clears(fake):
     _run(fake, "clears")
 
 
+def test_mx_workspace(fake):
+    """An MXFP4 handle's workspace holds what its kernels use, and calls without allocation take what fits."""
+    _run(fake, "mx_workspace")
+
+
 def test_hybrid_leaves_nothing(fake):
     """The offload executor's handle gives back every allocation, those of its store call too."""
     _run(fake, "hybrid_leaves_nothing")

@@ -274,9 +274,9 @@ __host__ __device__ constexpr size_t mx_row_bytes(int K) { return (size_t)mx_kti
 
 // Rows per expert on average from which the grouped products (mx.hip) take
 // items of 128 rows.  us a call, 64-row / 128-row items, H=2048 I=768 E=128
-// top-8: 9 rows 75 / 79, 16 rows 78 / 81, 32 rows 103 / 88, 94 rows 147 / 124;
-// 12 rows Zipf-routed 86 / 78; H=4096 I=768 E=16 top-2: 11 rows 32 / 33,
-// Zipf-routed 55 / 37 (an expert's many rows read its weights half as often).
+// top-8: 9 rows 78 / 81, 16 rows 82 / 85, 32 rows 108 / 97, 94 rows 163 / 139;
+// 12 rows Zipf-routed 95 / 92; H=4096 I=768 E=16 top-2: 11 rows 45 / 45,
+// Zipf-routed 68 / 48 (an expert's many rows read its weights half as often).
 constexpr int kMxBigRows = 10;
 inline bool mx_big(int64_t n, int64_t E) { return n >= kMxBigRows * E; }
 
@@ -303,8 +303,8 @@ struct MxArgs {
 // A token's down workgroups read their experts' weights for themselves, the
 // sorted path reads an expert's once: with more pairs than experts the bytes
 // read again decide.  us a call, decode / sorted: H=4096 I=1408 E=16 top-2,
-// 32 pairs (49 MB read again) 50 / 53, 64 pairs (147 MB) 81 / 54; H=2048 I=768
-// E=16 top-4, 64 pairs (40 MB) 20 / 25; E=128 top-8, 64 pairs (0) 31 / 43.
+// 32 pairs (49 MB read again) 49 / 50, 64 pairs (147 MB) 79 / 47; H=2048 I=768
+// E=16 top-4, 64 pairs (40 MB) 20 / 30; E=128 top-8, 64 pairs (0) 30 / 40.
 constexpr int64_t kMxDecodeAgain = 64 << 20;
 inline bool mx_decode_ok(int64_t n, int64_t K, int64_t E, int64_t H, int64_t I) {
   return n <= 64 && K <= 16 && (n <= E || (n - E) * (H * I / 32 * 17) <= kMxDecodeAgain);

@@ -236,9 +236,9 @@ __device__ __forceinline__ void mx_gemm_item(const MxArgs& a, unsigned char* sme
 
 // 64-row items at four waves per SIMD, 128-row items at two (twice the accumulators).
 //
-// gate_up / down, H=2048 I=768 E=128 top-8: T = 333 skewed 43 / 30 us, 5.0 /
-// 3.6 TB/s of weights, the memory rate; T = 4096 95 / 118 us, 2.2 / 0.9 PFLOP/s:
-// the K loop alone runs at 5 (the instruction in registers at 5.9), the items'
+// gate_up / down, H=2048 I=768 E=128 top-8: T = 333 skewed 49 / 40 us, 4.4 TB/s
+// of weights and 3.2 of weights and outputs; T = 4096 94 / 116 us, 2.2 / 0.9
+// PFLOP/s: the K loop alone runs at 5 (the instruction in registers at 5.9), the items'
 // first loads and their epilogues, gate_up's quantization and down's 268 MB
 // of expert outputs, take the rest.
 template <bool DOWN>

@@ -15,9 +15,11 @@
 // them in the grid; a block travels as 8 tagged 8-byte units (handover.hpp):
 // 6 words of codes, the scale byte, one word unused.  Two launches otherwise.
 //
-// One launch, H=2048 I=768 E=128 top-8: T = 1 8.6 us for 20 MB, bound by its
-// chain (ids, rows, weights, the sums' meeting, the hand-over, down); T = 8
-// 23.4 us for the weights of some 50 experts, 5.5 TB/s.
+// One launch, H=2048 I=768 E=128 top-8, weights that no cache holds: T = 1
+// 10.6 us for 20 MB, bound by its chain (ids, rows, weights, the sums' meeting,
+// the hand-over, down); T = 8 28 us for the weights of some 50 experts, 4.6
+// TB/s.  Two launches, H=2048 I=512 E=128 top-10: T = 1 6.1 + 5.1 us, T = 6
+// 15.7 + 11.2 us for some 50 experts, 3.1 TB/s.
 #pragma clang fp contract(off)
 #include "handover.hpp"
 #include "mi_moe_sched.hpp"

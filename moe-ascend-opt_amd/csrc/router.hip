@@ -26,7 +26,7 @@ constexpr int kScoreWaves = 4;
 constexpr int kScoreMaxE = 512;
 // Tokens from which a row of 16 lanes takes one (topk_scores_rows_kernel),
 // not a wave.  us, row / wave: E=256 top-8 in groups T = 2048 7.1 / 6.2, 4096
-// 7.2 / 8.5, 16384 16.3 / 22.6; E=128 top-8 2048 4.4 / 4.3, 4096 4.5 / 6.0;
+// 7.2 / 8.5, 16384 15.4 / 22.6; E=128 top-8 2048 4.4 / 4.3, 4096 4.5 / 6.0;
 // E=64 top-6 1024 3.4 / 3.2, 4096 3.5 / 4.6, 100000 24 / 55.
 constexpr int kScoreRowsT = 3000;
 
@@ -172,7 +172,9 @@ __device__ __forceinline__ void load_lane(const void* logits, const float* bias,
 // it), and only where several experts reach it in 64 bits among them.
 //
 // Bound by a chain of dependent steps, the 64-bit scores and K maxima: T = 1
-// E = 256 top-8 in 8 groups 4.2 us.
+// E = 256 top-8 in 8 groups 4.2 us, E = 512 5.7, E = 384 (groups through LDS)
+// 7.5.  More than 256 experts take it at any T: T = 16384 top-8 in 8 groups
+// E = 512 36 us, E = 384 45 us.
 template <int LDT, int NJ>   // logits: 0 fp16, 1 bf16, 2 fp32; NJ = ceil(E / 64), a power of two
 __global__ __launch_bounds__(kScoreWaves * kWave) void topk_scores_kernel(const void* __restrict__ logits, const float* __restrict__ bias,
                                                                           ScoreArgs a, int32_t* __restrict__ ids_out,
@@ -322,7 +324,8 @@ __global__ __launch_bounds__(kScoreWaves * kWave) void topk_scores_kernel(const 
 // order of the other kernel: the same bits.
 //
 // Bound by vector issue, about half of it the scores, half the picks:
-// T = 16384 E = 256 top-8 bf16 in 8 groups 16 us (reading its 8 MB: 2 us).
+// T = 16384 E = 256 top-8 bf16 in 8 groups 15.4 us a call (17.1 traced by
+// itself; reading its 8 MB: 2 us).
 //
 // Choices are compared as integers that order like their fp32 roundings; 0
 // is one that is taken.

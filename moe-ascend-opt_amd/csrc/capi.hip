@@ -110,7 +110,12 @@ struct DevBuf {
     release();
     if (b == 0) b = 256;
     hipError_t e = hipMalloc(&p, b);
-    if (e == hipSuccess) bytes = b;
+    if (e == hipSuccess) {
+      bytes = b;
+    } else {
+      p = nullptr;
+      (void)hipGetLastError();   // reported here, not by the next check of a launch
+    }
     return e;
   }
 };

@@ -66,7 +66,12 @@ struct DBuf {
   hipError_t alloc(size_t b) {
     release();
     hipError_t e = hipMalloc(&p, b ? b : 256);
-    if (e == hipSuccess) bytes = b; else p = nullptr;
+    if (e == hipSuccess) {
+      bytes = b;
+    } else {
+      p = nullptr;
+      (void)hipGetLastError();   // reported here, not by the next check of a launch
+    }
     return e;
   }
   void release() {
@@ -87,7 +92,12 @@ struct PinBuf {
   hipError_t alloc(size_t b) {
     release();
     hipError_t e = hipHostMalloc(&p, b ? b : 256, hipHostMallocDefault);
-    if (e == hipSuccess) bytes = b; else p = nullptr;
+    if (e == hipSuccess) {
+      bytes = b;
+    } else {
+      p = nullptr;
+      (void)hipGetLastError();   // reported here, not by the next check of a launch
+    }
     return e;
   }
   void release() {

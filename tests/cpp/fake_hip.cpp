@@ -9,6 +9,7 @@ namespace {
 struct Block { size_t bytes; bool cleared; };
 std::map<void*, Block> live;
 long fail_at = -1, mallocs = 0, launches = 0, syncs = 0;
+int last_error = 0;     // kept until hipGetLastError takes it
 int unordered = 0;      // launches while a clear on the default stream may still run
 bool clearing = false;
 struct Dim3 { unsigned x, y, z; };
@@ -18,6 +19,7 @@ constexpr int kOutOfMemory = 2;
 
 extern "C" {
 // ---------------------------------------------------------------- for the tests
+int fake_last_error() { return last_error; }
 void fake_fail_at(long n) { fail_at = n; mallocs = 0; }   // the n-th allocation from now on fails (-1: none)
 long fake_mallocs() { return mallocs; }
 long fake_launches() { return launches; }
@@ -37,7 +39,7 @@ int hipGetDevice(int* d) { *d = 0; return 0; }
 int hipDeviceGetAttribute(int* v, int, int) { *v = 65536; return 0; }
 int hipMalloc(void** p, size_t bytes) {
   *p = nullptr;
-  if (mallocs++ == fail_at) return kOutOfMemory;
+  if (mallocs++ == fail_at) return last_error = kOutOfMemory;
   *p = std::malloc(bytes);
   live[*p] = Block{bytes, false};
   return 0;
@@ -81,7 +83,11 @@ int hipGetSymbolAddress(void** p, const void*) {
   return 0;
 }
 int hipFuncSetAttribute(const void*, int, int) { return 0; }
-int hipGetLastError() { return 0; }
+int hipGetLastError() {
+  const int e = last_error;
+  last_error = 0;
+  return e;
+}
 const char* hipGetErrorString(int e) { return e ? "out of memory" : "no error"; }
 int __hipPushCallConfiguration(Dim3 g, Dim3 b, size_t shared, void* stream) {
   config = Config{g, b, shared, stream};

@@ -93,6 +93,7 @@ def retried(d, quant, before, call, after, first=None):
                 d.ok("destroy", h)
                 return None
             assert rc == EHIP, rc
+            assert d.f.fake_last_error() == 0, "the caller's next check of a launch reports it"
         rc = after(h)
         assert rc == 0, (fail, rc, d.lib.mi_moe_last_error())
         left = d.live()
@@ -231,6 +232,7 @@ def hybrid_staging(d):
         assert forward(h, 1) == 0
         d.f.fake_fail_at(fail)
         assert fail < 0 or forward(h, 400) == EHIP
+        assert d.f.fake_last_error() == 0
         d.f.fake_fail_at(-1)
         assert forward(h, 1) == 0
         sizes = d.live()

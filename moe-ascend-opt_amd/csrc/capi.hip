@@ -128,7 +128,7 @@ struct BufBytes {
 // had, none: callers take a buffer that is there as a sign that its fellows are.
 // Clears have ended on return, since a caller's stream may not wait for the
 // default one.
-hipError_t alloc_all(std::initializer_list<BufBytes> bufs, bool cleared) {
+int alloc_all(const char* what, std::initializer_list<BufBytes> bufs, bool cleared) {
   hipError_t e = hipSuccess;
   for (const BufBytes& b : bufs) {
     if (!b.bytes) continue;
@@ -137,9 +137,13 @@ hipError_t alloc_all(std::initializer_list<BufBytes> bufs, bool cleared) {
     if (e != hipSuccess) break;
   }
   if (e == hipSuccess && cleared) e = hipStreamSynchronize(nullptr);
-  if (e != hipSuccess)
-    for (const BufBytes& b : bufs) b.buf->release();
-  return e;
+  if (e == hipSuccess) return MI_MOE_OK;
+  size_t bytes = 0;
+  for (const BufBytes& b : bufs) {
+    b.buf->release();
+    bytes += b.bytes;
+  }
+  return fail(MI_MOE_EHIP, "allocating %s (%zu bytes) failed: %s", what, bytes, hipGetErrorString(e));
 }
 
 // Scoped temporary device copy of a caller buffer (host or device source).
@@ -211,9 +215,11 @@ size_t xq_row_bytes(const mi_moe_handle* h) { return h->quant == MI_MOE_MXFP4 ? 
 
 int ensure_workspace(mi_moe_handle* h, int64_t T, int64_t n, hipStream_t st) {
   if (h->r_U.p == nullptr) {
-    HIPCHK(alloc_all({{&h->r_counts, (size_t)h->E * sizeof(int32_t)}, {&h->r_starts, (size_t)(h->E + 1) * sizeof(int32_t)},
-                      {&h->r_active, (size_t)h->E * sizeof(int32_t)}, {&h->r_U, sizeof(int32_t)},
-                      {&h->r_ntiles, sizeof(int32_t)}}, false));
+    const int rc = alloc_all("the routing counters",
+                             {{&h->r_counts, (size_t)h->E * sizeof(int32_t)}, {&h->r_starts, (size_t)(h->E + 1) * sizeof(int32_t)},
+                              {&h->r_active, (size_t)h->E * sizeof(int32_t)}, {&h->r_U, sizeof(int32_t)},
+                              {&h->r_ntiles, sizeof(int32_t)}}, false);
+    if (rc) return rc;
   }
   if (T <= h->cap_T && n <= h->cap_n) return MI_MOE_OK;
   int64_t capT = h->cap_T ? h->cap_T : 16;
@@ -228,15 +234,17 @@ int ensure_workspace(mi_moe_handle* h, int64_t T, int64_t n, hipStream_t st) {
   }
   h->cap_T = h->cap_n = 0;   // until every buffer is there
   const bool xq = h->quant != MI_MOE_W4A16, mx = h->quant == MI_MOE_MXFP4;   // MX packets hold their scales
-  HIPCHK(alloc_all({{&h->act, (size_t)capn * act_row_bytes(h)},
-                    {&h->act_d, mx ? 0 : (size_t)capn * (h->I / 32) * sizeof(float)},
-                    {&h->eout, (size_t)capn * h->H * sizeof(float)},
-                    {&h->r_tok, (size_t)capn * sizeof(int32_t)},
-                    {&h->r_scat, (size_t)capn * sizeof(int32_t)},
-                    {&h->r_tiles, (size_t)gemm_tiles_max(capn, (int)h->E) * 4 * sizeof(int32_t)},
-                    {&h->r_chunk, (size_t)route_chunks((int)capn) * h->E * sizeof(int32_t)},
-                    {&h->xq, xq ? (size_t)capT * xq_row_bytes(h) : 0},
-                    {&h->xd, xq && !mx ? (size_t)capT * (h->H / 32) * sizeof(float) : 0}}, false));
+  const int rc = alloc_all("the workspace",
+                           {{&h->act, (size_t)capn * act_row_bytes(h)},
+                            {&h->act_d, mx ? 0 : (size_t)capn * (h->I / 32) * sizeof(float)},
+                            {&h->eout, (size_t)capn * h->H * sizeof(float)},
+                            {&h->r_tok, (size_t)capn * sizeof(int32_t)},
+                            {&h->r_scat, (size_t)capn * sizeof(int32_t)},
+                            {&h->r_tiles, (size_t)gemm_tiles_max(capn, (int)h->E) * 4 * sizeof(int32_t)},
+                            {&h->r_chunk, (size_t)route_chunks((int)capn) * h->E * sizeof(int32_t)},
+                            {&h->xq, xq ? (size_t)capT * xq_row_bytes(h) : 0},
+                            {&h->xd, xq && !mx ? (size_t)capT * (h->H / 32) * sizeof(float) : 0}}, false);
+  if (rc) return rc;
   h->cap_T = capT;
   h->cap_n = capn;
   return MI_MOE_OK;
@@ -428,11 +436,10 @@ int forward_w4a16(mi_moe_handle* h, const void* x, void* y, const float* tw, con
 int q_alloc_weights(mi_moe_handle* h) {
   const int64_t E = h->E, H = h->H, I = h->I;
   const int64_t bb = h->quant == MI_MOE_Q8_0 ? 2048 : 1024;  // bytes per (tile, block)
-  HIPCHK(alloc_all({{&h->w13, (size_t)E * (I / 32) * (H / 32) * bb},
-                    {&h->w13_s, (size_t)E * (I / 32) * (H / 32) * 64 * 2},
-                    {&h->w2, (size_t)E * (H / 64) * (I / 32) * bb},
-                    {&h->w2_s, (size_t)E * (H / 64) * (I / 32) * 64 * 2}}, true));
-  return MI_MOE_OK;
+  return alloc_all("weights", {{&h->w13, (size_t)E * (I / 32) * (H / 32) * bb},
+                               {&h->w13_s, (size_t)E * (I / 32) * (H / 32) * 64 * 2},
+                               {&h->w2, (size_t)E * (H / 64) * (I / 32) * bb},
+                               {&h->w2_s, (size_t)E * (H / 64) * (I / 32) * 64 * 2}}, true);
 }
 
 int forward_q(mi_moe_handle* h, const void* x, void* y, const float* tw, const int32_t* ids,
@@ -488,9 +495,8 @@ int forward_q(mi_moe_handle* h, const void* x, void* y, const float* tw, const i
 int mx_alloc_weights(mi_moe_handle* h) {
   const size_t E = (size_t)h->E, t13 = E * (h->I / 32) * mx_ktiles((int)h->H), t2 = E * (h->H / 64) * mx_ktiles((int)h->I);
   // zeros stay where K is no multiple of 128, and in what has not been stored
-  HIPCHK(alloc_all({{&h->w13, t13 * kMxTileBytes}, {&h->w13_s, t13 * kMxTileScaleBytes},
-                    {&h->w2, t2 * kMxTileBytes}, {&h->w2_s, t2 * kMxTileScaleBytes}}, true));
-  return MI_MOE_OK;
+  return alloc_all("weights", {{&h->w13, t13 * kMxTileBytes}, {&h->w13_s, t13 * kMxTileScaleBytes},
+                               {&h->w2, t2 * kMxTileBytes}, {&h->w2_s, t2 * kMxTileScaleBytes}}, true);
 }
 
 int forward_mx(mi_moe_handle* h, const void* x, void* y, const float* tw, const int32_t* ids, int64_t T, int64_t K,
@@ -641,9 +647,10 @@ MI_API int mi_moe_create(int64_t E, int64_t H, int64_t I, int quant_type, mi_moe
   }
   // the one-launch decode units (zeroed: no dispatch has tag 0)
   if (I <= kTagActMaxI &&
-      alloc_all({{&h->tact, tagged_act_bytes((int)I)}}, true) != hipSuccess) {
+      alloc_all("the decode hand-over buffer", {{&h->tact, tagged_act_bytes((int)I)}}, true) != MI_MOE_OK) {
+    const std::string msg = g_err;
     mi_moe_destroy(h);
-    return fail(MI_MOE_EHIP, "allocating the decode hand-over buffer failed");
+    return fail(MI_MOE_EHIP, "%s", msg.c_str());
   }
   // the no-alloc entry point's scratch address on this device (once per device)
   if (init_scratch(h->device) != MI_MOE_OK) {
@@ -729,10 +736,11 @@ MI_API int mi_moe_store_awq(mi_moe_handle* h, const int32_t* w13_q, const int32_
   HIPCHK(f.stage(w2_s, s2, src_on_device, st));
   const int64_t NT13 = 2 * (I / 16), G1 = H / 128, CH = I / 32, MQ = H / 64, G2 = I / 128;
   if (!h->w13.p) {
-    HIPCHK(alloc_all({{&h->w13, (size_t)E * NT13 * G1 * 1024},
-                      {&h->w13_s, (size_t)E * (I / 16) * 80 * G1},   // metadata blocks
-                      {&h->w2, (size_t)E * CH * MQ * 1024},
-                      {&h->w2_s, (size_t)E * MQ * 4 * w2_meta_sec_bytes((int)G2)}}, false));   // metadata sections
+    rc = alloc_all("weights", {{&h->w13, (size_t)E * NT13 * G1 * 1024},
+                               {&h->w13_s, (size_t)E * (I / 16) * 80 * G1},   // metadata blocks
+                               {&h->w2, (size_t)E * CH * MQ * 1024},
+                               {&h->w2_s, (size_t)E * MQ * 4 * w2_meta_sec_bytes((int)G2)}}, false);   // metadata sections
+    if (rc) return rc;
   } else {
     HIPCHK(hipDeviceSynchronize());   // the weights that are replaced may be in use on any stream
   }
@@ -935,7 +943,9 @@ int picks_buffer(mi_moe_handle* h, int64_t need, hipStream_t st, int32_t*& ids, 
       h->r_rw.retire(h->retired);
     }
     h->cap_r = 0;   // until both are there
-    HIPCHK(alloc_all({{&h->r_rids, (size_t)cap * sizeof(int32_t)}, {&h->r_rw, (size_t)cap * sizeof(float)}}, false));
+    const int rc = alloc_all("router picks", {{&h->r_rids, (size_t)cap * sizeof(int32_t)}, {&h->r_rw, (size_t)cap * sizeof(float)}},
+                             false);
+    if (rc) return rc;
     h->cap_r = cap;
   }
   ids = (int32_t*)h->r_rids.p;

@@ -92,7 +92,7 @@ def retried(d, quant, before, call, after, first=None):
                 assert rc == 0
                 d.ok("destroy", h)
                 return None
-            assert rc == EHIP, rc
+            assert rc == EHIP and b"out of memory" in d.lib.mi_moe_last_error(), (rc, d.lib.mi_moe_last_error())
             assert d.f.fake_last_error() == 0, "the caller's next check of a launch reports it"
         rc = after(h)
         assert rc == 0, (fail, rc, d.lib.mi_moe_last_error())

@@ -325,6 +325,71 @@ int mi_moe_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t ro
                          int64_t cols, int format, void* out, int dtype,
                          void* stream);
 
+/* ------------------------------------------------------------------------
+ * Products on rows sorted by expert (ragged groups), for weights in 16 bits
+ * with their gradients, and for int8 weights.  No reference counterpart: the
+ * parts of an expert layer for callers that build their own.
+ *   starts [E+1] int32 on the device, ascending, as mi_moe_route writes them:
+ *   rows starts[e] <= r < starts[e+1] belong to expert e.  It is read as its
+ *   running maximum within [0, M], so any contents are safe; outputs of rows
+ *   that belong to no expert are 0.  An expert may have no rows.
+ * Strides count elements.  x, dy and w are read in 16-byte pieces: their
+ * addresses, row lengths and strides are multiples of 16 bytes (8 elements of
+ * 16 bits, 16 of int8).  M <= 2^26, N and K <= 2^20, E <= 512.  Sums are in
+ * fp32 (int32 for int8), in an order that the sizes alone decide, and rounded
+ * once.  Each call is one launch, stream-ordered, without a workspace; it can be
+ * captured into a graph.  Calls may overlap. */
+
+/* y[r] = W[e] x[r]: x [M,K], w [E,N,K] fp16 or bf16 -> y [M,N], contiguous, of
+ * the same type. */
+int mi_moe_grouped_matmul(const void* x, int64_t x_stride, const void* w,
+                          int64_t w_expert_stride, int64_t w_stride,
+                          const int32_t* starts, int64_t M, int64_t N, int64_t K,
+                          int64_t E, int dtype, void* y, void* stream);
+
+/* Its gradient of x: dx[r] = W[e]^T dy[r], dy [M,N] -> dx [M,K], contiguous. */
+int mi_moe_grouped_matmul_dx(const void* dy, int64_t dy_stride, const void* w,
+                             int64_t w_expert_stride, int64_t w_stride,
+                             const int32_t* starts, int64_t M, int64_t N, int64_t K,
+                             int64_t E, int dtype, void* dx, void* stream);
+
+/* Its gradient of w: dw[e] = sum over e's rows of dy[r] x[r]^T -> dw [E,N,K],
+ * contiguous; 0 for an expert without rows. */
+int mi_moe_grouped_matmul_dw(const void* dy, int64_t dy_stride, const void* x,
+                             int64_t x_stride, const int32_t* starts, int64_t M,
+                             int64_t N, int64_t K, int64_t E, int dtype, void* dw,
+                             void* stream);
+
+/* y[r][n] = sum_k x[r][k] w[e][n][k] * w_scales[e][n] * x_scales[r]: x [M,K],
+ * w [E,N,K] int8, x_scales [M], w_scales [E,N] fp32 -> y [M,N] fp16, bf16 or
+ * fp32 (out_dtype), contiguous.  The sum is exact (K <= 131056). */
+int mi_moe_grouped_matmul_int8(const int8_t* x, int64_t x_stride, const float* x_scales,
+                               const int8_t* w, int64_t w_expert_stride, int64_t w_stride,
+                               const float* w_scales, const int32_t* starts, int64_t M,
+                               int64_t N, int64_t K, int64_t E, int out_dtype, void* y,
+                               void* stream);
+
+/* The same with one weight for all rows: w [N,K], w_scales [N], and bias [N]
+ * fp32 (or null) added in fp32 before the one rounding. */
+int mi_moe_int8_matmul(const int8_t* x, int64_t x_stride, const float* x_scales,
+                       const int8_t* w, int64_t w_stride, const float* w_scales,
+                       const float* bias, int64_t M, int64_t N, int64_t K, int out_dtype,
+                       void* y, void* stream);
+
+/* int8 codes with a scale for each row: x, rows of cols values (fp16, bf16 or
+ * fp32) row_stride elements apart -> codes [rows,cols], scales [rows] fp32.
+ *   scale = max(amax / 127, 2^-126), rounded to fp32
+ *   code  = the integer nearest to x / scale, ties to even
+ * A row with a NaN or an infinity gets scale NaN and codes 0.  Any cols, stride
+ * and alignment (multiples of 16 bytes are read in whole pieces). */
+int mi_moe_int8_quantize(const void* x, int dtype, int64_t rows, int64_t cols,
+                         int64_t row_stride, int8_t* codes, float* scales, void* stream);
+
+/* out = code * scale, the product in fp32 (fp16: the exact one), rounded to
+ * dtype: out [rows,cols] fp16, bf16 or fp32. */
+int mi_moe_int8_dequantize(const int8_t* codes, const float* scales, int64_t rows,
+                           int64_t cols, void* out, int dtype, void* stream);
+
 /* Router top-k + softmax followed by mi_moe_forward on the same stream:
  * router_logits [T,E] with E the handle's expert count.  The picks go to
  * topk_ids_out / topk_w_out ([T,K], device) when both are given, else to a

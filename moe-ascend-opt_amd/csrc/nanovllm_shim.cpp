@@ -14,6 +14,7 @@
 // or with MIMOE_HOST_WEIGHTS=1; never with MIMOE_HOST_WEIGHTS=0).
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/custom_class.h>
 #include <tuple>
 #include <optional>
@@ -446,6 +447,212 @@ at::Tensor mx_dequantize_hip(const at::Tensor& codes, const at::Tensor& scales, 
   return out;
 }
 
+// ------------------------------------------------------------------ products on rows sorted by expert
+// An operand of the products: rows of whole 16-byte pieces (`per16` elements).
+// A view that has them is read in place; others are copied, with zeros behind
+// the values of a row where its length is no multiple.
+at::Tensor rows16(const at::Tensor& t, int64_t per16) {
+  const int64_t d = t.dim(), n = t.size(-1);
+  bool ok = t.stride(-1) == 1 && n % per16 == 0 && aligned16(t.data_ptr());
+  if (t.size(d - 2) > 1) ok = ok && t.stride(d - 2) >= n && t.stride(d - 2) % per16 == 0 && t.stride(d - 2) <= (1 << 22);
+  if (d == 3 && t.size(0) > 1) ok = ok && t.stride(0) >= 0 && t.stride(0) % per16 == 0;
+  if (ok) return t;
+  if (n % per16) return at::constant_pad_nd(t, {0, per16 - n % per16}).contiguous();
+  return t.is_contiguous() ? t.clone(at::MemoryFormat::Contiguous) : t.contiguous();
+}
+int64_t row_stride(const at::Tensor& t) { return t.size(t.dim() - 2) > 1 ? t.stride(t.dim() - 2) : t.size(-1); }
+int64_t expert_stride(const at::Tensor& w) { return w.size(0) > 1 ? w.stride(0) : 0; }
+
+void check_starts(const at::Tensor& starts, int64_t E, const at::Tensor& x) {
+  TORCH_CHECK(starts.dim() == 1 && starts.scalar_type() == at::kInt && starts.size(0) == E + 1,
+              "starts must be int32 [E+1] with E=", E, " experts");
+  TORCH_CHECK(starts.device() == x.device(), "all tensors must be on the same device");
+}
+void check_16bit(const at::Tensor& a, const at::Tensor& b) {
+  TORCH_CHECK(a.is_cuda() && b.device() == a.device(), "all tensors must be on the same device");
+  TORCH_CHECK(a.scalar_type() == b.scalar_type(), "operands must have one dtype, got ", a.scalar_type(), " and ", b.scalar_type());
+}
+
+// Weights stored as [E,K,N] (a view with its last two dimensions exchanged)
+// are taken as they are.
+bool stored_across(const at::Tensor& w) { return w.stride(2) != 1 && w.stride(1) == 1 && w.size(1) > 1; }
+
+// out[r] = W[e] x[r] (across false: w [E,N,K]), or W[e]^T x[r] (w [E,K,N]).
+at::Tensor grouped_rows(const at::Tensor& x, const at::Tensor& w, const at::Tensor& starts, bool across) {
+  const int64_t M = x.size(0), E = w.size(0), P = w.size(across ? 2 : 1);
+  at::Tensor a = rows16(x, 8), b = rows16(w, 8);
+  const int64_t extra = a.size(1) - b.size(across ? 1 : 2);   // x was padded along the products' index
+  if (across && extra > 0) b = at::constant_pad_nd(b, {0, 0, 0, extra});
+  const int64_t K = a.size(1), P8 = across ? b.size(2) : P;
+  at::Tensor s = contig(starts), out = at::empty({M, P8}, x.options().memory_format(at::MemoryFormat::Contiguous));
+  if (across)
+    check_status(mi_moe_grouped_matmul_dx(a.data_ptr(), row_stride(a), b.data_ptr(), expert_stride(b), row_stride(b),
+                                          s.data_ptr<int32_t>(), M, K, P8, E, act_code(x), out.data_ptr(), stream_of(x)),
+                 "moe_grouped_matmul");
+  else
+    check_status(mi_moe_grouped_matmul(a.data_ptr(), row_stride(a), b.data_ptr(), expert_stride(b), row_stride(b),
+                                       s.data_ptr<int32_t>(), M, P8, K, E, act_code(x), out.data_ptr(), stream_of(x)),
+                 "moe_grouped_matmul");
+  return P8 == P ? out : out.narrow(1, 0, P).contiguous();
+}
+
+// x [M,K], w [E,N,K] -> y [M,N].
+at::Tensor moe_grouped_matmul_hip(const at::Tensor& x, const at::Tensor& w, const at::Tensor& starts) {
+  TORCH_CHECK(x.dim() == 2 && w.dim() == 3 && w.size(2) == x.size(1) && w.size(0) > 0 && w.size(1) > 0 && w.size(2) > 0,
+              "moe_grouped_matmul: expected x [M,K], w [E,N,K]");
+  check_16bit(x, w);
+  check_starts(starts, w.size(0), x);
+  c10::hip::HIPGuard guard(x.get_device());
+  const bool across = stored_across(w);
+  return grouped_rows(x, across ? w.transpose(1, 2) : w, starts, across);
+}
+
+// dy [M,N], w [E,N,K] -> dx [M,K].
+at::Tensor moe_grouped_matmul_dx_hip(const at::Tensor& dy, const at::Tensor& w, const at::Tensor& starts) {
+  TORCH_CHECK(dy.dim() == 2 && w.dim() == 3 && w.size(1) == dy.size(1) && w.size(0) > 0 && w.size(1) > 0 && w.size(2) > 0,
+              "moe_grouped_matmul_dx: expected dy [M,N], w [E,N,K]");
+  check_16bit(dy, w);
+  check_starts(starts, w.size(0), dy);
+  c10::hip::HIPGuard guard(dy.get_device());
+  const bool across = stored_across(w);
+  return grouped_rows(dy, across ? w.transpose(1, 2) : w, starts, !across);
+}
+
+// dy [M,N], x [M,K] -> dw [E,N,K].
+at::Tensor moe_grouped_matmul_dw_hip(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& starts) {
+  TORCH_CHECK(dy.dim() == 2 && x.dim() == 2 && dy.size(0) == x.size(0) && dy.size(1) > 0 && x.size(1) > 0,
+              "moe_grouped_matmul_dw: expected dy [M,N], x [M,K]");
+  check_16bit(dy, x);
+  TORCH_CHECK(starts.dim() == 1 && starts.size(0) > 1, "starts must be int32 [E+1]");
+  const int64_t E = starts.size(0) - 1, M = x.size(0), N = dy.size(1), K = x.size(1);
+  check_starts(starts, E, x);
+  c10::hip::HIPGuard guard(x.get_device());
+  at::Tensor a = rows16(dy, 8), b = rows16(x, 8), s = contig(starts);
+  const int64_t N8 = a.size(1), K8 = b.size(1);
+  at::Tensor dw = at::empty({E, N8, K8}, x.options().memory_format(at::MemoryFormat::Contiguous));
+  check_status(mi_moe_grouped_matmul_dw(a.data_ptr(), row_stride(a), b.data_ptr(), row_stride(b), s.data_ptr<int32_t>(), M, N8,
+                                        K8, E, act_code(x), dw.data_ptr(), stream_of(x)),
+               "moe_grouped_matmul_dw");
+  return N8 == N && K8 == K ? dw : dw.narrow(1, 0, N).narrow(2, 0, K).contiguous();
+}
+
+// The differentiable form: each gradient is one of the products above.
+struct GroupedMatmul : torch::autograd::Function<GroupedMatmul> {
+  static at::Tensor call(const char* op, const at::Tensor& a, const at::Tensor& b, const at::Tensor& starts) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return c10::Dispatcher::singleton()
+        .findSchemaOrThrow(op, "")
+        .typed<at::Tensor(const at::Tensor&, const at::Tensor&, const at::Tensor&)>()
+        .call(a, b, starts);
+  }
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& starts) {
+    // what no gradient needs is not kept
+    ctx->save_for_backward({w.requires_grad() ? x : at::Tensor(), x.requires_grad() ? w : at::Tensor(), starts});
+    ctx->saved_data["across"] = w.dim() == 3 && stored_across(w);
+    return call("nanovllm::moe_grouped_matmul", x, w, starts);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "moe_grouped_matmul: no second derivatives (create_graph=True)");
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &x = saved[0], &w = saved[1], &starts = saved[2], &dy = grads[0];
+    at::Tensor dx, dw;
+    if (!dy.defined()) return {dx, dw, at::Tensor()};
+    if (ctx->needs_input_grad(0)) dx = call("nanovllm::moe_grouped_matmul_dx", dy, w, starts);
+    if (ctx->needs_input_grad(1))   // laid out as the weights are
+      dw = ctx->saved_data["across"].toBool() ? call("nanovllm::moe_grouped_matmul_dw", x, dy, starts).transpose(1, 2)
+                                              : call("nanovllm::moe_grouped_matmul_dw", dy, x, starts);
+    return {dx, dw, at::Tensor()};
+  }
+};
+at::Tensor moe_grouped_matmul_autograd(const at::Tensor& x, const at::Tensor& w, const at::Tensor& starts) {
+  return GroupedMatmul::apply(x, w, starts);
+}
+
+int out_code(at::ScalarType t) {
+  if (t == at::kFloat) return MI_MOE_F32;
+  if (t == at::kBFloat16) return MI_MOE_BF16;
+  TORCH_CHECK(t == at::kHalf, "dtype must be float32, bfloat16 or float16, got ", t);
+  return MI_MOE_F16;
+}
+void check_int8(const at::Tensor& x, const at::Tensor& xs, const at::Tensor& w, const at::Tensor& ws) {
+  TORCH_CHECK(x.scalar_type() == at::kChar && w.scalar_type() == at::kChar, "x and w must be int8");
+  TORCH_CHECK(xs.scalar_type() == at::kFloat && ws.scalar_type() == at::kFloat, "scales must be float32");
+  TORCH_CHECK(x.is_cuda() && w.device() == x.device() && xs.device() == x.device() && ws.device() == x.device(),
+              "all tensors must be on the same device");
+  TORCH_CHECK(x.dim() == 2 && w.size(-1) == x.size(1) && w.numel() > 0, "expected x [M,K] and w [...,N,K]");
+  TORCH_CHECK(xs.sizes() == x.sizes().slice(0, 1), "x_scales must be [M], a scale for each row");
+  TORCH_CHECK(ws.sizes() == w.sizes().slice(0, w.dim() - 1), "w_scales must be [...,N], a scale for each row of w");
+}
+
+// x [M,K] int8, w [N,K] int8, a scale for each row of both -> [M,N].
+at::Tensor int8_matmul_hip(const at::Tensor& x, const at::Tensor& x_scales, const at::Tensor& w, const at::Tensor& w_scales,
+                           const std::optional<at::Tensor>& bias, at::ScalarType dtype) {
+  TORCH_CHECK(w.dim() == 2, "int8_matmul: expected w [N,K]");
+  check_int8(x, x_scales, w, w_scales);
+  const int out = out_code(dtype);
+  const bool has = bias.has_value() && bias->defined();
+  if (has)
+    TORCH_CHECK(bias->scalar_type() == at::kFloat && bias->dim() == 1 && bias->size(0) == w.size(0) && bias->device() == x.device(),
+                "bias must be a float32 [N] tensor on the device of x");
+  c10::hip::HIPGuard guard(x.get_device());
+  at::Tensor a = rows16(x, 16), b = rows16(w, 16), xs = contig(x_scales), ws = contig(w_scales), bs = has ? contig(*bias) : at::Tensor();
+  const int64_t M = a.size(0), K = a.size(1), N = b.size(0);
+  at::Tensor y = at::empty({M, N}, x.options().dtype(dtype).memory_format(at::MemoryFormat::Contiguous));
+  check_status(mi_moe_int8_matmul(a.data_ptr<int8_t>(), row_stride(a), xs.data_ptr<float>(), b.data_ptr<int8_t>(), row_stride(b),
+                                  ws.data_ptr<float>(), has ? bs.data_ptr<float>() : nullptr, M, N, K, out, y.data_ptr(), stream_of(x)),
+               "int8_matmul");
+  return y;
+}
+
+// The same with a weight for each expert, w [E,N,K], and ragged rows.
+at::Tensor moe_grouped_matmul_int8_hip(const at::Tensor& x, const at::Tensor& x_scales, const at::Tensor& w,
+                                       const at::Tensor& w_scales, const at::Tensor& starts, at::ScalarType dtype) {
+  TORCH_CHECK(w.dim() == 3, "moe_grouped_matmul_int8: expected w [E,N,K]");
+  check_int8(x, x_scales, w, w_scales);
+  check_starts(starts, w.size(0), x);
+  const int out = out_code(dtype);
+  c10::hip::HIPGuard guard(x.get_device());
+  at::Tensor a = rows16(x, 16), b = rows16(w, 16), xs = contig(x_scales), ws = contig(w_scales), s = contig(starts);
+  const int64_t M = a.size(0), K = a.size(1), N = b.size(1), E = b.size(0);
+  at::Tensor y = at::empty({M, N}, x.options().dtype(dtype).memory_format(at::MemoryFormat::Contiguous));
+  check_status(mi_moe_grouped_matmul_int8(a.data_ptr<int8_t>(), row_stride(a), xs.data_ptr<float>(), b.data_ptr<int8_t>(),
+                                          expert_stride(b), row_stride(b), ws.data_ptr<float>(), s.data_ptr<int32_t>(), M, N, K, E,
+                                          out, y.data_ptr(), stream_of(x)),
+               "moe_grouped_matmul_int8");
+  return y;
+}
+
+// x [...,C] -> int8 codes [...,C] and a scale for each row [...].
+std::tuple<at::Tensor, at::Tensor> int8_quantize_hip(const at::Tensor& x) {
+  const int dt = mx_value_code(x.scalar_type());
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "int8_quantize: expected [..., C] with C > 0");
+  c10::hip::HIPGuard guard(x.get_device());
+  const int64_t C = x.size(-1), rows = x.numel() / C;
+  const bool in_place = x.is_contiguous() || (x.dim() == 2 && x.size(0) > 1 && x.stride(1) == 1 && x.stride(0) >= C);
+  at::Tensor v = in_place ? x : x.contiguous();
+  at::Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kChar).memory_format(at::MemoryFormat::Contiguous));
+  at::Tensor scales = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  check_status(mi_moe_int8_quantize(v.data_ptr(), dt, rows, C, v.is_contiguous() ? C : v.stride(0), codes.data_ptr<int8_t>(),
+                                    scales.data_ptr<float>(), stream_of(x)),
+               "int8_quantize");
+  return {codes, scales};
+}
+
+at::Tensor int8_dequantize_hip(const at::Tensor& codes, const at::Tensor& scales, at::ScalarType dtype) {
+  const int dt = mx_value_code(dtype);
+  TORCH_CHECK(codes.scalar_type() == at::kChar && scales.scalar_type() == at::kFloat, "codes must be int8, scales float32");
+  TORCH_CHECK(codes.is_cuda() && scales.device() == codes.device(), "codes and scales must be on one device");
+  TORCH_CHECK(codes.dim() >= 1 && codes.size(-1) > 0 && scales.sizes() == codes.sizes().slice(0, codes.dim() - 1),
+              "int8_dequantize: expected codes [..., C] and scales [...]");
+  c10::hip::HIPGuard guard(codes.get_device());
+  at::Tensor c = contig(codes), s = contig(scales);
+  at::Tensor out = at::empty(c.sizes(), c.options().dtype(dtype));
+  check_status(mi_moe_int8_dequantize(c.data_ptr<int8_t>(), s.data_ptr<float>(), s.numel(), c.size(-1), out.data_ptr(), dt,
+                                      stream_of(c)),
+               "int8_dequantize");
+  return out;
+}
+
 int scale_code(const at::Tensor& d) {
   if (d.scalar_type() == at::kBFloat16) return MI_MOE_BF16;
   TORCH_CHECK(d.scalar_type() == at::kHalf, "scales must be float16 or bfloat16");
@@ -683,7 +890,16 @@ TORCH_LIBRARY_FRAGMENT(nanovllm, m) {
         "__torch__.torch.classes.nanovllm.MoEInfer moe) -> Tensor");
   m.def("mx_quantize(Tensor x, str format) -> (Tensor, Tensor)");
   m.def("mx_dequantize(Tensor codes, Tensor scales, str format, ScalarType dtype) -> Tensor");
+  m.def("moe_grouped_matmul(Tensor x, Tensor w, Tensor starts) -> Tensor");
+  m.def("moe_grouped_matmul_dx(Tensor dy, Tensor w, Tensor starts) -> Tensor");
+  m.def("moe_grouped_matmul_dw(Tensor dy, Tensor x, Tensor starts) -> Tensor");
+  m.def("moe_grouped_matmul_int8(Tensor x, Tensor x_scales, Tensor w, Tensor w_scales, Tensor starts, ScalarType dtype) -> Tensor");
+  m.def("int8_matmul(Tensor x, Tensor x_scales, Tensor w, Tensor w_scales, Tensor? bias, ScalarType dtype) -> Tensor");
+  m.def("int8_quantize(Tensor x) -> (Tensor, Tensor)");
+  m.def("int8_dequantize(Tensor codes, Tensor scales, ScalarType dtype) -> Tensor");
 }
+
+TORCH_LIBRARY_IMPL(nanovllm, Autograd, m) { m.impl("moe_grouped_matmul", &moe_grouped_matmul_autograd); }
 
 TORCH_LIBRARY_IMPL(nanovllm, CUDA, m) {
   m.impl("moe_forward", &moe_forward_hip);
@@ -694,6 +910,13 @@ TORCH_LIBRARY_IMPL(nanovllm, CUDA, m) {
   m.impl("moe_forward_scores", &moe_forward_scores_hip);
   m.impl("mx_quantize", &mx_quantize_hip);
   m.impl("mx_dequantize", &mx_dequantize_hip);
+  m.impl("moe_grouped_matmul", &moe_grouped_matmul_hip);
+  m.impl("moe_grouped_matmul_dx", &moe_grouped_matmul_dx_hip);
+  m.impl("moe_grouped_matmul_dw", &moe_grouped_matmul_dw_hip);
+  m.impl("moe_grouped_matmul_int8", &moe_grouped_matmul_int8_hip);
+  m.impl("int8_matmul", &int8_matmul_hip);
+  m.impl("int8_quantize", &int8_quantize_hip);
+  m.impl("int8_dequantize", &int8_dequantize_hip);
   m.impl("moe_forward_npu_stream", &moe_forward_hip);
   m.impl("moe_forward_npu_graph_out", &moe_forward_graph_out_impl);
 }

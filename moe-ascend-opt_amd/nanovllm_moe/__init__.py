@@ -15,14 +15,23 @@ sigmoid scores, a bias for the choice alone, expert groups); ``moe_forward_logit
 and ``moe_forward_scores`` run them in front of the layer.  MX block formats:
 ``mx_quantize(x, "mxfp4" | "mxfp6")`` and ``mx_dequantize``.
 
+Products on rows sorted by expert (``starts``: int32 [E+1], rows starts[e] <=
+r < starts[e+1] are expert e's; other rows give 0):
+``moe_grouped_matmul(x, w, starts)`` for fp16 / bf16 weights [E,N,K], with
+gradients of x and w (``moe_grouped_matmul_dx`` / ``_dw`` alone), and
+``moe_grouped_matmul_int8(x, x_scales, w, w_scales, starts, dtype)``.
+``int8_matmul(x, x_scales, w, w_scales, bias, dtype)`` is the latter with one
+weight [N,K]; ``int8_quantize`` and ``int8_dequantize`` go between values and
+int8 codes with a scale for each row.
+
 The op dispatches on the tensors' device, like the reference's registration
 (Int8-gemm/nanovllm_ops.cpp:410-412).  HIP tensors run the hand-written HIP
 kernels of ``libmimoe.so`` on the current stream; a missing library raises,
 and the HIP key never falls back to the host.  CPU tensors run the reference
 CPU algorithm on host cores (the CPU key: Q8_0 / Q4_0 on the host engine,
 W4A16 on the host executor), from the host copy of the weights a handle keeps
-when no HIP device is present or MIMOE_HOST_WEIGHTS=1.  MXFP4 layers and the MX
-ops run on HIP tensors only.
+when no HIP device is present or MIMOE_HOST_WEIGHTS=1.  MXFP4 layers, the MX
+ops and these products run on HIP tensors only.
 """
 from __future__ import annotations
 
@@ -59,6 +68,8 @@ C_SYMBOLS = (
     "mi_moe_cpu_isa_name", "mi_moe_cpu_topk_softmax", "mi_moe_cpu_create_numa",
     "mi_moe_store_mxfp4", "mi_moe_topk_scores", "mi_moe_cpu_topk_scores", "mi_moe_forward_scores",
     "mi_moe_mx_quantize", "mi_moe_mx_dequantize",
+    "mi_moe_grouped_matmul", "mi_moe_grouped_matmul_dx", "mi_moe_grouped_matmul_dw",
+    "mi_moe_grouped_matmul_int8", "mi_moe_int8_matmul", "mi_moe_int8_quantize", "mi_moe_int8_dequantize",
 )
 
 
@@ -136,6 +147,13 @@ def capi():
     L.mi_moe_forward_scores.argtypes = [P, P, P, P, I, I64, I64, P, I, I64, I64, I64, I, F32c, I, P, P, P]
     L.mi_moe_mx_quantize.argtypes = [P, I, I64, I64, I64, I, P, P, P]
     L.mi_moe_mx_dequantize.argtypes = [P, P, I64, I64, I, P, I, P]
+    L.mi_moe_grouped_matmul.argtypes = [P, I64, P, I64, I64, P, I64, I64, I64, I64, I, P, P]
+    L.mi_moe_grouped_matmul_dx.argtypes = [P, I64, P, I64, I64, P, I64, I64, I64, I64, I, P, P]
+    L.mi_moe_grouped_matmul_dw.argtypes = [P, I64, P, I64, P, I64, I64, I64, I64, I, P, P]
+    L.mi_moe_grouped_matmul_int8.argtypes = [P, I64, P, P, I64, I64, P, P, I64, I64, I64, I64, I, P, P]
+    L.mi_moe_int8_matmul.argtypes = [P, I64, P, P, I64, P, P, I64, I64, I64, I, P, P]
+    L.mi_moe_int8_quantize.argtypes = [P, I, I64, I64, I64, P, P, P]
+    L.mi_moe_int8_dequantize.argtypes = [P, P, I64, I64, P, I, P]
     L.mi_moe_cpu_isa_name.restype = ctypes.c_char_p
     L.mi_moe_cpu_isa_name.argtypes = [I]
     for name in C_SYMBOLS:

@@ -15,8 +15,12 @@ namespace {
 
 constexpr int kThreads = 512, kWaves = 8;
 constexpr int kTile = 256;          // output columns of a tile, and most rows
-constexpr int kStepBytes = 128;     // of a row with the products' index along it, a step; or 64 rows across it
-constexpr int kOperand = kTile * kStepBytes;   // LDS of an operand's step: 32 KB in either form
+// A step of the products' index: a cache line of a row, or 64 rows across it.
+// (Loads of 64 bytes of a row make twice the requests to the L2, and those
+// bound the loop: bf16 8192 x 8192 x 4096 444 us, 402 with whole lines.)
+constexpr int kStepBytes = 128;
+constexpr int kStepRows = 64;
+constexpr int kLds = 163840;        // all of a compute unit's
 constexpr uint32_t kOutside = 0x80000000u;     // an offset beyond any buffer: loads give zero
 
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
@@ -52,6 +56,7 @@ template <int N>
 __device__ __forceinline__ void wait_loads_meet() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
+__device__ __forceinline__ void meet() { asm volatile("s_barrier" ::: "memory"); }
 
 // Every load and store of a tile goes through a buffer: what lies past its
 // end, or at kOutside, reads as zero and is not written.
@@ -62,108 +67,198 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, int64
 
 // One operand's share of a tile.  COLS false: DIM rows with the products'
 // index along the row ([row][128 B] in LDS, the 16-byte pieces of a row
-// permuted by the row, so that 8 rows read at one place lie in different
+// permuted by the row, so that rows read at one place lie in different
 // banks).  COLS true: the products' index across rows of 16-bit values ([64
 // rows][2 DIM B], the 32-byte chunks of a row permuted by the row, so that
-// the 8 rows of half a transposed read do).
-template <bool COLS, int DIM>
+// the 8 rows of half a transposed read do).  NSUB: subtiles of a wave.
+template <bool COLS, int DIM, int NSUB>
 struct Operand {
-  static constexpr int kIssues = (DIM + 63) / 64;
+  static constexpr int kIssues = (DIM + 63) / 64;   // loads of a wave a step
   static constexpr int kBytes = kIssues * 8192;
+  static constexpr int kReads = COLS ? NSUB : 2;    // LDS addresses of a wave
+  // loads: the next step's
   const unsigned char* base;
-  int64_t bytes;       // from base to the end of what belongs to the tile
-  uint32_t ld, off0, step;
-  int tail;            // bytes (COLS: rows) that the products' index spans
+  uint32_t size;       // bytes of it that belong to the tile
+  uint32_t off[kIssues];
+  int left;            // steps (COLS: rows) from there to the end
+  uint32_t ld;
+  int ragged;          // the last step's 16-byte pieces (0: all eight); !COLS
+  // reads
+  uint32_t at[kReads];
 
-  // base: the tile's first element; n: its rows (COLS: columns); len: length
-  // of the products' index in bytes of a row (COLS: in rows).
-  __device__ __forceinline__ void set(const unsigned char* b, int n, uint32_t ld_, int len) {
+  // b: the tile's first element; n: its rows (COLS: columns); len: length of
+  // the products' index in bytes of a row (COLS: in rows); sub: the wave's
+  // first subtile; lds: where the ring begins for this operand.
+  __device__ __forceinline__ void set(const unsigned char* b, int n, uint32_t ld_, int len, int sub, uint32_t lds) {
     base = b;
     ld = ld_;
-    tail = len;
-    const int t = threadIdx.x;
+    const int t = threadIdx.x, lane = t & 63, q = lane >> 4, r = lane & 15;
     if constexpr (COLS) {
-      const int k = t >> 5, piece = (t & 31) ^ (swizzle(k) << 1);
-      off0 = 8 * piece < n ? (uint32_t)k * ld + 16u * piece : kOutside;
-      step = 16 * ld;
-      bytes = (int64_t)len * ld;
+      static_assert(DIM == 256 || DIM == 128, "a row of 32 or 16 pieces");
+      constexpr int kPieces = DIM / 8, kRows = kThreads / kPieces;   // of a row; rows of an issue
+      const int k = t / kPieces, piece = t % kPieces;
+#pragma unroll
+      for (int i = 0; i < kIssues; ++i) {
+        const int row = k + kRows * i, c = piece ^ (swizzle(row) << 1);
+        off[i] = 8 * c < n ? (uint32_t)row * ld + 16u * c : kOutside;
+      }
+      left = len;
+      const int kr = 8 * q + (r >> 2);
+#pragma unroll
+      for (int i = 0; i < NSUB; ++i) at[i] = lds + kr * (2 * DIM) + (((sub + i) ^ swizzle(kr)) << 5) + ((r & 3) << 3);
     } else {
-      const int row = t >> 3, piece = (t & 7) ^ (row & 7);
-      off0 = (uint32_t)row * ld + 16u * piece;
-      step = 64 * ld;
-      bytes = (int64_t)(n - 1) * ld + len;
+#pragma unroll
+      for (int i = 0; i < kIssues; ++i) {
+        const int row = 64 * i + (t >> 3);
+        off[i] = row < min(n, DIM) ? (uint32_t)row * ld + 16u * piece_of(t) : kOutside;
+      }
+      left = (len + kStepBytes - 1) / kStepBytes;
+      ragged = (len % kStepBytes) >> 4;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) at[h] = lds + (16 * sub + r) * kStepBytes + (((4 * h + q) ^ (r & 7)) << 4);
     }
+    limit();
   }
   static __device__ __forceinline__ int swizzle(int k) { return (k & 3) | ((k >> 1) & 4); }
+  static __device__ __forceinline__ int piece_of(int t) { return (t & 7) ^ ((t >> 3) & 7); }
 
-  __device__ __forceinline__ void load(int s, uint32_t lds) const {
-    const uint32_t dst = lds + (threadIdx.x >> 6) * 1024;
+  // What the next step's loads may read: nothing past the last step.
+  __device__ __forceinline__ void limit() {
     if constexpr (COLS) {
-      const int64_t skip = (int64_t)s * 64 * ld;
-      const __amdgpu_buffer_rsrc_t buf = buffer_of(base + skip, bytes - skip);
-#pragma unroll
-      for (int i = 0; i < kIssues; ++i)
-        load_to_lds(buf, off0 == kOutside ? kOutside : off0 + i * step, uni(dst + i * 8192));
+      size = (uint32_t)max(0, min(left, kStepRows)) * ld;
     } else {
-      const int skip = s * kStepBytes;
-      const __amdgpu_buffer_rsrc_t buf = buffer_of(base + skip, bytes - skip);
-      const int piece = (threadIdx.x & 7) ^ ((threadIdx.x >> 3) & 7);
-      const bool in = skip + 16 * piece < tail;
+      size = left > 0 ? 0x7fffffffu : 0u;
+      if (left == 1 && ragged) {   // uniform, once
 #pragma unroll
-      for (int i = 0; i < kIssues; ++i) load_to_lds(buf, in ? off0 + i * step : kOutside, uni(dst + i * 8192));
+        for (int i = 0; i < kIssues; ++i) off[i] = piece_of(threadIdx.x) < ragged ? off[i] : kOutside;
+      }
     }
   }
-  // What the matrix instruction takes of subtile s (16 rows, or columns), half c of the step.
-  static __device__ __forceinline__ u32x4_t get(const lds_byte* lds, int s, int c) {
-    const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15;
+  __device__ __forceinline__ void advance() {
+    base += COLS ? (uint64_t)kStepRows * ld : (uint64_t)kStepBytes;
+    left -= COLS ? kStepRows : 1;
+    limit();
+  }
+  // Loads of a step to LDS at `dst`, this wave's first kilobyte of it.
+  __device__ __forceinline__ void load(uint32_t dst) const {
+    const __amdgpu_buffer_rsrc_t buf = __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, (int)size, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < kIssues; ++i) load_to_lds(buf, off[i], dst + i * 8192);
+  }
+  // What the matrix instruction takes of the wave's subtile i (16 rows, or
+  // columns), half h of the step.
+  __device__ __forceinline__ u32x4_t get(int i, int h) const {
     if constexpr (COLS) {
-      const int k = 32 * c + 8 * q + (r >> 2);
-      const lds_byte* p = lds + k * (2 * DIM) + ((s ^ swizzle(k)) << 5) + ((r & 3) << 3);
-      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)p);
-      const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(p + 4 * (2 * DIM)));
+      const uint32_t p = at[i] + h * 32 * (2 * DIM);
+      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(uintptr_t)p);
+      const s16x4_t hi =
+          __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(uintptr_t)(p + 4 * (2 * DIM)));
       const u32x2_t a = __builtin_bit_cast(u32x2_t, lo), b = __builtin_bit_cast(u32x2_t, hi);
       return u32x4_t{a.x, a.y, b.x, b.y};
     } else {
-      return *(const __attribute__((address_space(3))) u32x4_t*)(lds + (16 * s + r) * kStepBytes + (((4 * c + q) ^ (r & 7)) << 4));
+      return *(const __attribute__((address_space(3))) u32x4_t*)(uintptr_t)(at[h] + i * 16 * kStepBytes);
     }
+  }
+  __device__ __forceinline__ void move(uint32_t d) {
+#pragma unroll
+    for (int i = 0; i < kReads; ++i) at[i] += d;
   }
 };
 
-// acc[i][j] += subtile p0 + i of P times subtile q0 + j of Q, over all steps.
+// acc[i][u * NU + j] += the wave's subtile i of P times its subtile j of half
+// u of Q, over all steps.
+//
+// The steps pass through a ring of RING LDS buffers.  The two waves of a SIMD
+// take turns: while one reads its operands from LDS and starts loads, the
+// other runs its matrix instructions (`late` waves are one turn behind).
+//   turn 4 s      early: read P, Q0 of step s     late: products with Q1, step s - 1
+//   turn 4 s + 1  early: products with Q0         late: read P, Q0 of step s
+//   turn 4 s + 2  early: read Q1                  late: products with Q0
+//   turn 4 s + 3  early: products with Q1         late: read Q1
+// What has been read is in registers, so P and Q0 of step s + RING are loaded
+// into the places of step s from turn 4 s + 2 on, with the reads of Q1, and Q1
+// of step s + RING from turn 4 s + 4 on, with the next reads of P and Q0.
+// Every wave ends its reads by waiting until all but its last (RING - 1) steps'
+// worth of loads are done: what is read two turns later is then in LDS.
+// Addresses are moved on among the matrix instructions, whose issue leaves room.
+template <class OP, class OQ>
+struct Ring {
+  static constexpr int kStage = OP::kBytes + 2 * OQ::kBytes, kLoads = OP::kIssues + 2 * OQ::kIssues;
+  static constexpr int kSize = kLds / kStage;
+  static_assert(kSize >= 2, "a step ahead");
+};
 template <class T, class OP, class OQ, int NP, int NQ>
-__device__ __forceinline__ void products(unsigned char* smem, const OP& P, const OQ& Q, int steps, int p0, int q0,
-                                         typename T::acc (&acc)[NP][NQ]) {
-  lds_byte* sm = (lds_byte*)smem;
-  const uint32_t lds = (uint32_t)(uintptr_t)sm;
-  constexpr int STAGE = OP::kBytes + OQ::kBytes;
+__device__ __forceinline__ void products(OP& P, OQ& Q0, OQ& Q1, uint32_t lds, int steps, bool late, typename T::acc (&acc)[NP][NQ]) {
+  constexpr int NU = NQ / 2, STAGE = Ring<OP, OQ>::kStage, RING = Ring<OP, OQ>::kSize, AHEAD = (RING - 1) * Ring<OP, OQ>::kLoads;
+  const uint32_t mine = lds + uni(threadIdx.x >> 6) * 1024;
 #pragma unroll
   for (int i = 0; i < NP; ++i)
 #pragma unroll
     for (int j = 0; j < NQ; ++j) acc[i][j] = typename T::acc{0, 0, 0, 0};
-  if (steps > 0) {   // uniform
-    P.load(0, lds);
-    Q.load(0, lds + OP::kBytes);
-  }
-  for (int s = 0; s < steps; ++s) {
-    wait_loads_meet<0>();
-    const int cur = (s & 1) * STAGE, nxt = STAGE - cur;
-    if (s + 1 < steps) {   // uniform
-      P.load(s + 1, lds + nxt);
-      Q.load(s + 1, lds + nxt + OP::kBytes);
+#pragma unroll
+  for (int s = 0; s < RING; ++s) {
+    P.load(mine + s * STAGE);
+    Q0.load(mine + s * STAGE + OP::kBytes);
+    P.advance();
+    Q0.advance();
+    if (s < RING - 1) {
+      Q1.load(mine + s * STAGE + OP::kBytes + OQ::kBytes);
+      Q1.advance();
     }
+  }
+  wait_loads_meet<AHEAD>();
+  if (late) meet();
+  uint32_t cur = 0, prev = (RING - 1) * STAGE;
+  u32x4_t p[NP][2], q[NU][2];
+  auto turn = [&](int u) {
+    __builtin_amdgcn_sched_barrier(0);
+    wait_loads_meet<AHEAD>();
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      u32x4_t p[NP], q[NQ];
-#pragma unroll
-      for (int i = 0; i < NP; ++i) p[i] = OP::get(sm + cur, p0 + i, c);
-#pragma unroll
-      for (int j = 0; j < NQ; ++j) q[j] = OQ::get(sm + cur + OP::kBytes, q0 + j, c);
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < NP; ++i)
 #pragma unroll
-        for (int j = 0; j < NQ; ++j) mma(T{}, p[i], q[j], acc[i][j]);
+        for (int j = 0; j < NU; ++j) mma(T{}, p[i][h], q[j][h], acc[i][u * NU + j]);
+  };
+  auto over = [&] {
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
+    meet();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  for (int s = 0; s < steps; ++s) {
+    const uint32_t d = cur == (RING - 1) * STAGE ? (uint32_t)-(RING - 1) * STAGE : (uint32_t)STAGE;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) p[i][h] = P.get(i, h);
+#pragma unroll
+      for (int j = 0; j < NU; ++j) q[j][h] = Q0.get(j, h);
     }
+    Q1.load(mine + prev + OP::kBytes + OQ::kBytes);
+    turn(0);
+    Q1.advance();
+    P.move(d);
+    Q0.move(d);
+    over();
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < NU; ++j) q[j][h] = Q1.get(j, h);
+    P.load(mine + cur);
+    Q0.load(mine + cur + OP::kBytes);
+    turn(1);
+    P.advance();
+    Q0.advance();
+    Q1.move(d);
+    prev = cur;
+    cur += d;
+    over();
   }
+  if (!late) meet();
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load to LDS outlives the workgroup
 }
 
 // ------------------------------------------------------------ work items
@@ -250,15 +345,15 @@ struct Groups {
 // Items of one launch: each group adds less than one whole item.
 __host__ inline int64_t items_max(int64_t M, int64_t E, int most) { return M / most + (M < E + 2 ? M : E + 2); }
 
-// Place of workgroup b among `items` items and `blocks` blocks of columns:
-// XCD x takes the x-th eighth of the list, which goes through 8 blocks of
-// columns for every item, so that the workgroups that share an L2 share rows
-// and weights.
+// Place of workgroup b among `items` items and `blocks` blocks of columns.
+// The list goes through 8 blocks of columns for every item; the XCDs take
+// kRun places of it in turn, so that the workgroups that share an L2 at a time
+// share rows and weights, and experts of unequal sizes spread over all XCDs.
+constexpr int kRun = 8;
 __device__ __forceinline__ bool place(int b, int items, int blocks, int& item, int& block) {
-  const int total = items * blocks, per = (total + 7) >> 3, j = b >> 3;
-  if (j >= per) return false;
-  int l = (b & 7) * per + j;
-  if (l >= total) return false;
+  const int j = b >> 3;
+  int l = ((j / kRun) * 8 + (b & 7)) * kRun + j % kRun;
+  if (l >= items * blocks) return false;
   const int full = items * (blocks & ~7);
   int w = 8, b0 = 0;
   if (l < full) {
@@ -324,15 +419,18 @@ __device__ __forceinline__ void row_item(const RowProductArgs& a, unsigned char*
   constexpr int kElem = std::is_same<T, I8>::value ? 1 : 2;
   const int wave = uni(threadIdx.x >> 6), wp = wave & 3, wq = wave >> 2, lane = threadIdx.x & 63;
   const int np = min(kTile, a.P - p0);
-  Operand<WCOLS, kTile> W;
-  Operand<false, 32 * NQ> X;
-  const unsigned char* w = a.w + (int64_t)it.e * a.w_expert;
+  typedef Operand<WCOLS, kTile, 4> OpW;
+  typedef Operand<false, 16 * NQ, NQ / 2> OpX;   // half of the rows
+  OpW W;
+  OpX X0, X1;
+  const unsigned char *w = a.w + (int64_t)it.e * a.w_expert, *x = a.x + (int64_t)it.row0 * a.ldx;
   const int len = a.K * kElem;
-  if constexpr (WCOLS) W.set(w + (int64_t)p0 * kElem, np, a.ldw, a.K);
-  else W.set(w + (int64_t)p0 * a.ldw, np, a.ldw, len);
-  X.set(a.x + (int64_t)it.row0 * a.ldx, it.rows, a.ldx, len);
+  const uint32_t lds = (uint32_t)(uintptr_t)(lds_byte*)smem;
+  W.set(w + (int64_t)p0 * (WCOLS ? kElem : a.ldw), np, a.ldw, WCOLS ? a.K : len, 4 * wp, lds);
+  X0.set(x, it.rows, a.ldx, len, NQ / 2 * wq, lds + OpW::kBytes);
+  X1.set(x + (int64_t)(16 * NQ) * a.ldx, it.rows - 16 * NQ, a.ldx, len, NQ / 2 * wq, lds + OpW::kBytes + OpX::kBytes);
   typename T::acc acc[4][NQ];
-  products<T>(smem, W, X, (len + kStepBytes - 1) / kStepBytes, 4 * wp, NQ * wq, acc);
+  products<T>(W, X0, X1, lds, (len + kStepBytes - 1) / kStepBytes, wq != 0, acc);
   const __amdgpu_buffer_rsrc_t y = out_buffer<OUT>(a.y, (int64_t)it.row0 * a.ldy + p0);
   const bool vec = out_vec<OUT>(a.y, a.ldy);
   const int r = lane & 15, c0 = 64 * wp + 4 * (lane >> 4);
@@ -349,7 +447,7 @@ __device__ __forceinline__ void row_item(const RowProductArgs& a, unsigned char*
   }
 #pragma unroll
   for (int j = 0; j < NQ; ++j) {
-    const int row = 16 * (NQ * wq + j) + r;
+    const int row = 16 * (j / (NQ / 2) * NQ + NQ / 2 * wq + j % (NQ / 2)) + r;
     const bool in = row < it.rows;
     const uint32_t off = (uint32_t)row * (uint32_t)(a.ldy * kOutBytes<OUT>);
     float xs = 1.0f;
@@ -370,7 +468,7 @@ __device__ __forceinline__ void row_item(const RowProductArgs& a, unsigned char*
 
 template <class T, bool WCOLS, int OUT>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void row_product_kernel(RowProductArgs a) {
-  __shared__ __align__(16) unsigned char smem[4 * kOperand];
+  __shared__ __align__(16) unsigned char smem[kLds];
   const int blocks = (a.P + kTile - 1) / kTile;
   int item, block;
   Item it;
@@ -390,8 +488,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
                    min(kTile, a.P - p0), out_vec<OUT>(a.y, a.ldy));
     return;
   }
-  if (it.rows <= 32) row_item<T, WCOLS, OUT, 1>(a, smem, it, p0);
-  else if (it.rows <= 64) row_item<T, WCOLS, OUT, 2>(a, smem, it, p0);
+  if (it.rows <= 64) row_item<T, WCOLS, OUT, 2>(a, smem, it, p0);
   else if (it.rows <= 128) row_item<T, WCOLS, OUT, 4>(a, smem, it, p0);
   else if (it.rows <= 192) row_item<T, WCOLS, OUT, 6>(a, smem, it, p0);
   else row_item<T, WCOLS, OUT, 8>(a, smem, it, p0);
@@ -399,7 +496,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
 
 template <class T, int OUT>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void weight_grad_kernel(WeightGradArgs a) {
-  __shared__ __align__(16) unsigned char smem[4 * kOperand];
+  __shared__ __align__(16) unsigned char smem[kLds];
   const int bk = (a.K + kTile - 1) / kTile, bn = (a.N + kTile - 1) / kTile;
   int item, block;
   if (!place(blockIdx.x, a.E * bn, bk, item, block)) return;
@@ -412,17 +509,23 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   b = uni(min(b, a.M));
   const int end = uni(max(b, min(a.starts[e + 1], a.M))), rows = end - b;
   const int wave = uni(threadIdx.x >> 6), wp = wave & 3, wq = wave >> 2, lane = threadIdx.x & 63;
-  Operand<true, kTile> X, Y;
-  X.set(a.x + (int64_t)b * a.ldx + (int64_t)k0 * 2, min(kTile, a.K - k0), a.ldx, rows);
-  Y.set(a.dy + (int64_t)b * a.lddy + (int64_t)n0 * 2, min(kTile, a.N - n0), a.lddy, rows);
+  typedef Operand<true, kTile, 4> OpX;
+  typedef Operand<true, kTile / 2, 4> OpY;   // half of the columns
+  OpX X;
+  OpY Y0, Y1;
+  const uint32_t lds = (uint32_t)(uintptr_t)(lds_byte*)smem;
+  const unsigned char *x = a.x + (int64_t)b * a.ldx + (int64_t)k0 * 2, *dy = a.dy + (int64_t)b * a.lddy + (int64_t)n0 * 2;
+  X.set(x, min(kTile, a.K - k0), a.ldx, rows, 4 * wp, lds);
+  Y0.set(dy, min(kTile, a.N - n0), a.lddy, rows, 4 * wq, lds + OpX::kBytes);
+  Y1.set(dy + kTile, a.N - n0 - kTile / 2, a.lddy, rows, 4 * wq, lds + OpX::kBytes + OpY::kBytes);
   f32x4_t acc[4][8];
-  products<T>(smem, X, Y, (rows + 63) >> 6, 4 * wp, 8 * wq, acc);
+  products<T>(X, Y0, Y1, lds, (rows + kStepRows - 1) / kStepRows, wq != 0, acc);
   const __amdgpu_buffer_rsrc_t dw = out_buffer<OUT>(a.dw, ((int64_t)e * a.N + n0) * a.K + k0);
   const bool vec = out_vec<OUT>(a.dw, a.K);
   const int r = lane & 15, c0 = 64 * wp + 4 * (lane >> 4);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const int row = 16 * (8 * wq + j) + r;
+    const int row = 16 * (j / 4 * 8 + 4 * wq + j % 4) + r;
     const uint32_t off = (uint32_t)row * (uint32_t)(a.K * kOutBytes<OUT>);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -433,12 +536,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   }
 }
 
+unsigned grid_of(int64_t tiles) { return (unsigned)((tiles + 8 * kRun - 1) / (8 * kRun) * (8 * kRun)); }
+
 }  // namespace
 
 hipError_t launch_row_product(const RowProductArgs& a, int dt, int w_cols, int out, hipStream_t st) {
   const int64_t items = a.starts ? items_max(a.M, a.E, kTile) : (a.M + kTile - 1) / kTile;
   const int64_t blocks = (a.P + kTile - 1) / kTile;
-  const unsigned grid = (unsigned)((items * blocks + 7) / 8 * 8);
+  const unsigned grid = grid_of(items * blocks);
   if (dt == 2) {
     if (out == 0) row_product_kernel<I8, false, 0><<<grid, kThreads, 0, st>>>(a);
     else if (out == 1) row_product_kernel<I8, false, 1><<<grid, kThreads, 0, st>>>(a);
@@ -455,7 +560,7 @@ hipError_t launch_row_product(const RowProductArgs& a, int dt, int w_cols, int o
 
 hipError_t launch_weight_grad(const WeightGradArgs& a, int dt, hipStream_t st) {
   const int64_t tiles = (int64_t)a.E * ((a.N + kTile - 1) / kTile) * ((a.K + kTile - 1) / kTile);
-  const unsigned grid = (unsigned)((tiles + 7) / 8 * 8);
+  const unsigned grid = grid_of(tiles);
   if (dt == 1) weight_grad_kernel<BF16, 1><<<grid, kThreads, 0, st>>>(a);
   else weight_grad_kernel<F16, 0><<<grid, kThreads, 0, st>>>(a);
   return hipGetLastError();

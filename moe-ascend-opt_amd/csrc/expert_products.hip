@@ -13,15 +13,18 @@ namespace mimoe {
 
 namespace {
 
-constexpr int kThreads = 512, kWaves = 8;
+constexpr int kThreads = 512;
 constexpr int kTile = 256;          // output columns of a tile, and most rows
 // A step of the products' index: a cache line of a row, or 64 rows across it.
 // (Loads of 64 bytes of a row make twice the requests to the L2, and those
 // bound the loop: bf16 8192 x 8192 x 4096 444 us, 402 with whole lines.)
 constexpr int kStepBytes = 128;
 constexpr int kStepRows = 64;
-constexpr int kLds = 163840;        // all of a compute unit's
+constexpr int kLds = 163840 - 4096;   // of the operands; a compute unit's less the table of groups
 constexpr uint32_t kOutside = 0x80000000u;     // an offset beyond any buffer: loads give zero
+
+constexpr int kUnits = 256;            // compute units, 32 in each of 8 XCDs
+constexpr int kRun = 32;               // place()
 
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
@@ -40,6 +43,14 @@ __device__ __forceinline__ void mma(BF16, const u32x4_t& a, const u32x4_t& b, f3
 }
 __device__ __forceinline__ void mma(I8, const u32x4_t& a, const u32x4_t& b, i32x4_t& c) {
   c = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, a), __builtin_bit_cast(i32x4_t, b), c, 0, 0, 0);
+}
+
+// The lane, as a value that the compiler does not know: what follows from it
+// is computed where it is used, not kept in registers through a tile's products.
+__device__ __forceinline__ int lane_here() {
+  int l = threadIdx.x & 63;
+  asm volatile("" : "+v"(l));
+  return l;
 }
 
 __device__ __forceinline__ uint32_t uni(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -92,9 +103,8 @@ struct Operand {
   __device__ __forceinline__ void set(const unsigned char* b, int n, uint32_t ld_, int len, int sub, uint32_t lds) {
     base = b;
     ld = ld_;
-    const int t = threadIdx.x, lane = t & 63, q = lane >> 4, r = lane & 15;
+    const int lane = lane_here(), t = (threadIdx.x & ~63) | lane, q = lane >> 4, r = lane & 15;
     if constexpr (COLS) {
-      static_assert(DIM == 256 || DIM == 128, "a row of 32 or 16 pieces");
       constexpr int kPieces = DIM / 8, kRows = kThreads / kPieces;   // of a row; rows of an issue
       const int k = t / kPieces, piece = t % kPieces;
 #pragma unroll
@@ -105,12 +115,12 @@ struct Operand {
       left = len;
       const int kr = 8 * q + (r >> 2);
 #pragma unroll
-      for (int i = 0; i < NSUB; ++i) at[i] = lds + kr * (2 * DIM) + (((sub + i) ^ swizzle(kr)) << 5) + ((r & 3) << 3);
+      for (int i = 0; i < kReads; ++i) at[i] = lds + kr * (2 * DIM) + (((sub + i) ^ swizzle(kr)) << 5) + ((r & 3) << 3);
     } else {
 #pragma unroll
       for (int i = 0; i < kIssues; ++i) {
         const int row = 64 * i + (t >> 3);
-        off[i] = row < min(n, DIM) ? (uint32_t)row * ld + 16u * piece_of(t) : kOutside;
+        off[i] = row < n ? (uint32_t)row * ld + 16u * piece_of(t) : kOutside;
       }
       left = (len + kStepBytes - 1) / kStepBytes;
       ragged = (len % kStepBytes) >> 4;
@@ -119,7 +129,7 @@ struct Operand {
     }
     limit();
   }
-  static __device__ __forceinline__ int swizzle(int k) { return (k & 3) | ((k >> 1) & 4); }
+  static __device__ __forceinline__ int swizzle(int k) { return ((k & 3) | ((k >> 1) & 4)) & (DIM / 16 - 1); }
   static __device__ __forceinline__ int piece_of(int t) { return (t & 7) ^ ((t >> 3) & 7); }
 
   // What the next step's loads may read: nothing past the last step.
@@ -165,8 +175,8 @@ struct Operand {
   }
 };
 
-// acc[i][u * NU + j] += the wave's subtile i of P times its subtile j of half
-// u of Q, over all steps.
+// A tile's products: acc[i][u * NU + j] += the wave's subtile i of P times its
+// subtile j of half u of Q, over all steps.
 //
 // The steps pass through a ring of RING LDS buffers.  The two waves of a SIMD
 // take turns: while one reads its operands from LDS and starts loads, the
@@ -181,85 +191,103 @@ struct Operand {
 // Every wave ends its reads by waiting until all but its last (RING - 1) steps'
 // worth of loads are done: what is read two turns later is then in LDS.
 // Addresses are moved on among the matrix instructions, whose issue leaves room.
-template <class OP, class OQ>
+//
+// start() begins a tile's loads before the tile before it is stored.  STORES:
+// stores that each wave has then at least issued after them (`warm`); the
+// first step does not wait for these.
+template <class OP, class OQ, int STORES>
 struct Ring {
-  static constexpr int kStage = OP::kBytes + 2 * OQ::kBytes, kLoads = OP::kIssues + 2 * OQ::kIssues;
+  static constexpr int kStage = OP::kBytes + 2 * OQ::kBytes;
   static constexpr int kSize = kLds / kStage;
-  static_assert(kSize >= 2, "a step ahead");
-};
-template <class T, class OP, class OQ, int NP, int NQ>
-__device__ __forceinline__ void products(OP& P, OQ& Q0, OQ& Q1, uint32_t lds, int steps, bool late, typename T::acc (&acc)[NP][NQ]) {
-  constexpr int NU = NQ / 2, STAGE = Ring<OP, OQ>::kStage, RING = Ring<OP, OQ>::kSize, AHEAD = (RING - 1) * Ring<OP, OQ>::kLoads;
-  const uint32_t mine = lds + uni(threadIdx.x >> 6) * 1024;
+  static constexpr int kAhead = (kSize - 1) * (OP::kIssues + 2 * OQ::kIssues);
+  static_assert(kSize >= 2 && kAhead + STORES < 64, "a step ahead, within the counter");
+  OP P;
+  OQ Q0, Q1;
+  uint32_t mine;   // this wave's first kilobyte of the ring
+
+  __device__ __forceinline__ void start() {
 #pragma unroll
-  for (int i = 0; i < NP; ++i)
+    for (int s = 0; s < kSize; ++s) {
+      P.load(mine + s * kStage);
+      Q0.load(mine + s * kStage + OP::kBytes);
+      P.advance();
+      Q0.advance();
+      if (s < kSize - 1) {
+        Q1.load(mine + s * kStage + OP::kBytes + OQ::kBytes);
+        Q1.advance();
+      }
+    }
+    asm volatile("" ::: "memory");   // the stores that follow stay behind these loads
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  static __device__ __forceinline__ void wait(bool warm) {
+    __builtin_amdgcn_sched_barrier(0);
+    if (warm) wait_loads_meet<kAhead + STORES>();
+    else wait_loads_meet<kAhead>();
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  template <class T, int NP, int NQ>
+  __device__ __forceinline__ void products(int steps, bool late, bool warm, typename T::acc (&acc)[NP][NQ]) {
+    constexpr int NU = NQ / 2;
 #pragma unroll
-    for (int j = 0; j < NQ; ++j) acc[i][j] = typename T::acc{0, 0, 0, 0};
+    for (int i = 0; i < NP; ++i)
 #pragma unroll
-  for (int s = 0; s < RING; ++s) {
-    P.load(mine + s * STAGE);
-    Q0.load(mine + s * STAGE + OP::kBytes);
-    P.advance();
-    Q0.advance();
-    if (s < RING - 1) {
-      Q1.load(mine + s * STAGE + OP::kBytes + OQ::kBytes);
+      for (int j = 0; j < NQ; ++j) acc[i][j] = typename T::acc{0, 0, 0, 0};
+    wait(warm);
+    if (late) meet();
+    uint32_t cur = 0, prev = (kSize - 1) * kStage;
+    u32x4_t p[NP][2], q[NU][2];
+    auto multiply = [&](int u) {
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+          for (int j = 0; j < NU; ++j) mma(T{}, p[i][h], q[j][h], acc[i][u * NU + j]);
+    };
+    auto over = [&] {
+      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_sched_barrier(0);
+      meet();
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    for (int s = 0; s < steps; ++s) {
+      const bool first = warm && s == 0;
+      const uint32_t d = cur == (kSize - 1) * kStage ? (uint32_t)-(kSize - 1) * kStage : (uint32_t)kStage;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) p[i][h] = P.get(i, h);
+#pragma unroll
+        for (int j = 0; j < NU; ++j) q[j][h] = Q0.get(j, h);
+      }
+      Q1.load(mine + prev + OP::kBytes + OQ::kBytes);
+      wait(first);
+      multiply(0);
       Q1.advance();
+      P.move(d);
+      Q0.move(d);
+      over();
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < NU; ++j) q[j][h] = Q1.get(j, h);
+      P.load(mine + cur);
+      Q0.load(mine + cur + OP::kBytes);
+      wait(first);
+      multiply(1);
+      P.advance();
+      Q0.advance();
+      Q1.move(d);
+      prev = cur;
+      cur += d;
+      over();
     }
+    if (!late) meet();
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the ring is free, and no load to it outlives the workgroup
   }
-  wait_loads_meet<AHEAD>();
-  if (late) meet();
-  uint32_t cur = 0, prev = (RING - 1) * STAGE;
-  u32x4_t p[NP][2], q[NU][2];
-  auto turn = [&](int u) {
-    __builtin_amdgcn_sched_barrier(0);
-    wait_loads_meet<AHEAD>();
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < NP; ++i)
-#pragma unroll
-        for (int j = 0; j < NU; ++j) mma(T{}, p[i][h], q[j][h], acc[i][u * NU + j]);
-  };
-  auto over = [&] {
-    __builtin_amdgcn_s_setprio(0);
-    __builtin_amdgcn_sched_barrier(0);
-    meet();
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  for (int s = 0; s < steps; ++s) {
-    const uint32_t d = cur == (RING - 1) * STAGE ? (uint32_t)-(RING - 1) * STAGE : (uint32_t)STAGE;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int i = 0; i < NP; ++i) p[i][h] = P.get(i, h);
-#pragma unroll
-      for (int j = 0; j < NU; ++j) q[j][h] = Q0.get(j, h);
-    }
-    Q1.load(mine + prev + OP::kBytes + OQ::kBytes);
-    turn(0);
-    Q1.advance();
-    P.move(d);
-    Q0.move(d);
-    over();
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int j = 0; j < NU; ++j) q[j][h] = Q1.get(j, h);
-    P.load(mine + cur);
-    Q0.load(mine + cur + OP::kBytes);
-    turn(1);
-    P.advance();
-    Q0.advance();
-    Q1.move(d);
-    prev = cur;
-    cur += d;
-    over();
-  }
-  if (!late) meet();
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load to LDS outlives the workgroup
-}
+};
 
 // ------------------------------------------------------------ work items
 // Groups of rows: 0 the rows before the first expert's, 1 .. E the experts,
@@ -276,13 +304,15 @@ __device__ __forceinline__ int items_of(int rows, int most) { return (rows + mos
 
 struct Groups {
   static constexpr int kPer = (kGroupMaxE + 2 + kWave - 1) / kWave;
-  int begin[kPer + 1];   // first rows of this lane's groups, and of the next lane's first
-  int before;            // items of the lanes before this one
+  static constexpr int kTable = kWave * kPer + 1;
+  int* first;    // LDS: where group g begins; M from the last group's end on
+  int before;    // items of the groups of the lanes before this one
   int total;
 
-  __device__ __forceinline__ void read(const int32_t* starts, int E, int M, int most) {
+  // All waves; ends with a barrier.
+  __device__ __forceinline__ void read(int* table, const int32_t* starts, int E, int M, int most) {
     const int lane = threadIdx.x & 63;
-    int v[kPer];   // where group g ends
+    int end[kPer];   // of group g
     int m = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -291,22 +321,25 @@ struct Groups {
       s = g <= E ? s : M;
       s = s < 0 ? 0 : s > M ? M : s;
       m = m > s ? m : s;
-      v[i] = m;
+      end[i] = m;
     }
 #pragma unroll
     for (int d = 1; d < kWave; d <<= 1) {
       const int o = __shfl_up(m, d);
       if (lane >= d) m = m > o ? m : o;
     }
-    int first = __shfl_up(m, 1);
-    if (lane == 0) first = 0;
-    int n = 0;
-    begin[0] = first;
+    int at = __shfl_up(m, 1);
+    if (lane == 0) at = 0;
+    first = table;
+    int n = 0, b = at;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      begin[i + 1] = v[i] > first ? v[i] : first;
-      n += items_of(begin[i + 1] - begin[i], most);
+      const int e = end[i] > at ? end[i] : at;
+      if (threadIdx.x < kWave) table[lane * kPer + i] = b;
+      n += items_of(e - b, most);
+      b = e;
     }
+    if (threadIdx.x == kWave - 1) table[kWave * kPer] = b;
     int sum = n;
 #pragma unroll
     for (int d = 1; d < kWave; d <<= 1) {
@@ -315,45 +348,44 @@ struct Groups {
     }
     before = sum - n;
     total = __builtin_amdgcn_readlane(sum, 63);
+    __syncthreads();
   }
   __device__ __forceinline__ Item find(int index, int E, int most, int grain) const {
-    const int src = 63 - __builtin_clzll(__ballot(before <= index));   // the last lane whose items begin at or before it
-    int at = before, g = 0, k = 0, n = 1, b = 0, e = 0;
+    // the last lane whose items begin at or before index, then the group among its own
+    const int owner = 63 - __builtin_clzll(__ballot(before <= index)), g0 = owner * kPer, lane = lane_here();
+    const int i = lane < kPer ? lane : kPer - 1, b = first[g0 + i], e = first[g0 + i + 1];
+    const int n = lane < kPer ? items_of(e - b, most) : 0;
+    int end = n;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int c = items_of(begin[i + 1] - begin[i], most);
-      if (index >= at && index < at + c) {
-        g = (threadIdx.x & 63) * kPer + i;
-        k = index - at;
-        n = c;
-        b = begin[i];
-        e = begin[i + 1];
-      }
-      at += c;
+    for (int d = 1; d < 16; d <<= 1) {
+      const int o = __shfl_up(end, d);
+      if (lane >= d) end += o;
     }
-    g = __builtin_amdgcn_readlane(g, src);
-    k = __builtin_amdgcn_readlane(k, src);
-    n = __builtin_amdgcn_readlane(n, src);
-    b = __builtin_amdgcn_readlane(b, src);
-    e = __builtin_amdgcn_readlane(e, src);
-    const int size = ((e - b + n - 1) / n + grain - 1) / grain * grain;
-    const int row0 = b + k * size;
-    return Item{g == 0 || g > E ? -1 : g - 1, row0, max(0, min(size, e - row0))};
+    end += __builtin_amdgcn_readlane(before, owner);
+    const int at = __builtin_ctzll(__ballot(end > index));
+    const int k = index - (__builtin_amdgcn_readlane(end, at) - __builtin_amdgcn_readlane(n, at));
+    const int rows = __builtin_amdgcn_readlane(e, at) - __builtin_amdgcn_readlane(b, at), g = g0 + at;
+    const int size = ((rows + __builtin_amdgcn_readlane(n, at) - 1) / __builtin_amdgcn_readlane(n, at) + grain - 1) / grain * grain;
+    return Item{g == 0 || g > E ? -1 : g - 1, __builtin_amdgcn_readlane(b, at) + k * size, max(0, min(size, rows - k * size))};
   }
 };
+static_assert(Groups::kPer <= 16, "a lane's groups fit 16 lanes");
 
 // Items of one launch: each group adds less than one whole item.
 __host__ inline int64_t items_max(int64_t M, int64_t E, int most) { return M / most + (M < E + 2 ? M : E + 2); }
 
-// Place of workgroup b among `items` items and `blocks` blocks of columns.
-// The list goes through 8 blocks of columns for every item; the XCDs take
-// kRun places of it in turn, so that the workgroups that share an L2 at a time
-// share rows and weights, and experts of unequal sizes spread over all XCDs.
-constexpr int kRun = 8;
-__device__ __forceinline__ bool place(int b, int items, int blocks, int& item, int& block) {
-  const int j = b >> 3;
-  int l = ((j / kRun) * 8 + (b & 7)) * kRun + j % kRun;
-  if (l >= items * blocks) return false;
+// The n-th place in a list of `tiles` tiles that this workgroup takes: the
+// XCDs take up to kRun consecutive places in turn (XCD b % 8 runs workgroup b),
+// and an XCD's gridDim / 8 workgroups take its places in turn.  So the
+// workgroups that share an L2 at a time share rows and weights, and tiles of
+// unequal cost spread over all workgroups.
+__device__ __forceinline__ int place(int n, int tiles) {
+  const int run = min(kRun, (tiles + 7) >> 3), j = (blockIdx.x >> 3) + n * (gridDim.x >> 3);
+  return ((j / run) * 8 + (blockIdx.x & 7)) * run + j % run;
+}
+// Place l in the list of `items` items by `blocks` blocks of columns: 8 blocks
+// of columns for every item, then the next 8.
+__device__ __forceinline__ void tile_at(int l, int items, int blocks, int& item, int& block) {
   const int full = items * (blocks & ~7);
   int w = 8, b0 = 0;
   if (l < full) {
@@ -366,7 +398,6 @@ __device__ __forceinline__ bool place(int b, int items, int blocks, int& item, i
   }
   item = l / w;
   block = b0 + l - item * w;
-  return true;
 }
 
 // ------------------------------------------------------------ stores
@@ -402,7 +433,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t out_buffer(void* y, int64_t at
   return buffer_of((unsigned char*)y + at * kOutBytes<OUT>, 0x7fffffff);
 }
 template <int OUT>
-__device__ __forceinline__ bool out_vec(const void* y, int64_t ldy) { return (ldy & 3) == 0 && ((uintptr_t)y & 15) == 0; }
+__device__ __forceinline__ bool out_vec(const void* y, int64_t ldy) { return (ldy * kOutBytes<OUT> & 15) == 0 && ((uintptr_t)y & 15) == 0; }
 
 // `rows` rows of n <= 256 columns become zero.
 template <int OUT>
@@ -414,146 +445,373 @@ __device__ __forceinline__ void zero_rows(__amdgpu_buffer_rsrc_t y, uint32_t ld,
   }
 }
 
-template <class T, bool WCOLS, int OUT, int NQ>
-__device__ __forceinline__ void row_item(const RowProductArgs& a, unsigned char* smem, const Item& it, int p0) {
-  constexpr int kElem = std::is_same<T, I8>::value ? 1 : 2;
-  const int wave = uni(threadIdx.x >> 6), wp = wave & 3, wq = wave >> 2, lane = threadIdx.x & 63;
-  const int np = min(kTile, a.P - p0);
-  typedef Operand<WCOLS, kTile, 4> OpW;
-  typedef Operand<false, 16 * NQ, NQ / 2> OpX;   // half of the rows
-  OpW W;
-  OpX X0, X1;
-  const unsigned char *w = a.w + (int64_t)it.e * a.w_expert, *x = a.x + (int64_t)it.row0 * a.ldx;
-  const int len = a.K * kElem;
-  const uint32_t lds = (uint32_t)(uintptr_t)(lds_byte*)smem;
-  W.set(w + (int64_t)p0 * (WCOLS ? kElem : a.ldw), np, a.ldw, WCOLS ? a.K : len, 4 * wp, lds);
-  X0.set(x, it.rows, a.ldx, len, NQ / 2 * wq, lds + OpW::kBytes);
-  X1.set(x + (int64_t)(16 * NQ) * a.ldx, it.rows - 16 * NQ, a.ldx, len, NQ / 2 * wq, lds + OpW::kBytes + OpX::kBytes);
-  typename T::acc acc[4][NQ];
-  products<T>(W, X0, X1, lds, (len + kStepBytes - 1) / kStepBytes, wq != 0, acc);
-  const __amdgpu_buffer_rsrc_t y = out_buffer<OUT>(a.y, (int64_t)it.row0 * a.ldy + p0);
-  const bool vec = out_vec<OUT>(a.y, a.ldy);
-  const int r = lane & 15, c0 = 64 * wp + 4 * (lane >> 4);
-  float ws[4][4], bias[4][4];
-  if constexpr (kElem == 1) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int p = min(p0 + c0 + 16 * i + k, a.P - 1);
-        ws[i][k] = a.ws[(int64_t)it.e * a.P + p];
-        bias[i][k] = a.bias ? a.bias[p] : 0.0f;
-      }
-  }
+// The values of a wave's subtiles as they leave a tile's products: lane (r, q)
+// has columns 4 q .. 4 q + 3 of subtile i in row r of subtile j.  16-bit
+// values change places between lane rows 2 k and 2 k + 1, so that a lane
+// stores 16 bytes and four lanes 64 of a row.
+template <int OUT, int NP, int NQ, class Value>
+__device__ __forceinline__ void store_tile(__amdgpu_buffer_rsrc_t y, uint32_t ld, int rows, int cols, bool vec, int wp, int wq,
+                                           Value value) {
+  const int lane = lane_here(), r = lane & 15, q = lane >> 4;
 #pragma unroll
   for (int j = 0; j < NQ; ++j) {
     const int row = 16 * (j / (NQ / 2) * NQ + NQ / 2 * wq + j % (NQ / 2)) + r;
-    const bool in = row < it.rows;
-    const uint32_t off = (uint32_t)row * (uint32_t)(a.ldy * kOutBytes<OUT>);
-    float xs = 1.0f;
-    if constexpr (kElem == 1) xs = a.xs[it.row0 + (in ? row : 0)];
+    const bool in = row < rows;
+    if (OUT == 2 || NP == 1 || !vec) {   // uniform
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = c0 + 16 * i;
-      float v[4];
+      for (int i = 0; i < NP; ++i) {
+        const int c = 16 * NP * wp + 16 * i + 4 * q;
+        float v[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        v[k] = (float)acc[i][j][k];
-        if constexpr (kElem == 1) v[k] = v[k] * ws[i][k] * xs + bias[i][k];
+        for (int k = 0; k < 4; ++k) v[k] = value(i, j, k);
+        store4<OUT>(y, (uint32_t)row * ld + c * kOutBytes<OUT>, v, in ? cols - c : 0, vec);
       }
-      store4<OUT>(y, off + c * kOutBytes<OUT>, v, in ? np - c : 0, vec);
+    } else {
+#pragma unroll
+      for (int i = 0; i + 1 < NP; i += 2) {
+        uint32_t w[2][2];
+#pragma unroll
+        for (int o = 0; o < 2; ++o)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            w[o][k] = from_f32<OUT & 1>(value(i + o, j, 2 * k)) | (uint32_t)from_f32<OUT & 1>(value(i + o, j, 2 * k + 1)) << 16;
+        const auto s0 = __builtin_amdgcn_permlane16_swap(w[0][0], w[1][0], false, false);
+        const auto s1 = __builtin_amdgcn_permlane16_swap(w[0][1], w[1][1], false, false);
+        const int c = 16 * NP * wp + 16 * (i + (q & 1)) + 8 * (q >> 1);
+        const u32x4_t v = {s0[0], s1[0], s0[1], s1[1]};
+        __builtin_amdgcn_raw_buffer_store_b128(v, y, (int)(in && c < cols ? (uint32_t)row * ld + 2 * c : kOutside), 0, 0);
+      }
     }
   }
 }
 
-template <class T, bool WCOLS, int OUT>
+// ------------------------------------------------------------ rows
+// Items of up to 64 and 128 rows (SMALL) keep three steps in LDS, those of up
+// to 192 and 256 rows two.
+template <class T, bool WCOLS, int OUT, int NP>
+struct Rows {
+  static constexpr int kElem = std::is_same<T, I8>::value ? 1 : 2, kCols = 64 * NP;
+  typedef Operand<WCOLS, kCols, NP> OpW;
+  const RowProductArgs& a;
+  Groups groups;
+  uint32_t lds;
+  int wp, wq, n, blocks;
+  // the tile at hand
+  Item it;
+  int p0;
+  bool live;
+
+  __device__ __forceinline__ void next() {
+    const int items = a.starts ? groups.total : items_of(a.M, a.most), l = place(n++, items * blocks);
+    live = l < items * blocks;
+    if (!live) return;
+    int item, block;
+    tile_at(l, items, blocks, item, block);
+    it = a.starts ? groups.find(item, a.E, a.most, 32) : Item{0, item * a.most, min(a.most, a.M - item * a.most)};
+    p0 = block * kCols;
+  }
+  // rows of half an item as its products take them
+  static __device__ __forceinline__ int half(int rows) { return rows <= 64 ? 32 : rows <= 128 ? 64 : rows <= 192 ? 96 : 128; }
+
+  template <class R>
+  __device__ __forceinline__ void set(R& ring) const {
+    typedef decltype(ring.Q0) OpX;
+    const unsigned char *w = a.w + (int64_t)it.e * a.w_expert, *x = a.x + (int64_t)it.row0 * a.ldx;
+    const int len = a.K * kElem, h = half(it.rows);
+    ring.P.set(w + (int64_t)p0 * (WCOLS ? kElem : a.ldw), min(kCols, a.P - p0), a.ldw, WCOLS ? a.K : len, NP * wp, lds);
+    ring.Q0.set(x, min(it.rows, h), a.ldx, len, h / 32 * wq, lds + OpW::kBytes);
+    ring.Q1.set(x + (int64_t)h * a.ldx, it.rows - h, a.ldx, len, h / 32 * wq, lds + OpW::kBytes + OpX::kBytes);
+  }
+
+  // The tile at hand, whose loads have begun; begins those of the next one if
+  // it is of the same kind (returns whether).
+  template <bool SMALL, int NQ, class R>
+  __device__ __forceinline__ bool tile(R& ring, bool warm) {
+    typename T::acc acc[NP][NQ];
+    ring.template products<T>((a.K * kElem + kStepBytes - 1) / kStepBytes, wq != 0, warm, acc);
+    const Item done = it;
+    const int d0 = p0, cols = min(kCols, a.P - p0), lane = lane_here(), r = lane & 15, q = lane >> 4;
+    float ws[NP][4], bias[NP][4], xs[NQ];
+    if constexpr (kElem == 1) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int p = min(d0 + 16 * NP * wp + 16 * i + 4 * q + k, a.P - 1);
+          ws[i][k] = a.ws[(int64_t)done.e * a.P + p];
+          bias[i][k] = a.bias ? a.bias[p] : 0.0f;
+        }
+#pragma unroll
+      for (int j = 0; j < NQ; ++j)
+        xs[j] = a.xs[done.row0 + min(16 * (j / (NQ / 2) * NQ + NQ / 2 * wq + j % (NQ / 2)) + r, done.rows - 1)];
+    }
+    next();
+    const bool same = live && it.e >= 0 && it.rows > 0 && (it.rows <= 128) == SMALL;
+    if (same) {
+      set(ring);
+      ring.start();
+    }
+    store_tile<OUT, NP, NQ>(out_buffer<OUT>(a.y, (int64_t)done.row0 * a.ldy + d0), (uint32_t)(a.ldy * kOutBytes<OUT>), done.rows, cols,
+                        out_vec<OUT>(a.y, a.ldy), wp, wq, [&](int i, int j, int k) {
+                          const float v = (float)acc[i][j][k];
+                          if constexpr (kElem == 1) return v * ws[i][k] * xs[j] + bias[i][k];
+                          return v;
+                        });
+    return same;
+  }
+  template <bool SMALL>
+  __device__ __forceinline__ void tiles() {
+    // stores of the smaller kind of tile
+    Ring<OpW, Operand<false, SMALL ? 64 : 128, 0>, (SMALL ? 2 : 6) * (OUT == 2 || NP == 1 ? NP : NP / 2)> ring;
+    ring.mine = lds + uni(threadIdx.x >> 6) * 1024;
+    __syncthreads();   // the ring's former loads and reads are over
+    set(ring);
+    ring.start();
+    for (bool warm = false, same = true; same; warm = true) {
+      if (SMALL) same = it.rows <= 64 ? tile<SMALL, 2>(ring, warm) : tile<SMALL, 4>(ring, warm);
+      else same = it.rows <= 192 ? tile<SMALL, 6>(ring, warm) : tile<SMALL, 8>(ring, warm);
+    }
+  }
+};
+
+template <class T, bool WCOLS, int OUT, int NP>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void row_product_kernel(RowProductArgs a) {
   __shared__ __align__(16) unsigned char smem[kLds];
-  const int blocks = (a.P + kTile - 1) / kTile;
-  int item, block;
-  Item it;
-  if (a.starts) {
-    Groups g;
-    g.read(a.starts, a.E, a.M, kTile);
-    if (!place(blockIdx.x, g.total, blocks, item, block)) return;
-    it = g.find(item, a.E, kTile, 32);
-  } else {
-    if (!place(blockIdx.x, items_of(a.M, kTile), blocks, item, block)) return;
-    it = Item{0, item * kTile, min(kTile, a.M - item * kTile)};
+  __shared__ int table[Groups::kTable];
+  const int wave = uni(threadIdx.x >> 6);
+  Rows<T, WCOLS, OUT, NP> rows{a};
+  rows.lds = (uint32_t)(uintptr_t)(lds_byte*)smem;
+  rows.wp = wave & 3;
+  rows.wq = wave >> 2;
+  rows.n = 0;
+  rows.blocks = (a.P + rows.kCols - 1) / rows.kCols;
+  if (a.starts) rows.groups.read(table, a.starts, a.E, a.M, a.most);
+  rows.next();
+  while (rows.live) {
+    const Item& it = rows.it;
+    if (it.e < 0 || it.rows <= 0) {
+      zero_rows<OUT>(out_buffer<OUT>(a.y, (int64_t)it.row0 * a.ldy + rows.p0), (uint32_t)(a.ldy * kOutBytes<OUT>), it.rows,
+                     min(rows.kCols, a.P - rows.p0), out_vec<OUT>(a.y, a.ldy));
+      rows.next();
+    } else if (it.rows <= 128) {
+      rows.template tiles<true>();
+    } else {
+      rows.template tiles<false>();
+    }
   }
-  const int p0 = block * kTile;
-  if (it.rows <= 0) return;
-  if (it.e < 0) {
-    zero_rows<OUT>(out_buffer<OUT>(a.y, (int64_t)it.row0 * a.ldy + p0), (uint32_t)(a.ldy * kOutBytes<OUT>), it.rows,
-                   min(kTile, a.P - p0), out_vec<OUT>(a.y, a.ldy));
-    return;
+}
+
+// ------------------------------------------------------------ few rows
+// Products of few rows (a decode call, some rows an expert) are bound by the
+// weights' bytes, or by latency.  A workgroup takes 16 columns of an item of up
+// to 64 rows; its 4 waves split the products' index, load what the matrix
+// instruction takes straight to registers, many loads at once, and add up
+// through LDS.
+constexpr int kFewThreads = 256, kFewRows = 64, kFewCols = 16;
+
+template <class T, int OUT, int MT>
+__device__ __forceinline__ void few_item(const RowProductArgs& a, float* sums, const Item& it, int p0) {
+  constexpr int kElem = std::is_same<T, I8>::value ? 1 : 2, kBatch = MT == 1 ? 8 : 4;
+  const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
+  const int len = a.K * kElem, chunks = (len + 63) >> 6, per = (chunks + 3) >> 2, c0 = wave * per, c1 = min(chunks, c0 + per);
+  const __amdgpu_buffer_rsrc_t wb = buffer_of(a.w + (int64_t)it.e * a.w_expert + (int64_t)p0 * a.ldw, 0x7fffffff);
+  const __amdgpu_buffer_rsrc_t xb = buffer_of(a.x + (int64_t)it.row0 * a.ldx, 0x7fffffff);
+  const uint32_t wo = p0 + r < a.P ? r * a.ldw : kOutside;
+  uint32_t xo[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) xo[m] = 16 * m + r < it.rows ? (16 * m + r) * a.ldx : kOutside;
+  typename T::acc acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m] = typename T::acc{0, 0, 0, 0};
+  for (int c = c0; c < c1; c += kBatch) {
+    u32x4_t w[kBatch], x[kBatch][MT];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const uint32_t at = 64 * (c + u) + 16 * q;
+      const bool in = c + u < c1 && at < (uint32_t)len;
+      w[u] = __builtin_amdgcn_raw_buffer_load_b128(wb, (int)(in && wo != kOutside ? wo + at : kOutside), 0, 0);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        x[u][m] = __builtin_amdgcn_raw_buffer_load_b128(xb, (int)(in && xo[m] != kOutside ? xo[m] + at : kOutside), 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) mma(T{}, w[u], x[u][m], acc[m]);
   }
-  if (it.rows <= 64) row_item<T, WCOLS, OUT, 2>(a, smem, it, p0);
-  else if (it.rows <= 128) row_item<T, WCOLS, OUT, 4>(a, smem, it, p0);
-  else if (it.rows <= 192) row_item<T, WCOLS, OUT, 6>(a, smem, it, p0);
-  else row_item<T, WCOLS, OUT, 8>(a, smem, it, p0);
+  typedef typename T::acc acc_t;
+  acc_t* part = reinterpret_cast<acc_t*>(sums);
+#pragma unroll
+  for (int m = 0; m < MT; ++m) part[(wave * MT + m) * kWave + lane] = acc[m];
+  __syncthreads();
+  // a thread an output: column t % 16 of rows t / 16, + 16, ..
+  const int n = threadIdx.x & 15, row = threadIdx.x >> 4;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    auto v = part[m * kWave + (n >> 2) * 16 + row][n & 3];
+#pragma unroll
+    for (int k = 1; k < 4; ++k) v += part[(k * MT + m) * kWave + (n >> 2) * 16 + row][n & 3];
+    const int mr = 16 * m + row, p = p0 + n;
+    if (mr < it.rows && p < a.P) {
+      float f = (float)v;
+      if constexpr (kElem == 1) f = f * a.ws[(int64_t)it.e * a.P + p] * a.xs[it.row0 + mr] + (a.bias ? a.bias[p] : 0.0f);
+      const int64_t at = (int64_t)(it.row0 + mr) * a.ldy + p;
+      if constexpr (OUT == 2) reinterpret_cast<float*>(a.y)[at] = f;
+      else reinterpret_cast<uint16_t*>(a.y)[at] = from_f32<OUT>(f);
+    }
+  }
+  __syncthreads();   // the sums may be written again
 }
 
 template <class T, int OUT>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void weight_grad_kernel(WeightGradArgs a) {
-  __shared__ __align__(16) unsigned char smem[kLds];
-  const int bk = (a.K + kTile - 1) / kTile, bn = (a.N + kTile - 1) / kTile;
-  int item, block;
-  if (!place(blockIdx.x, a.E * bn, bk, item, block)) return;
-  const int e = item / bn, n0 = (item - e * bn) * kTile, k0 = block * kTile;
-  // the expert's rows: starts as its running maximum within [0, M]
-  int b = 0;
-  for (int i = threadIdx.x & 63; i <= e; i += 64) b = max(b, a.starts[i]);
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) b = max(b, __shfl_xor(b, d));
-  b = uni(min(b, a.M));
-  const int end = uni(max(b, min(a.starts[e + 1], a.M))), rows = end - b;
-  const int wave = uni(threadIdx.x >> 6), wp = wave & 3, wq = wave >> 2, lane = threadIdx.x & 63;
-  typedef Operand<true, kTile, 4> OpX;
-  typedef Operand<true, kTile / 2, 4> OpY;   // half of the columns
-  OpX X;
-  OpY Y0, Y1;
-  const uint32_t lds = (uint32_t)(uintptr_t)(lds_byte*)smem;
-  const unsigned char *x = a.x + (int64_t)b * a.ldx + (int64_t)k0 * 2, *dy = a.dy + (int64_t)b * a.lddy + (int64_t)n0 * 2;
-  X.set(x, min(kTile, a.K - k0), a.ldx, rows, 4 * wp, lds);
-  Y0.set(dy, min(kTile, a.N - n0), a.lddy, rows, 4 * wq, lds + OpX::kBytes);
-  Y1.set(dy + kTile, a.N - n0 - kTile / 2, a.lddy, rows, 4 * wq, lds + OpX::kBytes + OpY::kBytes);
-  f32x4_t acc[4][8];
-  products<T>(X, Y0, Y1, lds, (rows + kStepRows - 1) / kStepRows, wq != 0, acc);
-  const __amdgpu_buffer_rsrc_t dw = out_buffer<OUT>(a.dw, ((int64_t)e * a.N + n0) * a.K + k0);
-  const bool vec = out_vec<OUT>(a.dw, a.K);
-  const int r = lane & 15, c0 = 64 * wp + 4 * (lane >> 4);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int row = 16 * (j / 4 * 8 + 4 * wq + j % 4) + r;
-    const uint32_t off = (uint32_t)row * (uint32_t)(a.K * kOutBytes<OUT>);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = c0 + 16 * i;
-      const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-      store4<OUT>(dw, off + c * kOutBytes<OUT>, v, row < a.N - n0 ? a.K - k0 - c : 0, vec);
+__global__ __launch_bounds__(kFewThreads) __attribute__((amdgpu_waves_per_eu(4))) void few_rows_kernel(RowProductArgs a) {
+  __shared__ __align__(16) float sums[4 * 4 * kWave * 4];
+  __shared__ int table[Groups::kTable];
+  Groups groups;
+  if (a.starts) groups.read(table, a.starts, a.E, a.M, kFewRows);
+  const int items = a.starts ? groups.total : items_of(a.M, kFewRows), blocks = (a.P + kFewCols - 1) / kFewCols;
+  for (int64_t l = blockIdx.x; l < (int64_t)items * blocks; l += gridDim.x) {
+    const int item = (int)(l / blocks), p0 = (int)(l - (int64_t)item * blocks) * kFewCols;
+    const Item it = a.starts ? groups.find(item, a.E, kFewRows, 16) : Item{0, item * kFewRows, min(kFewRows, a.M - item * kFewRows)};
+    if (it.e < 0) {
+      const int n = threadIdx.x & 15, p = p0 + n;
+      for (int row = threadIdx.x >> 4; row < it.rows; row += 16) {
+        const int64_t at = (int64_t)(it.row0 + row) * a.ldy + p;
+        if (p < a.P) {
+          if constexpr (OUT == 2) reinterpret_cast<float*>(a.y)[at] = 0.0f;
+          else reinterpret_cast<uint16_t*>(a.y)[at] = 0;
+        }
+      }
+    } else if (it.rows <= 16) {
+      few_item<T, OUT, 1>(a, sums, it, p0);
+    } else if (it.rows <= 32) {
+      few_item<T, OUT, 2>(a, sums, it, p0);
+    } else {
+      few_item<T, OUT, 4>(a, sums, it, p0);
     }
   }
 }
 
-unsigned grid_of(int64_t tiles) { return (unsigned)((tiles + 8 * kRun - 1) / (8 * kRun) * (8 * kRun)); }
+// ------------------------------------------------------------ weight gradient
+template <class T, int OUT>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void weight_grad_kernel(WeightGradArgs a) {
+  __shared__ __align__(16) unsigned char smem[kLds];
+  __shared__ int table[Groups::kTable];
+  typedef Operand<true, kTile, 4> OpX;
+  typedef Operand<true, kTile / 2, 4> OpY;   // half of the columns of dy
+  const int wave = uni(threadIdx.x >> 6), wp = wave & 3, wq = wave >> 2;
+  const uint32_t lds = (uint32_t)(uintptr_t)(lds_byte*)smem;
+  const int bk = (a.K + kTile - 1) / kTile, bn = (a.N + kTile - 1) / kTile;
+  Groups groups;
+  groups.read(table, a.starts, a.E, a.M, kTile);
+  Ring<OpX, OpY, 16> ring;
+  ring.mine = lds + wave * 1024;
+  int n = 0, e, n0, k0, rows;
+  auto next = [&]() -> bool {
+    const int each = bn * bk, l = place(n++, a.E * each);
+    if (l >= a.E * each) return false;
+    e = l / each;   // one expert after the other: tiles of one cost
+    int item, block;
+    tile_at(l - e * each, bn, bk, item, block);
+    n0 = item * kTile;
+    k0 = block * kTile;
+    const int b = uni(table[e + 1]);
+    rows = uni(table[e + 2]) - b;
+    const unsigned char *x = a.x + (int64_t)b * a.ldx + (int64_t)k0 * 2, *dy = a.dy + (int64_t)b * a.lddy + (int64_t)n0 * 2;
+    ring.P.set(x, min(kTile, a.K - k0), a.ldx, rows, 4 * wp, lds);
+    ring.Q0.set(dy, min(kTile, a.N - n0), a.lddy, rows, 4 * wq, lds + OpX::kBytes);
+    ring.Q1.set(dy + kTile, a.N - n0 - kTile / 2, a.lddy, rows, 4 * wq, lds + OpX::kBytes + OpY::kBytes);
+    ring.start();
+    return true;
+  };
+  bool more = next();
+  for (bool warm = false; more; warm = true) {
+    f32x4_t acc[4][8];
+    ring.template products<T>((rows + kStepRows - 1) / kStepRows, wq != 0, warm, acc);
+    const int de = e, dn = n0, dk = k0;
+    more = next();
+    store_tile<OUT, 4, 8>(out_buffer<OUT>(a.dw, ((int64_t)de * a.N + dn) * a.K + dk), (uint32_t)(a.K * kOutBytes<OUT>), a.N - dn, a.K - dk,
+                       out_vec<OUT>(a.dw, a.K), wp, wq, [&](int i, int j, int k) { return acc[i][j][k]; });
+  }
+}
+
+// A workgroup a compute unit, or as many as there are tiles.
+unsigned grid_of(int64_t tiles) {
+  const int64_t all = (tiles + 255) / 256 * 256;   // whole runs of every XCD
+  return (unsigned)(all < kUnits ? all : kUnits);
+}
+
+// Up to this many bytes * rows (rows * columns * row length of the weights in
+// bytes) the few-rows kernel: it reads the weights at the rate of a copy, and the rows again for every 16
+// columns.  us, few / tiles: int8 one weight 4096 x 4096 16 rows 6.7 / 16, 64 rows (1.1e9) 14 / 17, 128 rows (2.1e9) 22 / 21;
+// 8192 x 8192 16 rows (1.1e9) 20 / 28, 32 rows (2.1e9) 28 / 28; bf16 128 experts 1536 x 2048, 128 rows (0.8e9) 109 / 118, 512
+// rows (3.2e9) 178 / 181, 1024 rows 203 / 184; 8 experts 4096 x 4096, 64 rows (2.1e9) 67 / 68, 256 rows 118 / 70.
+constexpr int64_t kFewWork = 3 << 29;
+
+// Rows and columns of a tile: 256 x 256 (least LDS and L2 traffic for a
+// product) unless that leaves compute units without one; then the shape with most tiles that
+// still has one for each.  Narrow and low tiles keep more steps in LDS, which
+// hides more of the memory's latency.  us, 256 x 256 / 256 x 128 / 128 x 128 / 256 x 64 / 128 x 64, int8 4096 x 4096: 256 rows 49 / 28 /
+// 22 / 25 / 21 (128 tiles), 1024 rows 51 / 31 / 25 / 29 / 41 (256 tiles at 128 x 128), 2048 rows 55 / 40 / 50 / 59 / 78.
+struct Shape {
+  int rows, np;
+};
+Shape tile_shape(const RowProductArgs& a) {
+  constexpr Shape shapes[] = {{256, 4}, {256, 2}, {128, 2}, {256, 1}, {128, 1}};
+  Shape best = shapes[0];
+  int64_t most = 0;
+  for (const Shape& s : shapes) {
+    // experts of few rows are an item each; others leave half an item over on average
+    const int64_t groups = a.M < a.E ? a.M : a.E, whole = a.M / s.rows;
+    const int64_t items = !a.starts ? (a.M + s.rows - 1) / s.rows : groups > whole + groups / 2 ? groups : whole + groups / 2;
+    const int64_t tiles = items * ((a.P + 64 * s.np - 1) / (64 * s.np));
+    if (tiles <= kUnits && tiles > most) {
+      most = tiles;
+      best = s;
+    }
+  }
+  return best;
+}
+
+template <class T, int OUT>
+void few_rows(const RowProductArgs& a, hipStream_t st) {
+  const int64_t items = a.starts ? items_max(a.M, a.E, kFewRows) : (a.M + kFewRows - 1) / kFewRows;
+  const int64_t tiles = items * ((a.P + kFewCols - 1) / kFewCols);
+  few_rows_kernel<T, OUT><<<(unsigned)(tiles < 4 * kUnits ? tiles : 4 * kUnits), kFewThreads, 0, st>>>(a);
+}
+
+template <class T, bool WCOLS, int OUT, int NP>
+void tiles(const RowProductArgs& a, hipStream_t st) {
+  const int64_t items = a.starts ? items_max(a.M, a.E, a.most) : (a.M + a.most - 1) / a.most;
+  row_product_kernel<T, WCOLS, OUT, NP><<<grid_of(items * ((a.P + 64 * NP - 1) / (64 * NP))), kThreads, 0, st>>>(a);
+}
+
+template <class T, bool WCOLS, int OUT>
+void row_product(const RowProductArgs& a, hipStream_t st) {
+  if constexpr (!WCOLS) {
+    if ((int64_t)a.M * a.P * a.K <= kFewWork / (std::is_same<T, I8>::value ? 1 : 2)) return few_rows<T, OUT>(a, st);
+  }
+  const Shape s = tile_shape(a);
+  RowProductArgs b = a;
+  b.most = s.rows;
+  if (s.np == 1) tiles<T, WCOLS, OUT, 1>(b, st);
+  else if (s.np == 2) tiles<T, WCOLS, OUT, 2>(b, st);
+  else tiles<T, WCOLS, OUT, 4>(b, st);
+}
 
 }  // namespace
 
 hipError_t launch_row_product(const RowProductArgs& a, int dt, int w_cols, int out, hipStream_t st) {
-  const int64_t items = a.starts ? items_max(a.M, a.E, kTile) : (a.M + kTile - 1) / kTile;
-  const int64_t blocks = (a.P + kTile - 1) / kTile;
-  const unsigned grid = grid_of(items * blocks);
   if (dt == 2) {
-    if (out == 0) row_product_kernel<I8, false, 0><<<grid, kThreads, 0, st>>>(a);
-    else if (out == 1) row_product_kernel<I8, false, 1><<<grid, kThreads, 0, st>>>(a);
-    else row_product_kernel<I8, false, 2><<<grid, kThreads, 0, st>>>(a);
+    if (out == 0) row_product<I8, false, 0>(a, st);
+    else if (out == 1) row_product<I8, false, 1>(a, st);
+    else row_product<I8, false, 2>(a, st);
   } else if (dt == 1) {
-    if (w_cols) row_product_kernel<BF16, true, 1><<<grid, kThreads, 0, st>>>(a);
-    else row_product_kernel<BF16, false, 1><<<grid, kThreads, 0, st>>>(a);
+    if (w_cols) row_product<BF16, true, 1>(a, st);
+    else row_product<BF16, false, 1>(a, st);
   } else {
-    if (w_cols) row_product_kernel<F16, true, 0><<<grid, kThreads, 0, st>>>(a);
-    else row_product_kernel<F16, false, 0><<<grid, kThreads, 0, st>>>(a);
+    if (w_cols) row_product<F16, true, 0>(a, st);
+    else row_product<F16, false, 0>(a, st);
   }
   return hipGetLastError();
 }

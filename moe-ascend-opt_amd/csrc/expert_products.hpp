@@ -22,6 +22,7 @@ struct RowProductArgs {
   int64_t ldy;                 // elements
   uint32_t ldx, ldw;
   int M, P, K, E;
+  int most;                    // rows of an item (set by the launcher)
 };
 
 // dw[e][n][k] = sum over rows r of e of dy[r][n] x[r][k]

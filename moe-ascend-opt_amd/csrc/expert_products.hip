@@ -97,13 +97,12 @@ struct Operand {
   // reads
   uint32_t at[kReads];
 
-  // b: the tile's first element; n: its rows (COLS: columns); len: length of
-  // the products' index in bytes of a row (COLS: in rows); sub: the wave's
-  // first subtile; lds: where the ring begins for this operand.
-  __device__ __forceinline__ void set(const unsigned char* b, int n, uint32_t ld_, int len, int sub, uint32_t lds) {
+  // What to load: b: the tile's first element; n: its rows (COLS: columns);
+  // len: length of the products' index in bytes of a row (COLS: in rows).
+  __device__ __forceinline__ void source(const unsigned char* b, int n, uint32_t ld_, int len) {
     base = b;
     ld = ld_;
-    const int lane = lane_here(), t = (threadIdx.x & ~63) | lane, q = lane >> 4, r = lane & 15;
+    const int t = (threadIdx.x & ~63) | lane_here();
     if constexpr (COLS) {
       constexpr int kPieces = DIM / 8, kRows = kThreads / kPieces;   // of a row; rows of an issue
       const int k = t / kPieces, piece = t % kPieces;
@@ -113,9 +112,6 @@ struct Operand {
         off[i] = 8 * c < n ? (uint32_t)row * ld + 16u * c : kOutside;
       }
       left = len;
-      const int kr = 8 * q + (r >> 2);
-#pragma unroll
-      for (int i = 0; i < kReads; ++i) at[i] = lds + kr * (2 * DIM) + (((sub + i) ^ swizzle(kr)) << 5) + ((r & 3) << 3);
     } else {
 #pragma unroll
       for (int i = 0; i < kIssues; ++i) {
@@ -124,10 +120,21 @@ struct Operand {
       }
       left = (len + kStepBytes - 1) / kStepBytes;
       ragged = (len % kStepBytes) >> 4;
+    }
+    limit();
+  }
+  // Where to read: sub: the wave's first subtile; lds: where the ring begins
+  // for this operand.
+  __device__ __forceinline__ void reads(int sub, uint32_t lds) {
+    const int lane = lane_here(), q = lane >> 4, r = lane & 15;
+    if constexpr (COLS) {
+      const int kr = 8 * q + (r >> 2);
+#pragma unroll
+      for (int i = 0; i < kReads; ++i) at[i] = lds + kr * (2 * DIM) + (((sub + i) ^ swizzle(kr)) << 5) + ((r & 3) << 3);
+    } else {
 #pragma unroll
       for (int h = 0; h < 2; ++h) at[h] = lds + (16 * sub + r) * kStepBytes + (((4 * h + q) ^ (r & 7)) << 4);
     }
-    limit();
   }
   static __device__ __forceinline__ int swizzle(int k) { return ((k & 3) | ((k >> 1) & 4)) & (DIM / 16 - 1); }
   static __device__ __forceinline__ int piece_of(int t) { return (t & 7) ^ ((t >> 3) & 7); }
@@ -192,9 +199,13 @@ struct Operand {
 // worth of loads are done: what is read two turns later is then in LDS.
 // Addresses are moved on among the matrix instructions, whose issue leaves room.
 //
-// start() begins a tile's loads before the tile before it is stored.  STORES:
-// stores that each wave has then at least issued after them (`warm`); the
-// first step does not wait for these.
+// start() begins a tile's loads before the tile before it is stored; with FLOW
+// the ring runs on from tile to tile, the loads of a tile's last RING steps
+// being the next tile's first.  (Short sums gain: dw of 32768 rows of 128
+// experts, 4 steps a tile, 423 us, 389 with FLOW.  Long ones lose the registers:
+// int8 8192 x 8192 x 4096 236 us, 240 with FLOW.)  Each wave issues at least
+// STORES stores between two tiles (`warm`: there was a tile before); the first
+// step does not wait for these.
 template <class OP, class OQ, int STORES>
 struct Ring {
   static constexpr int kStage = OP::kBytes + 2 * OQ::kBytes;
@@ -203,9 +214,13 @@ struct Ring {
   static_assert(kSize >= 2 && kAhead + STORES < 64, "a step ahead, within the counter");
   OP P;
   OQ Q0, Q1;
-  uint32_t mine;   // this wave's first kilobyte of the ring
+  uint32_t mine;        // this wave's first kilobyte of the ring
+  uint32_t cur, prev;   // places of the step at hand and of the one before
 
+  // The first tile's loads, from the ring's first place on.
   __device__ __forceinline__ void start() {
+    cur = 0;
+    prev = (kSize - 1) * kStage;
 #pragma unroll
     for (int s = 0; s < kSize; ++s) {
       P.load(mine + s * kStage);
@@ -217,8 +232,6 @@ struct Ring {
         Q1.advance();
       }
     }
-    asm volatile("" ::: "memory");   // the stores that follow stay behind these loads
-    __builtin_amdgcn_sched_barrier(0);
   }
   static __device__ __forceinline__ void wait(bool warm) {
     __builtin_amdgcn_sched_barrier(0);
@@ -226,8 +239,10 @@ struct Ring {
     else wait_loads_meet<kAhead>();
     __builtin_amdgcn_sched_barrier(0);
   }
-  template <class T, int NP, int NQ>
-  __device__ __forceinline__ void products(int steps, bool late, bool warm, typename T::acc (&acc)[NP][NQ]) {
+  // FLOW: steps is at least RING; next0 / next1 set the sources of P and Q0 /
+  // of Q1 to the next tile.  Else the ring is left empty.
+  template <class T, bool FLOW, int NP, int NQ, class Next0, class Next1>
+  __device__ __forceinline__ void products(int steps, bool late, bool warm, typename T::acc (&acc)[NP][NQ], Next0 next0, Next1 next1) {
     constexpr int NU = NQ / 2;
 #pragma unroll
     for (int i = 0; i < NP; ++i)
@@ -235,7 +250,6 @@ struct Ring {
       for (int j = 0; j < NQ; ++j) acc[i][j] = typename T::acc{0, 0, 0, 0};
     wait(warm);
     if (late) meet();
-    uint32_t cur = 0, prev = (kSize - 1) * kStage;
     u32x4_t p[NP][2], q[NU][2];
     auto multiply = [&](int u) {
       __builtin_amdgcn_s_setprio(1);
@@ -252,8 +266,8 @@ struct Ring {
       meet();
       __builtin_amdgcn_sched_barrier(0);
     };
-    for (int s = 0; s < steps; ++s) {
-      const bool first = warm && s == 0;
+    // change: the step whose loads are the next tile's first
+    auto step = [&](bool first, auto change) {
       const uint32_t d = cur == (kSize - 1) * kStage ? (uint32_t)-(kSize - 1) * kStage : (uint32_t)kStage;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -268,6 +282,7 @@ struct Ring {
       Q1.advance();
       P.move(d);
       Q0.move(d);
+      if constexpr (decltype(change)::value) next0();
       over();
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -280,13 +295,29 @@ struct Ring {
       P.advance();
       Q0.advance();
       Q1.move(d);
+      if constexpr (decltype(change)::value) next1();
       prev = cur;
       cur += d;
       over();
+    };
+    const int plain = FLOW ? steps - kSize : steps;
+    for (int s = 0; s < plain; ++s) step(warm && s == 0, std::false_type{});
+    if constexpr (FLOW) {
+      step(warm && plain == 0, std::true_type{});
+#pragma unroll 1
+      for (int s = 1; s < kSize; ++s) step(false, std::false_type{});
     }
     if (!late) meet();
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the ring is free, and no load to it outlives the workgroup
+    if constexpr (FLOW) fence();
+    else drain();
   }
+  // The stores that follow stay behind the loads so far.
+  static __device__ __forceinline__ void fence() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // No load to LDS is under way any more.
+  static __device__ __forceinline__ void drain() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 };
 
 // ------------------------------------------------------------ work items
@@ -374,13 +405,16 @@ static_assert(Groups::kPer <= 16, "a lane's groups fit 16 lanes");
 // Items of one launch: each group adds less than one whole item.
 __host__ inline int64_t items_max(int64_t M, int64_t E, int most) { return M / most + (M < E + 2 ? M : E + 2); }
 
-// The n-th place in a list of `tiles` tiles that this workgroup takes: the
-// XCDs take up to kRun consecutive places in turn (XCD b % 8 runs workgroup b),
-// and an XCD's gridDim / 8 workgroups take its places in turn.  So the
-// workgroups that share an L2 at a time share rows and weights, and tiles of
-// unequal cost spread over all workgroups.
-__device__ __forceinline__ int place(int n, int tiles) {
-  const int run = min(kRun, (tiles + 7) >> 3), j = (blockIdx.x >> 3) + n * (gridDim.x >> 3);
+// The n-th place in a list of `tiles` tiles that this workgroup takes.  The
+// XCDs take runs of consecutive places in turn (XCD b % 8 runs workgroup b),
+// and an XCD's gridDim / 8 workgroups take its places in turn: those that share
+// an L2 at a time share rows and weights, and tiles of unequal cost spread over
+// all workgroups.  Runs are of equal numbers, about kRun places long, and whole
+// groups of `unit` places (those that share rows); fewer cuts between runs read
+// less twice.
+__device__ __forceinline__ int place(int n, int tiles, int unit) {
+  const int each = (tiles + 7) >> 3, rounds = (each + kRun - 1) / kRun, run = ((each + rounds - 1) / rounds + unit - 1) / unit * unit;
+  const int j = (blockIdx.x >> 3) + n * (gridDim.x >> 3);
   return ((j / run) * 8 + (blockIdx.x & 7)) * run + j % run;
 }
 // Place l in the list of `items` items by `blocks` blocks of columns: 8 blocks
@@ -401,6 +435,16 @@ __device__ __forceinline__ void tile_at(int l, int items, int blocks, int& item,
 }
 
 // ------------------------------------------------------------ stores
+// Two values rounded to 16 bits, to nearest even: one instruction for bf16 (in
+// integer operations a 256 x 256 tile's stores take 8000 cycles of its SIMDs).
+template <int OUT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (OUT == 1) return __builtin_bit_cast(uint32_t, bf16x2_t{(__bf16)a, (__bf16)b});
+  return __builtin_bit_cast(uint32_t, f16x2_t{(_Float16)a, (_Float16)b});
+}
+template <int OUT>
+__device__ __forceinline__ uint16_t pack1(float a) { return (uint16_t)pack2<OUT>(a, 0.0f); }
+
 template <int OUT>
 constexpr int kOutBytes = OUT == 2 ? 4 : 2;
 
@@ -418,13 +462,13 @@ __device__ __forceinline__ void store4(__amdgpu_buffer_rsrc_t y, uint32_t off, c
         __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[i]), y, (int)(i < n ? off + 4 * i : kOutside), 0, 0);
     }
   } else {
-    const uint16_t h[4] = {from_f32<OUT>(v[0]), from_f32<OUT>(v[1]), from_f32<OUT>(v[2]), from_f32<OUT>(v[3])};
+    const u32x2_t w = {pack2<OUT>(v[0], v[1]), pack2<OUT>(v[2], v[3])};
     if (vec) {
-      const u32x2_t w = {h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16};
       __builtin_amdgcn_raw_buffer_store_b64(w, y, (int)(n > 0 ? off : kOutside), 0, 0);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) __builtin_amdgcn_raw_buffer_store_b16(h[i], y, (int)(i < n ? off + 2 * i : kOutside), 0, 0);
+      for (int i = 0; i < 4; ++i)
+        __builtin_amdgcn_raw_buffer_store_b16((uint16_t)(w[i >> 1] >> (16 * (i & 1))), y, (int)(i < n ? off + 2 * i : kOutside), 0, 0);
     }
   }
 }
@@ -474,7 +518,7 @@ __device__ __forceinline__ void store_tile(__amdgpu_buffer_rsrc_t y, uint32_t ld
         for (int o = 0; o < 2; ++o)
 #pragma unroll
           for (int k = 0; k < 2; ++k)
-            w[o][k] = from_f32<OUT & 1>(value(i + o, j, 2 * k)) | (uint32_t)from_f32<OUT & 1>(value(i + o, j, 2 * k + 1)) << 16;
+            w[o][k] = pack2<OUT & 1>(value(i + o, j, 2 * k), value(i + o, j, 2 * k + 1));
         const auto s0 = __builtin_amdgcn_permlane16_swap(w[0][0], w[1][0], false, false);
         const auto s1 = __builtin_amdgcn_permlane16_swap(w[0][1], w[1][1], false, false);
         const int c = 16 * NP * wp + 16 * (i + (q & 1)) + 8 * (q >> 1);
@@ -502,7 +546,7 @@ struct Rows {
   bool live;
 
   __device__ __forceinline__ void next() {
-    const int items = a.starts ? groups.total : items_of(a.M, a.most), l = place(n++, items * blocks);
+    const int items = a.starts ? groups.total : items_of(a.M, a.most), l = place(n++, items * blocks, items * blocks < kUnits ? 1 : min(blocks, 8));
     live = l < items * blocks;
     if (!live) return;
     int item, block;
@@ -514,23 +558,28 @@ struct Rows {
   static __device__ __forceinline__ int half(int rows) { return rows <= 64 ? 32 : rows <= 128 ? 64 : rows <= 192 ? 96 : 128; }
 
   template <class R>
-  __device__ __forceinline__ void set(R& ring) const {
+  __device__ __forceinline__ void start(R& ring) const {
     typedef decltype(ring.Q0) OpX;
     const unsigned char *w = a.w + (int64_t)it.e * a.w_expert, *x = a.x + (int64_t)it.row0 * a.ldx;
     const int len = a.K * kElem, h = half(it.rows);
-    ring.P.set(w + (int64_t)p0 * (WCOLS ? kElem : a.ldw), min(kCols, a.P - p0), a.ldw, WCOLS ? a.K : len, NP * wp, lds);
-    ring.Q0.set(x, min(it.rows, h), a.ldx, len, h / 32 * wq, lds + OpW::kBytes);
-    ring.Q1.set(x + (int64_t)h * a.ldx, it.rows - h, a.ldx, len, h / 32 * wq, lds + OpW::kBytes + OpX::kBytes);
+    ring.P.source(w + (int64_t)p0 * (WCOLS ? kElem : a.ldw), min(kCols, a.P - p0), a.ldw, WCOLS ? a.K : len);
+    ring.Q0.source(x, min(it.rows, h), a.ldx, len);
+    ring.Q1.source(x + (int64_t)h * a.ldx, it.rows - h, a.ldx, len);
+    ring.P.reads(NP * wp, lds);
+    ring.Q0.reads(h / 32 * wq, lds + OpW::kBytes);
+    ring.Q1.reads(h / 32 * wq, lds + OpW::kBytes + OpX::kBytes);
+    ring.start();
   }
 
   // The tile at hand, whose loads have begun; begins those of the next one if
   // it is of the same kind (returns whether).
   template <bool SMALL, int NQ, class R>
   __device__ __forceinline__ bool tile(R& ring, bool warm) {
-    typename T::acc acc[NP][NQ];
-    ring.template products<T>((a.K * kElem + kStepBytes - 1) / kStepBytes, wq != 0, warm, acc);
     const Item done = it;
-    const int d0 = p0, cols = min(kCols, a.P - p0), lane = lane_here(), r = lane & 15, q = lane >> 4;
+    const int d0 = p0, cols = min(kCols, a.P - p0);
+    typename T::acc acc[NP][NQ];
+    ring.template products<T, false>((a.K * kElem + kStepBytes - 1) / kStepBytes, wq != 0, warm, acc, [] {}, [] {});
+    const int lane = lane_here(), r = lane & 15, q = lane >> 4;
     float ws[NP][4], bias[NP][4], xs[NQ];
     if constexpr (kElem == 1) {
 #pragma unroll
@@ -548,15 +597,15 @@ struct Rows {
     next();
     const bool same = live && it.e >= 0 && it.rows > 0 && (it.rows <= 128) == SMALL;
     if (same) {
-      set(ring);
-      ring.start();
+      start(ring);
+      ring.fence();
     }
     store_tile<OUT, NP, NQ>(out_buffer<OUT>(a.y, (int64_t)done.row0 * a.ldy + d0), (uint32_t)(a.ldy * kOutBytes<OUT>), done.rows, cols,
-                        out_vec<OUT>(a.y, a.ldy), wp, wq, [&](int i, int j, int k) {
-                          const float v = (float)acc[i][j][k];
-                          if constexpr (kElem == 1) return v * ws[i][k] * xs[j] + bias[i][k];
-                          return v;
-                        });
+                            out_vec<OUT>(a.y, a.ldy), wp, wq, [&](int i, int j, int k) {
+                              const float v = (float)acc[i][j][k];
+                              if constexpr (kElem == 1) return v * ws[i][k] * xs[j] + bias[i][k];
+                              return v;
+                            });
     return same;
   }
   template <bool SMALL>
@@ -564,13 +613,12 @@ struct Rows {
     // stores of the smaller kind of tile
     Ring<OpW, Operand<false, SMALL ? 64 : 128, 0>, (SMALL ? 2 : 6) * (OUT == 2 || NP == 1 ? NP : NP / 2)> ring;
     ring.mine = lds + uni(threadIdx.x >> 6) * 1024;
-    __syncthreads();   // the ring's former loads and reads are over
-    set(ring);
-    ring.start();
+    start(ring);
     for (bool warm = false, same = true; same; warm = true) {
       if (SMALL) same = it.rows <= 64 ? tile<SMALL, 2>(ring, warm) : tile<SMALL, 4>(ring, warm);
       else same = it.rows <= 192 ? tile<SMALL, 6>(ring, warm) : tile<SMALL, 8>(ring, warm);
     }
+    __syncthreads();   // the ring may be another's
   }
 };
 
@@ -657,7 +705,7 @@ __device__ __forceinline__ void few_item(const RowProductArgs& a, float* sums, c
       if constexpr (kElem == 1) f = f * a.ws[(int64_t)it.e * a.P + p] * a.xs[it.row0 + mr] + (a.bias ? a.bias[p] : 0.0f);
       const int64_t at = (int64_t)(it.row0 + mr) * a.ldy + p;
       if constexpr (OUT == 2) reinterpret_cast<float*>(a.y)[at] = f;
-      else reinterpret_cast<uint16_t*>(a.y)[at] = from_f32<OUT>(f);
+      else reinterpret_cast<uint16_t*>(a.y)[at] = pack1<OUT>(f);
     }
   }
   __syncthreads();   // the sums may be written again
@@ -707,32 +755,50 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   Ring<OpX, OpY, 16> ring;
   ring.mine = lds + wave * 1024;
   int n = 0, e, n0, k0, rows;
+  const unsigned char* dy;
   auto next = [&]() -> bool {
-    const int each = bn * bk, l = place(n++, a.E * each);
+    const int each = bn * bk, l = place(n++, a.E * each, 1);
     if (l >= a.E * each) return false;
     e = l / each;   // one expert after the other: tiles of one cost
     int item, block;
     tile_at(l - e * each, bn, bk, item, block);
     n0 = item * kTile;
     k0 = block * kTile;
-    const int b = uni(table[e + 1]);
-    rows = uni(table[e + 2]) - b;
-    const unsigned char *x = a.x + (int64_t)b * a.ldx + (int64_t)k0 * 2, *dy = a.dy + (int64_t)b * a.lddy + (int64_t)n0 * 2;
-    ring.P.set(x, min(kTile, a.K - k0), a.ldx, rows, 4 * wp, lds);
-    ring.Q0.set(dy, min(kTile, a.N - n0), a.lddy, rows, 4 * wq, lds + OpX::kBytes);
-    ring.Q1.set(dy + kTile, a.N - n0 - kTile / 2, a.lddy, rows, 4 * wq, lds + OpX::kBytes + OpY::kBytes);
-    ring.start();
+    rows = uni(table[e + 2]) - uni(table[e + 1]);
     return true;
   };
+  auto source0 = [&] {
+    const int64_t b = uni(table[e + 1]);
+    dy = a.dy + b * a.lddy + (int64_t)n0 * 2;
+    ring.P.source(a.x + b * a.ldx + (int64_t)k0 * 2, min(kTile, a.K - k0), a.ldx, rows);
+    ring.Q0.source(dy, min(kTile / 2, a.N - n0), a.lddy, rows);
+  };
+  auto source1 = [&] { ring.Q1.source(dy + kTile, a.N - n0 - kTile / 2, a.lddy, rows); };
   bool more = next();
+  if (!more) return;
+  ring.P.reads(4 * wp, lds);
+  ring.Q0.reads(4 * wq, lds + OpX::kBytes);
+  ring.Q1.reads(4 * wq, lds + OpX::kBytes + OpY::kBytes);
+  source0();
+  source1();
+  ring.start();
   for (bool warm = false; more; warm = true) {
     f32x4_t acc[4][8];
-    ring.template products<T>((rows + kStepRows - 1) / kStepRows, wq != 0, warm, acc);
     const int de = e, dn = n0, dk = k0;
-    more = next();
+    // at least as many steps as the ring has places: sums of no or few rows go on with zeros
+    ring.template products<T, true>(
+        max((rows + kStepRows - 1) / kStepRows, ring.kSize), wq != 0, warm, acc,
+        [&] {
+          more = next();
+          if (more) source0();
+        },
+        [&] {
+          if (more) source1();
+        });
     store_tile<OUT, 4, 8>(out_buffer<OUT>(a.dw, ((int64_t)de * a.N + dn) * a.K + dk), (uint32_t)(a.K * kOutBytes<OUT>), a.N - dn, a.K - dk,
-                       out_vec<OUT>(a.dw, a.K), wp, wq, [&](int i, int j, int k) { return acc[i][j][k]; });
+                          out_vec<OUT>(a.dw, a.K), wp, wq, [&](int i, int j, int k) { return acc[i][j][k]; });
   }
+  ring.drain();   // no load to LDS outlives the workgroup
 }
 
 // A workgroup a compute unit, or as many as there are tiles.

@@ -538,18 +538,12 @@ at::Tensor moe_grouped_matmul_dw_hip(const at::Tensor& dy, const at::Tensor& x, 
 
 // The differentiable form: each gradient is one of the products above.
 struct GroupedMatmul : torch::autograd::Function<GroupedMatmul> {
-  static at::Tensor call(const char* op, const at::Tensor& a, const at::Tensor& b, const at::Tensor& starts) {
-    at::AutoDispatchBelowADInplaceOrView guard;
-    return c10::Dispatcher::singleton()
-        .findSchemaOrThrow(op, "")
-        .typed<at::Tensor(const at::Tensor&, const at::Tensor&, const at::Tensor&)>()
-        .call(a, b, starts);
-  }
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& starts) {
     // what no gradient needs is not kept
     ctx->save_for_backward({w.requires_grad() ? x : at::Tensor(), x.requires_grad() ? w : at::Tensor(), starts});
     ctx->saved_data["across"] = w.dim() == 3 && stored_across(w);
-    return call("nanovllm::moe_grouped_matmul", x, w, starts);
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return moe_grouped_matmul_hip(x, w, starts);
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "moe_grouped_matmul: no second derivatives (create_graph=True)");
@@ -557,10 +551,10 @@ struct GroupedMatmul : torch::autograd::Function<GroupedMatmul> {
     const at::Tensor &x = saved[0], &w = saved[1], &starts = saved[2], &dy = grads[0];
     at::Tensor dx, dw;
     if (!dy.defined()) return {dx, dw, at::Tensor()};
-    if (ctx->needs_input_grad(0)) dx = call("nanovllm::moe_grouped_matmul_dx", dy, w, starts);
+    if (ctx->needs_input_grad(0)) dx = moe_grouped_matmul_dx_hip(dy, w, starts);
     if (ctx->needs_input_grad(1))   // laid out as the weights are
-      dw = ctx->saved_data["across"].toBool() ? call("nanovllm::moe_grouped_matmul_dw", x, dy, starts).transpose(1, 2)
-                                              : call("nanovllm::moe_grouped_matmul_dw", dy, x, starts);
+      dw = ctx->saved_data["across"].toBool() ? moe_grouped_matmul_dw_hip(x, dy, starts).transpose(1, 2)
+                                              : moe_grouped_matmul_dw_hip(dy, x, starts);
     return {dx, dw, at::Tensor()};
   }
 };
@@ -899,7 +893,7 @@ TORCH_LIBRARY_FRAGMENT(nanovllm, m) {
   m.def("int8_dequantize(Tensor codes, Tensor scales, ScalarType dtype) -> Tensor");
 }
 
-TORCH_LIBRARY_IMPL(nanovllm, Autograd, m) { m.impl("moe_grouped_matmul", &moe_grouped_matmul_autograd); }
+TORCH_LIBRARY_IMPL(nanovllm, AutogradCUDA, m) { m.impl("moe_grouped_matmul", &moe_grouped_matmul_autograd); }
 
 TORCH_LIBRARY_IMPL(nanovllm, CUDA, m) {
   m.impl("moe_forward", &moe_forward_hip);

@@ -30,7 +30,7 @@ def sum_slack(mag, n):
 def grouped(x, w, starts, dtype):
     """y[r] = W[e] x[r] -> (exact, bound)."""
     M, N = x.shape[0], w.shape[1]
-    y = torch.zeros(M, N, dtype=torch.float64)
+    y = torch.zeros(M, N, dtype=torch.float64, device=x.device)
     slack = torch.zeros_like(y)
     for e, a, b in spans(starts, M):
         y[a:b] = x[a:b].double() @ w[e].double().t()
@@ -43,7 +43,7 @@ def grouped_dx(dy, w, starts, dtype):
 
 
 def grouped_dw(dy, x, starts, E, dtype):
-    dw = torch.zeros(E, dy.shape[1], x.shape[1], dtype=torch.float64)
+    dw = torch.zeros(E, dy.shape[1], x.shape[1], dtype=torch.float64, device=x.device)
     slack = torch.zeros_like(dw)
     for e, a, b in spans(starts, x.shape[0]):
         g, v = dy[a:b].double(), x[a:b].double()
@@ -55,13 +55,13 @@ def grouped_dw(dy, x, starts, E, dtype):
 def int8_rows(x, xs, w, ws, bias, dtype):
     """Exact integer sum, then four fp32 roundings (the sum, times ws, times xs, plus bias) of 2^-24 each, then dtype's."""
     p = (x.double() @ w.double().t()) * ws.double() * xs.double().unsqueeze(1)
-    b = torch.zeros(w.shape[0], dtype=torch.float64) if bias is None else bias.double()
+    b = torch.zeros(w.shape[0], dtype=torch.float64, device=x.device) if bias is None else bias.double()
     slack = (p.abs() + b.abs()) * (4 * 2.0 ** -24 * (1 + 2.0 ** -20))
     return p + b, round_bound(p + b, slack, dtype)
 
 
 def int8_grouped(x, xs, w, ws, starts, dtype):
-    y = torch.zeros(x.shape[0], w.shape[1], dtype=torch.float64)
+    y = torch.zeros(x.shape[0], w.shape[1], dtype=torch.float64, device=x.device)
     bound = torch.zeros_like(y)
     for e, a, b in spans(starts, x.shape[0]):
         y[a:b], bound[a:b] = int8_rows(x[a:b], xs[a:b], w[e], ws[e], None, dtype)
@@ -83,6 +83,6 @@ def within(got, exact, bound):
     assert got.shape == exact.shape
     if got.numel() == 0:
         return 0.0
-    d = (got.cpu().double() - exact).abs()
+    d = (got.to(exact.device).double() - exact).abs()
     assert bool(torch.isfinite(d).all())
     return float(torch.where(d == 0, d, d / bound).max())   # a bound of 0: exactly zero

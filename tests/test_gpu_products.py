@@ -36,7 +36,8 @@ def _data(E, N, K, M, dt, seed):
 def _check_all(cuda, x, w, dy, starts, what=""):
     """Forward and both gradients, through autograd and through the ops."""
     ops, E, dt = torch.ops.nanovllm, w.shape[0], x.dtype
-    xc, wc, gc, sc = x.to(cuda).requires_grad_(), w.to(cuda).requires_grad_(), dy.to(cuda), starts.to(cuda)
+    xc, wc = (t.to(cuda).detach().requires_grad_() for t in (x, w))
+    gc, sc = dy.to(cuda), starts.to(cuda)
     _say("[products]", what, tuple(x.shape), tuple(w.shape), dt)
     y = ops.moe_grouped_matmul(xc, wc, sc)
     dx, dw = torch.autograd.grad(y, (xc, wc), gc)
@@ -74,6 +75,24 @@ def test_grouped_odd_sizes(cuda, N, K):
 def test_grouped_long(cuda, N, K, counts):
     x, w, dy = _data(len(counts), N, K, sum(counts), torch.bfloat16, seed=N)
     _check_all(cuda, x, w, dy, _starts(counts))
+
+
+# Calls of more work than the few-rows kernel takes, one for each tile shape, and with several tiles a workgroup.
+# rows of each expert, head, tail, N, K
+TILES = {"256x256": ([300] * 8, 0, 7, 4104, 256), "256x128": ([250, 250, 3, 250], 2, 0, 2056, 1032),
+         "128x128": ([513], 0, 0, 2048, 1600), "256x64": ([33] * 12, 0, 0, 1280, 2048), "128x64": ([400], 0, 3, 1000, 2056),
+         "rounds": ([1000, 3, 900, 1200], 0, 300, 8200, 136), "mixed": ([10, 200, 300, 0, 70, 129, 512, 1] * 5, 5, 270, 4104, 96),
+         "one step": ([700, 0, 900], 0, 0, 9000, 64), "long": ([130, 257], 0, 0, 1032, 4104)}
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("name", TILES)
+def test_grouped_tiles(cuda, dt, name):
+    counts, head, tail, N, K = TILES[name]
+    g = torch.Generator(device="cuda").manual_seed(N + K)
+    M, E = head + sum(counts) + tail, len(counts)
+    x, w, dy = (torch.randn(*s, generator=g, device=cuda).to(DT[dt]) for s in ((M, K), (E, N, K), (M, N)))
+    _check_all(cuda, x, w, dy, _starts(counts, head), name)
 
 
 def test_grouped_many_experts(cuda):
@@ -303,6 +322,25 @@ def test_int8_grouped(cuda, out, counts, head, tail, N, K):
     _say("[int8 grouped]", counts[:8], N, K, out)
     y = torch.ops.nanovllm.moe_grouped_matmul_int8(x.to(cuda), xs.to(cuda), w.to(cuda), ws.to(cuda), s.to(cuda), out)
     assert ref.within(y, *ref.int8_grouped(x, xs, w, ws, s.tolist(), out)) <= 1.0
+
+
+@pytest.mark.parametrize("out", OUT)
+@pytest.mark.parametrize("name", TILES)
+def test_int8_tiles(cuda, out, name):
+    counts, head, tail, N, K = TILES[name]
+    K = 2 * K // 16 * 16
+    M, E = head + sum(counts) + tail, len(counts)
+    g = torch.Generator(device="cuda").manual_seed(N + K)
+    x, w = (torch.randint(-128, 128, s, generator=g, device=cuda, dtype=torch.int32).to(torch.int8) for s in ((M, K), (E, N, K)))
+    xs, ws = (torch.rand(s, generator=g, device=cuda) * 0.001 + 1e-5 for s in ((M,), (E, N)))
+    s = _starts(counts, head)
+    _say("[int8 tiles]", name, M, N, K, E, out)
+    ops = torch.ops.nanovllm
+    y = ops.moe_grouped_matmul_int8(x, xs, w, ws, s.to(cuda), out)
+    assert ref.within(y, *ref.int8_grouped(x, xs, w, ws, s.tolist(), out)) <= 1.0
+    bias = torch.randn(N, generator=g, device=cuda)
+    y = ops.int8_matmul(x, xs, w[0], ws[0], bias, out)
+    assert ref.within(y, *ref.int8_rows(x, xs, w[0], ws[0], bias, out)) <= 1.0
 
 
 def _same_codes(cuda, x):

@@ -3,6 +3,17 @@
 // for each row and output channel, on the matrix cores of gfx950.
 //
 //   y[r] = W[e] x[r]      dx[r] = W[e]^T dy[r]      dW[e] = sum_r dy[r] x[r]^T
+//
+// Sums run in fp32 (int32 for int8, exact) in an order that the sizes alone
+// decide, and each output is rounded once.  Operands are read as they lie in
+// memory: rows along the sum as the matrix instruction takes them, rows across
+// it through transposed LDS reads, so no product needs a transposed copy.
+//
+// Which kernel: few_rows_kernel for calls of little work, else tiles of 256 x
+// 256 outputs down to 128 x 64 (kFewWork, tile_shape).  Measured: bf16 8192 x
+// 8192 x 4096 404 us, 1.36 PFLOP/s (the library's 1.49); int8 the same size 232 us,
+// 2.37 POP/s (2.2).  The loop alone, its steps in the L2, would take 364 us at
+// bf16: the card's power holds its clock at 1.9 to 2.1 GHz by then.
 #pragma clang fp contract(off)
 #include <type_traits>
 
@@ -182,8 +193,8 @@ struct Operand {
   }
 };
 
-// A tile's products: acc[i][u * NU + j] += the wave's subtile i of P times its
-// subtile j of half u of Q, over all steps.
+// A tile's products: acc[i][u * NQ / 2 + j] += the wave's subtile i of P times
+// its subtile j of half u of Q, over all steps.
 //
 // The steps pass through a ring of RING LDS buffers.  The two waves of a SIMD
 // take turns: while one reads its operands from LDS and starts loads, the
@@ -328,11 +339,10 @@ struct Item {
   int e, row0, rows;   // e < 0: rows of no expert
 };
 
-// Item `index` of all groups' items of at most `most` rows; a group's rows
-// are split evenly, in multiples of `grain`.  False: past the last item;
-// `total` is their number.
 __device__ __forceinline__ int items_of(int rows, int most) { return (rows + most - 1) / most; }
 
+// The groups' items of at most `most` rows, found by every workgroup for
+// itself: no launch before, no list in memory.
 struct Groups {
   static constexpr int kPer = (kGroupMaxE + 2 + kWave - 1) / kWave;
   static constexpr int kTable = kWave * kPer + 1;
@@ -381,6 +391,7 @@ struct Groups {
     total = __builtin_amdgcn_readlane(sum, 63);
     __syncthreads();
   }
+  // Item `index`: a group's rows are split evenly, in multiples of `grain`.
   __device__ __forceinline__ Item find(int index, int E, int most, int grain) const {
     // the last lane whose items begin at or before index, then the group among its own
     const int owner = 63 - __builtin_clzll(__ballot(before <= index)), g0 = owner * kPer, lane = lane_here();
@@ -410,8 +421,8 @@ __host__ inline int64_t items_max(int64_t M, int64_t E, int most) { return M / m
 // and an XCD's gridDim / 8 workgroups take its places in turn: those that share
 // an L2 at a time share rows and weights, and tiles of unequal cost spread over
 // all workgroups.  Runs are of equal numbers, about kRun places long, and whole
-// groups of `unit` places (those that share rows); fewer cuts between runs read
-// less twice.
+// groups of `unit` places (those that share rows).  us, runs of 32 / 200: dw of 16384
+// rows of 8 skewed experts 512 / 892, bf16 32768 rows of 128 experts 270 / 275.
 __device__ __forceinline__ int place(int n, int tiles, int unit) {
   const int each = (tiles + 7) >> 3, rounds = (each + kRun - 1) / kRun, run = ((each + rounds - 1) / rounds + unit - 1) / unit * unit;
   const int j = (blockIdx.x >> 3) + n * (gridDim.x >> 3);
@@ -546,8 +557,9 @@ struct Rows {
   bool live;
 
   __device__ __forceinline__ void next() {
-    const int items = a.starts ? groups.total : items_of(a.M, a.most), l = place(n++, items * blocks, items * blocks < kUnits ? 1 : min(blocks, 8));
-    live = l < items * blocks;
+    const int items = a.starts ? groups.total : items_of(a.M, a.most), tiles = items * blocks;
+    const int l = place(n++, tiles, tiles < kUnits ? 1 : min(blocks, 8));
+    live = l < tiles;
     if (!live) return;
     int item, block;
     tile_at(l, items, blocks, item, block);
@@ -622,6 +634,13 @@ struct Rows {
   }
 };
 
+// Tiles of up to 256 rows by 64 NP columns: 8 waves, two rows of four.  256
+// rows an expert put the weights' bytes and the products in balance: bf16 32768
+// rows of 128 experts, N=1536 K=2048: 270 us, 3.8 TB/s of what it has to move and
+// 0.76 PFLOP/s (without loads 177 us; with loads of the L2 alone 198); its dx 285.
+// 16384 rows of 8 skewed experts, 4096 x 4096: 468 us, 1.17 PFLOP/s.  Rows that are
+// no whole cache lines (K=1440) make twice the requests to the L2: 30000 rows
+// of 64 experts, N=4096: 431 us, 0.82 PFLOP/s.
 template <class T, bool WCOLS, int OUT, int NP>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void row_product_kernel(RowProductArgs a) {
   __shared__ __align__(16) unsigned char smem[kLds];
@@ -654,7 +673,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
 // weights' bytes, or by latency.  A workgroup takes 16 columns of an item of up
 // to 64 rows; its 4 waves split the products' index, load what the matrix
 // instruction takes straight to registers, many loads at once, and add up
-// through LDS.
+// through LDS (in the order of the waves).  bf16, one token's 8 of 128 experts
+// 1536 x 2048, 50 MB: 11.6 us, 4.3 TB/s; int8 450 rows of 128 experts 1024 x 2048,
+// 268 MB: 60 us, 4.5 TB/s (a copy: 4.9); int8 one row 4096 x 2048: 3.8 us.
 constexpr int kFewThreads = 256, kFewRows = 64, kFewCols = 16;
 
 template <class T, int OUT, int MT>
@@ -741,6 +762,13 @@ __global__ __launch_bounds__(kFewThreads) __attribute__((amdgpu_waves_per_eu(4))
 }
 
 // ------------------------------------------------------------ weight gradient
+// Both operands lie across the sum.  Tiles of 256 x 256 of dw, stored once: no
+// sum is split, so none is added up in memory.  Experts of 256 rows are bound
+// by the stores, which no product of the same tile overlaps: 32768 rows of 128
+// experts, 1536 x 2048, 805 MB of dw: 389 us (the stores alone 131, loads and
+// products without them 264; two workgroups of 4 waves a compute unit, so that
+// one stores while the other multiplies, took 454).  16384 rows of 8 experts 4096 x 4096:
+// 500 us, 1.1 PFLOP/s.
 template <class T, int OUT>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void weight_grad_kernel(WeightGradArgs a) {
   __shared__ __align__(16) unsigned char smem[kLds];
@@ -807,18 +835,22 @@ unsigned grid_of(int64_t tiles) {
   return (unsigned)(all < kUnits ? all : kUnits);
 }
 
-// Up to this many bytes * rows (rows * columns * row length of the weights in
-// bytes) the few-rows kernel: it reads the weights at the rate of a copy, and the rows again for every 16
-// columns.  us, few / tiles: int8 one weight 4096 x 4096 16 rows 6.7 / 16, 64 rows (1.1e9) 14 / 17, 128 rows (2.1e9) 22 / 21;
-// 8192 x 8192 16 rows (1.1e9) 20 / 28, 32 rows (2.1e9) 28 / 28; bf16 128 experts 1536 x 2048, 128 rows (0.8e9) 109 / 118, 512
-// rows (3.2e9) 178 / 181, 1024 rows 203 / 184; 8 experts 4096 x 4096, 64 rows (2.1e9) 67 / 68, 256 rows 118 / 70.
+// Up to this much work (rows * columns * bytes of a weight row) the few-rows
+// kernel runs: it reads the weights at the rate of a copy, but the rows again
+// for every 16 columns.  us, few / tiles: int8, one weight 4096 x 4096: 16 rows
+// 6.7 / 16, 64 rows (1.1e9) 14 / 17, 128 rows (2.1e9) 22 / 21; 8192 x 8192: 16 rows
+// (1.1e9) 20 / 28, 32 rows (2.1e9) 28 / 28; bf16, 128 experts 1536 x 2048: 128 rows
+// (0.8e9) 109 / 118, 512 rows (3.2e9) 178 / 181, 1024 rows 203 / 184; 8 experts 4096 x
+// 4096: 64 rows (2.1e9) 67 / 68, 256 rows 118 / 70.
 constexpr int64_t kFewWork = 3 << 29;
 
-// Rows and columns of a tile: 256 x 256 (least LDS and L2 traffic for a
-// product) unless that leaves compute units without one; then the shape with most tiles that
-// still has one for each.  Narrow and low tiles keep more steps in LDS, which
-// hides more of the memory's latency.  us, 256 x 256 / 256 x 128 / 128 x 128 / 256 x 64 / 128 x 64, int8 4096 x 4096: 256 rows 49 / 28 /
-// 22 / 25 / 21 (128 tiles), 1024 rows 51 / 31 / 25 / 29 / 41 (256 tiles at 128 x 128), 2048 rows 55 / 40 / 50 / 59 / 78.
+// Rows and columns of a tile: 256 x 256, which moves least through the L2 and
+// LDS for a product, unless that leaves compute units without a tile; then the
+// shape with most tiles that still has a unit for each.  Narrow and low tiles
+// keep more steps in LDS, which hides more of the memory's latency.  us at 256 x
+// 256 / 256 x 128 / 128 x 128 / 256 x 64 / 128 x 64, int8 4096 x 4096: 256 rows 49 / 28 / 22 / 25 /
+// 21 (the last has 128 tiles), 1024 rows 51 / 31 / 25 / 29 / 41 (128 x 128 has 256), 2048 rows
+// 55 / 40 / 50 / 59 / 78 (256 x 128 has 256).
 struct Shape {
   int rows, np;
 };

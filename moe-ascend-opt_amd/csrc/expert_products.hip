@@ -92,8 +92,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, int64
 // permuted by the row, so that rows read at one place lie in different
 // banks).  COLS true: the products' index across rows of 16-bit values ([64
 // rows][2 DIM B], the 32-byte chunks of a row permuted by the row, so that
-// the 8 rows of half a transposed read do).  NSUB: subtiles of a wave.
-template <bool COLS, int DIM, int NSUB>
+// the 8 rows of half a transposed read do).  NSUB: subtiles of a wave.  WRAP:
+// the sum may begin anywhere in the row and wrap around.
+template <bool COLS, int DIM, int NSUB, bool WRAP = false>
 struct Operand {
   static constexpr int kIssues = (DIM + 63) / 64;   // loads of a wave a step
   static constexpr int kBytes = kIssues * 8192;
@@ -105,12 +106,14 @@ struct Operand {
   int left;            // steps (COLS: rows) from there to the end
   uint32_t ld;
   int ragged;          // the last step's 16-byte pieces (0: all eight); !COLS
+  int wrap, steps;     // steps to the row's end, and of a row; WRAP
   // reads
   uint32_t at[kReads];
 
   // What to load: b: the tile's first element; n: its rows (COLS: columns);
-  // len: length of the products' index in bytes of a row (COLS: in rows).
-  __device__ __forceinline__ void source(const unsigned char* b, int n, uint32_t ld_, int len) {
+  // len: length of the products' index in bytes of a row (COLS: in rows); from:
+  // the step to begin with (WRAP, rows of whole steps; else 0).
+  __device__ __forceinline__ void source(const unsigned char* b, int n, uint32_t ld_, int len, int from = 0) {
     base = b;
     ld = ld_;
     const int t = (threadIdx.x & ~63) | lane_here();
@@ -131,6 +134,11 @@ struct Operand {
       }
       left = (len + kStepBytes - 1) / kStepBytes;
       ragged = (len % kStepBytes) >> 4;
+      if constexpr (WRAP) {
+        steps = left;
+        wrap = steps - from;
+        base += (int64_t)from * kStepBytes;
+      }
     }
     limit();
   }
@@ -165,6 +173,7 @@ struct Operand {
   __device__ __forceinline__ void advance() {
     base += COLS ? (uint64_t)kStepRows * ld : (uint64_t)kStepBytes;
     left -= COLS ? kStepRows : 1;
+    if constexpr (WRAP) base -= --wrap == 0 ? (uint64_t)steps * kStepBytes : 0;
     limit();
   }
   // Loads of a step to LDS at `dst`, this wave's first kilobyte of it.
@@ -546,7 +555,18 @@ __device__ __forceinline__ void store_tile(__amdgpu_buffer_rsrc_t y, uint32_t ld
 template <class T, bool WCOLS, int OUT, int NP>
 struct Rows {
   static constexpr int kElem = std::is_same<T, I8>::value ? 1 : 2, kCols = 64 * NP;
-  typedef Operand<WCOLS, kCols, NP> OpW;
+  // Items of few rows read the weights at the rate of the memory.  Where rows
+  // are a power of two long, all workgroups at one place of theirs would put
+  // their reads on few of its channels, so neighbours begin at different steps
+  // (bf16, 128 experts 1536 x 2048: 512 rows 184 us, 160 so; 4096 rows 199, 169).
+  // Tiles bound by their products lose 2% by the longer loop, and narrow ones
+  // of one weight (int8 alone has these) 5 to 15%.
+  template <bool SMALL>
+  static constexpr bool kWrap = SMALL && !WCOLS && (NP == 4 || (NP == 2 && kElem == 2));
+  template <bool SMALL>
+  using OpW = Operand<WCOLS, kCols, NP, kWrap<SMALL>>;
+  template <bool SMALL>
+  using OpX = Operand<false, SMALL ? 64 : 128, 0, kWrap<SMALL>>;   // half of the rows
   const RowProductArgs& a;
   Groups groups;
   uint32_t lds;
@@ -569,17 +589,18 @@ struct Rows {
   // rows of half an item as its products take them
   static __device__ __forceinline__ int half(int rows) { return rows <= 64 ? 32 : rows <= 128 ? 64 : rows <= 192 ? 96 : 128; }
 
-  template <class R>
+  template <bool SMALL, class R>
   __device__ __forceinline__ void start(R& ring) const {
-    typedef decltype(ring.Q0) OpX;
+    constexpr int kW = OpW<SMALL>::kBytes, kX = OpX<SMALL>::kBytes;
     const unsigned char *w = a.w + (int64_t)it.e * a.w_expert, *x = a.x + (int64_t)it.row0 * a.ldx;
     const int len = a.K * kElem, h = half(it.rows);
-    ring.P.source(w + (int64_t)p0 * (WCOLS ? kElem : a.ldw), min(kCols, a.P - p0), a.ldw, WCOLS ? a.K : len);
-    ring.Q0.source(x, min(it.rows, h), a.ldx, len);
-    ring.Q1.source(x + (int64_t)h * a.ldx, it.rows - h, a.ldx, len);
+    const int from = kWrap<SMALL> && a.starts && len % kStepBytes == 0 ? (int)(blockIdx.x >> 3) % (len / kStepBytes) : 0;
+    ring.P.source(w + (int64_t)p0 * (WCOLS ? kElem : a.ldw), min(kCols, a.P - p0), a.ldw, WCOLS ? a.K : len, from);
+    ring.Q0.source(x, min(it.rows, h), a.ldx, len, from);
+    ring.Q1.source(x + (int64_t)h * a.ldx, it.rows - h, a.ldx, len, from);
     ring.P.reads(NP * wp, lds);
-    ring.Q0.reads(h / 32 * wq, lds + OpW::kBytes);
-    ring.Q1.reads(h / 32 * wq, lds + OpW::kBytes + OpX::kBytes);
+    ring.Q0.reads(h / 32 * wq, lds + kW);
+    ring.Q1.reads(h / 32 * wq, lds + kW + kX);
     ring.start();
   }
 
@@ -609,7 +630,7 @@ struct Rows {
     next();
     const bool same = live && it.e >= 0 && it.rows > 0 && (it.rows <= 128) == SMALL;
     if (same) {
-      start(ring);
+      start<SMALL>(ring);
       ring.fence();
     }
     store_tile<OUT, NP, NQ>(out_buffer<OUT>(a.y, (int64_t)done.row0 * a.ldy + d0), (uint32_t)(a.ldy * kOutBytes<OUT>), done.rows, cols,
@@ -623,9 +644,9 @@ struct Rows {
   template <bool SMALL>
   __device__ __forceinline__ void tiles() {
     // stores of the smaller kind of tile
-    Ring<OpW, Operand<false, SMALL ? 64 : 128, 0>, (SMALL ? 2 : 6) * (OUT == 2 || NP == 1 ? NP : NP / 2)> ring;
+    Ring<OpW<SMALL>, OpX<SMALL>, (SMALL ? 2 : 6) * (OUT == 2 || NP == 1 ? NP : NP / 2)> ring;
     ring.mine = lds + uni(threadIdx.x >> 6) * 1024;
-    start(ring);
+    start<SMALL>(ring);
     for (bool warm = false, same = true; same; warm = true) {
       if (SMALL) same = it.rows <= 64 ? tile<SMALL, 2>(ring, warm) : tile<SMALL, 4>(ring, warm);
       else same = it.rows <= 192 ? tile<SMALL, 6>(ring, warm) : tile<SMALL, 8>(ring, warm);

@@ -110,6 +110,51 @@ def test_grouped_any_starts(cuda, starts):
     _check_all(cuda, x, w, dy, torch.tensor(starts, dtype=torch.int32))
 
 
+def test_grouped_beyond_32_bits(cuda):
+    """Weights, rows, outputs and gradients of more than 4 GiB, checked at their ends."""
+    ops, dt = torch.ops.nanovllm, torch.bfloat16
+    g = torch.Generator(device="cuda").manual_seed(1)
+    E, N, K = 36, 8192, 8192   # 4.8 GB of weights
+    w = torch.empty(E, N, K, dtype=dt, device=cuda)
+    for e in (0, E - 1):
+        w[e] = torch.randn(N, K, generator=g, device=cuda) * 0.02
+    s = _starts([70] + [0] * (E - 2) + [90])
+    x, dy = (torch.randn(160, n, generator=g, device=cuda).to(dt) for n in (K, N))
+    y, dx = ops.moe_grouped_matmul(x, w, s.to(cuda)), ops.moe_grouped_matmul_dx(dy, w, s.to(cuda))
+    dw = ops.moe_grouped_matmul_dw(dy, x, s.to(cuda))
+    for e, r in ((0, slice(0, 70)), (E - 1, slice(70, 160))):
+        st = [0, r.stop - r.start]
+        assert ref.within(y[r], *ref.grouped(x[r], w[e:e + 1], st, dt)) <= 1.0
+        assert ref.within(dx[r], *ref.grouped_dx(dy[r], w[e:e + 1], st, dt)) <= 1.0
+        assert ref.within(dw[e:e + 1], *ref.grouped_dw(dy[r], x[r], st, 1, dt)) <= 1.0
+    assert not bool(dw[1:E - 1].any())
+    del w, dw, x, dy, y, dx
+    M, N, K = 300000, 8192, 64   # 4.9 GB of outputs, then of rows
+    x, w = torch.randn(M, K, generator=g, device=cuda).to(dt), torch.randn(2, N, K, generator=g, device=cuda).to(dt)
+    s = torch.tensor([0, 100000, M - 3], dtype=torch.int32, device=cuda)
+    y = ops.moe_grouped_matmul(x, w, s)
+    assert ref.within(y[M - 500:M - 3], *ref.grouped(x[M - 500:M - 3], w[1:], [0, 497], dt)) <= 1.0
+    assert ref.within(y[99990:100000], *ref.grouped(x[99990:100000], w[:1], [0, 10], dt)) <= 1.0
+    assert not bool(y[M - 3:].any())
+    dx = ops.moe_grouped_matmul_dx(y, w, s)
+    assert ref.within(dx[M - 500:], *ref.grouped_dx(y[M - 500:], w[1:], [0, 497], dt)) <= 1.0
+
+
+def test_grouped_one_gradient(cuda):
+    """Only x, or only w, with a gradient; outputs of a sum (a gradient with stride 0)."""
+    x, w, _ = _data(3, 40, 48, 30, torch.bfloat16, seed=4)
+    s = _starts([10, 0, 18])
+    one = torch.ones(30, 40, dtype=torch.bfloat16)
+    for leaf in ("x", "w"):
+        a, b = x.to(cuda), w.to(cuda)
+        (a if leaf == "x" else b).requires_grad_()
+        torch.ops.nanovllm.moe_grouped_matmul(a, b, s.to(cuda)).sum().backward()
+        if leaf == "x":
+            assert b.grad is None and ref.within(a.grad, *ref.grouped_dx(one, w, s.tolist(), torch.bfloat16)) <= 1.0
+        else:
+            assert a.grad is None and ref.within(b.grad, *ref.grouped_dw(one, x, s.tolist(), 3, torch.bfloat16)) <= 1.0
+
+
 def test_grouped_layouts(cuda):
     """Views: rows of a wider tensor, a slice of the weights' rows, weights stored across, one weight for all experts."""
     E, N, K, counts = 4, 48, 64, [3, 40, 0, 20]
@@ -280,6 +325,13 @@ def test_int8_extremes(cuda):
     xs = torch.tensor([1.0, float("nan"), 2.0])
     y = f(x.to(cuda), xs.to(cuda), w.to(cuda), one.to(cuda), None, torch.float32).cpu()
     assert bool(y[1].isnan().all()) and bool(torch.isfinite(y[[0, 2]]).all())
+    x, w = torch.full((200, K), -128, dtype=torch.int8, device=cuda), torch.full((300, K), -128, dtype=torch.int8, device=cuda)
+    x[::3], w[::2] = 127, 126   # the same sums through tiles
+    s = torch.ones(300, device=cuda)
+    y = f(x, s[:200], w, s, None, torch.float32)
+    assert ref.within(y, *ref.int8_rows(x, s[:200], w, s, None, torch.float32)) <= 1.0
+    y = f(x[:1].expand(5, K), s[:5], w, s, None, torch.float32)   # one row for all
+    assert ref.within(y, *ref.int8_rows(x[:1].expand(5, K), s[:5], w, s, None, torch.float32)) <= 1.0
     with pytest.raises(RuntimeError, match="int32"):
         big = torch.zeros(1, 131057, dtype=torch.int8, device=cuda)
         f(big, one[:1].to(cuda), big, one[:1].to(cuda), None, torch.float32)
@@ -368,6 +420,24 @@ def test_quantize(cuda, dt, rows, cols):
     x = torch.randn(rows, cols, generator=g) * torch.exp(torch.randn(cols, generator=g))
     _say("[int8 quantize]", rows, cols, dt)
     _same_codes(cuda, x.to(dt).to(cuda))
+
+
+def test_quantize_many_rows(cuda):
+    """More rows than one launch takes, and more than 2^32 values."""
+    ops = torch.ops.nanovllm
+    g = torch.Generator(device="cuda").manual_seed(2)
+    for rows, cols in (((1 << 23) + 5, 8), (2200000, 2048)):
+        x = torch.empty(rows, cols, dtype=torch.bfloat16, device=cuda)
+        pick = torch.tensor([0, 1, (1 << 21) - 1, 1 << 21, rows // 2, rows - 2, rows - 1], device=cuda)
+        if rows > 1 << 23:
+            pick = torch.cat([pick, torch.tensor([(1 << 23) - 1, 1 << 23, (1 << 23) + 1], device=cuda)])
+        x[pick] = torch.randn(len(pick), cols, generator=g, device=cuda).to(torch.bfloat16)
+        q, s = ops.int8_quantize(x)
+        rq, rs = ref.quantize(x[pick].cpu())
+        assert torch.equal(q[pick].cpu(), rq) and torch.equal(s[pick].cpu(), rs)
+        v = ops.int8_dequantize(q, s, torch.float32)[pick].cpu()
+        assert torch.equal(v, rq.float() * rs.unsqueeze(1))
+        del x, q, s, v
 
 
 def test_quantize_borders(cuda):

@@ -4,8 +4,9 @@
 //
 //   y[r] = W[e] x[r]      dx[r] = W[e]^T dy[r]      dW[e] = sum_r dy[r] x[r]^T
 //
-// Sums run in fp32 (int32 for int8, exact) in an order that the sizes alone
-// decide, and each output is rounded once.  Operands are read as they lie in
+// Sums run in fp32 (int32 for int8, exact) in an order that follows from the
+// sizes, the expert and the output's column: a row's results are the same bits
+// wherever it lies and however many rows the experts have.  Operands are read as they lie in
 // memory: rows along the sum as the matrix instruction takes them, rows across
 // it through transposed LDS reads, so no product needs a transposed copy.
 //
@@ -552,21 +553,14 @@ __device__ __forceinline__ void store_tile(__amdgpu_buffer_rsrc_t y, uint32_t ld
 // ------------------------------------------------------------ rows
 // Items of up to 64 and 128 rows (SMALL) keep three steps in LDS, those of up
 // to 192 and 256 rows two.
-template <class T, bool WCOLS, int OUT, int NP>
+// WRAP: sums begin at a step of the row that the expert and the block of columns
+// decide, see wrap_sums().
+template <class T, bool WCOLS, int OUT, int NP, bool WRAP>
 struct Rows {
   static constexpr int kElem = std::is_same<T, I8>::value ? 1 : 2, kCols = 64 * NP;
-  // Items of few rows read the weights at the rate of the memory.  Where rows
-  // are a power of two long, all workgroups at one place of theirs would put
-  // their reads on few of its channels, so neighbours begin at different steps
-  // (bf16, 128 experts 1536 x 2048: 512 rows 184 us, 160 so; 4096 rows 199, 169).
-  // Tiles bound by their products lose 2% by the longer loop, and narrow ones
-  // of one weight (int8 alone has these) 5 to 15%.
+  using OpW = Operand<WCOLS, kCols, NP, WRAP>;
   template <bool SMALL>
-  static constexpr bool kWrap = SMALL && !WCOLS && (NP == 4 || (NP == 2 && kElem == 2));
-  template <bool SMALL>
-  using OpW = Operand<WCOLS, kCols, NP, kWrap<SMALL>>;
-  template <bool SMALL>
-  using OpX = Operand<false, SMALL ? 64 : 128, 0, kWrap<SMALL>>;   // half of the rows
+  using OpX = Operand<false, SMALL ? 64 : 128, 0, WRAP>;   // half of the rows
   const RowProductArgs& a;
   Groups groups;
   uint32_t lds;
@@ -591,10 +585,10 @@ struct Rows {
 
   template <bool SMALL, class R>
   __device__ __forceinline__ void start(R& ring) const {
-    constexpr int kW = OpW<SMALL>::kBytes, kX = OpX<SMALL>::kBytes;
+    constexpr int kW = OpW::kBytes, kX = OpX<SMALL>::kBytes;
     const unsigned char *w = a.w + (int64_t)it.e * a.w_expert, *x = a.x + (int64_t)it.row0 * a.ldx;
     const int len = a.K * kElem, h = half(it.rows);
-    const int from = kWrap<SMALL> && a.starts && len % kStepBytes == 0 ? (int)(blockIdx.x >> 3) % (len / kStepBytes) : 0;
+    const int from = WRAP ? (it.e * blocks + p0 / kCols) % (len / kStepBytes) : 0;
     ring.P.source(w + (int64_t)p0 * (WCOLS ? kElem : a.ldw), min(kCols, a.P - p0), a.ldw, WCOLS ? a.K : len, from);
     ring.Q0.source(x, min(it.rows, h), a.ldx, len, from);
     ring.Q1.source(x + (int64_t)h * a.ldx, it.rows - h, a.ldx, len, from);
@@ -644,7 +638,7 @@ struct Rows {
   template <bool SMALL>
   __device__ __forceinline__ void tiles() {
     // stores of the smaller kind of tile
-    Ring<OpW<SMALL>, OpX<SMALL>, (SMALL ? 2 : 6) * (OUT == 2 || NP == 1 ? NP : NP / 2)> ring;
+    Ring<OpW, OpX<SMALL>, (SMALL ? 2 : 6) * (OUT == 2 || NP == 1 ? NP : NP / 2)> ring;
     ring.mine = lds + uni(threadIdx.x >> 6) * 1024;
     start<SMALL>(ring);
     for (bool warm = false, same = true; same; warm = true) {
@@ -662,12 +656,12 @@ struct Rows {
 // 16384 rows of 8 skewed experts, 4096 x 4096: 468 us, 1.17 PFLOP/s.  Rows that are
 // no whole cache lines (K=1440) make twice the requests to the L2: 30000 rows
 // of 64 experts, N=4096: 431 us, 0.82 PFLOP/s.
-template <class T, bool WCOLS, int OUT, int NP>
+template <class T, bool WCOLS, int OUT, int NP, bool WRAP>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void row_product_kernel(RowProductArgs a) {
   __shared__ __align__(16) unsigned char smem[kLds];
   __shared__ int table[Groups::kTable];
   const int wave = uni(threadIdx.x >> 6);
-  Rows<T, WCOLS, OUT, NP> rows{a};
+  Rows<T, WCOLS, OUT, NP, WRAP> rows{a};
   rows.lds = (uint32_t)(uintptr_t)(lds_byte*)smem;
   rows.wp = wave & 3;
   rows.wq = wave >> 2;
@@ -899,10 +893,31 @@ void few_rows(const RowProductArgs& a, hipStream_t st) {
   few_rows_kernel<T, OUT><<<(unsigned)(tiles < 4 * kUnits ? tiles : 4 * kUnits), kFewThreads, 0, st>>>(a);
 }
 
+// Experts of few rows read the weights at the rate of the memory.  Where rows
+// are a power of two long, all workgroups at one place of theirs would put
+// their reads on few of its channels, so tiles begin their sums at different
+// steps.  Which one follows from the expert and the block of columns, and
+// whether from the sizes, for tiles of any number of rows, so that no sum's
+// order depends on starts.  bf16, us without / so: 128 experts 1536 x 2048, 512
+// rows 189 / 162, 4096 rows 200 / 171, 24576 rows 270 / 238; 8 experts 4096 x 4096,
+// 256 rows 70 / 59; skewed 160 to 224 rows an expert 1 to 3% slower, and so
+// from 256 rows an expert on.  int8, half as many steps: within 1.5% either way, not
+// done; nor in tiles of 64 columns, taken where compute units are left over.
+template <int NP, bool WCOLS, class T>
+constexpr bool kMayWrap = !WCOLS && !std::is_same<T, I8>::value && NP >= 2;
+bool wrap_sums(const RowProductArgs& a) { return a.starts && a.M < (int64_t)kTile * a.E && a.K * 2 % kStepBytes == 0; }
+
 template <class T, bool WCOLS, int OUT, int NP>
 void tiles(const RowProductArgs& a, hipStream_t st) {
   const int64_t items = a.starts ? items_max(a.M, a.E, a.most) : (a.M + a.most - 1) / a.most;
-  row_product_kernel<T, WCOLS, OUT, NP><<<grid_of(items * ((a.P + 64 * NP - 1) / (64 * NP))), kThreads, 0, st>>>(a);
+  const unsigned grid = grid_of(items * ((a.P + 64 * NP - 1) / (64 * NP)));
+  if constexpr (kMayWrap<NP, WCOLS, T>) {
+    if (wrap_sums(a)) {
+      row_product_kernel<T, WCOLS, OUT, NP, true><<<grid, kThreads, 0, st>>>(a);
+      return;
+    }
+  }
+  row_product_kernel<T, WCOLS, OUT, NP, false><<<grid, kThreads, 0, st>>>(a);
 }
 
 template <class T, bool WCOLS, int OUT>

@@ -212,3 +212,36 @@ def test_tiled_on_two_streams(cuda):
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+# M, E, N, K: the few-rows kernel, sums that begin inside the row in tiles of 256 and of 128 columns, others
+ORDER = [(700, 16, 520, 776), (4096, 128, 1536, 512), (1040, 16, 1544, 1280), (4100, 8, 2056, 1032)]
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("M,E,N,K", ORDER)
+def test_results_follow_from_the_row_alone(cuda, dt, M, E, N, K):
+    """At equal sizes a row's outputs do not depend, bit for bit, on how many rows its expert or others have, nor on where
+    it lies; an expert's weight gradient does not depend on the others."""
+    ops, e, most = torch.ops.nanovllm, E - 3, 300
+    own, owndy, w, x, dy = _rand(cuda, DT[dt], M + E, (most, K), (most, N), (E, N, K), (M, K), (M, N))
+    own[1], owndy[1] = own[0], owndy[0]   # two equal rows
+    first = None
+    for n, others in ((most, "even"), (most, "first"), (32, "even"), (128, "last"), (129, "even"), (20, "first"), (1, "none")):
+        rest, c = M - n, [0] * E
+        if others == "even":
+            c = [rest // (E - 1)] * E
+        elif others != "none":
+            c[0 if others == "first" else E - 1] = rest
+        c[e] = n
+        s = _starts(c)
+        a = int(s[e])
+        x[a:a + n], dy[a:a + n] = own[:n], owndy[:n]
+        s = s.to(cuda)
+        y, dx = ops.moe_grouped_matmul(x, w, s)[a:a + n], ops.moe_grouped_matmul_dx(dy, w, s)[a:a + n]
+        if first is None:
+            first = y.clone(), dx.clone(), ops.moe_grouped_matmul_dw(dy, x, s)[e].clone()
+            assert torch.equal(y[0], y[1]) and torch.equal(dx[0], dx[1])
+        assert torch.equal(y, first[0][:n]) and torch.equal(dx, first[1][:n]), (n, others)
+        if n == most:
+            assert torch.equal(ops.moe_grouped_matmul_dw(dy, x, s)[e], first[2]), (n, others)

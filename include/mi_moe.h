@@ -338,8 +338,9 @@ int mi_moe_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t ro
  * 16 bits, 16 of int8).  M <= 2^26, N and K <= 2^20, E <= 512.  Sums are in
  * fp32 (int32 for int8), in an order that follows from the sizes, the expert and
  * the output's column: not from where a row lies, nor from how many rows the
- * experts have.  They are rounded once.  Each call is one launch, stream-ordered, without a workspace; it can be
- * captured into a graph.  Calls may overlap. */
+ * experts have.  16-bit sums are rounded once; int8 ones as said below.  Each
+ * call is one launch, stream-ordered, without a workspace; it can be captured
+ * into a graph.  Calls may overlap. */
 
 /* y[r] = W[e] x[r]: x [M,K], w [E,N,K] fp16 or bf16 -> y [M,N], contiguous, of
  * the same type. */
@@ -363,7 +364,11 @@ int mi_moe_grouped_matmul_dw(const void* dy, int64_t dy_stride, const void* x,
 
 /* y[r][n] = sum_k x[r][k] w[e][n][k] * w_scales[e][n] * x_scales[r]: x [M,K],
  * w [E,N,K] int8, x_scales [M], w_scales [E,N] fp32 -> y [M,N] fp16, bf16 or
- * fp32 (out_dtype), contiguous.  The sum is exact (K <= 131056). */
+ * fp32 (out_dtype), contiguous.  The sum is exact (K <= 131056).  fp32 outputs
+ * are computed from it and the scales in 64 bits and rounded once; for 16-bit
+ * outputs the sum, each product and the bias round to fp32 (2^-24), then to the
+ * output's type; no factor takes a product out of fp32's range that belongs
+ * in it. */
 int mi_moe_grouped_matmul_int8(const int8_t* x, int64_t x_stride, const float* x_scales,
                                const int8_t* w, int64_t w_expert_stride, int64_t w_stride,
                                const float* w_scales, const int32_t* starts, int64_t M,
@@ -371,7 +376,7 @@ int mi_moe_grouped_matmul_int8(const int8_t* x, int64_t x_stride, const float* x
                                void* stream);
 
 /* The same with one weight for all rows: w [N,K], w_scales [N], and bias [N]
- * fp32 (or null) added in fp32 before the one rounding. */
+ * fp32 (or null) added before the last rounding. */
 int mi_moe_int8_matmul(const int8_t* x, int64_t x_stride, const float* x_scales,
                        const int8_t* w, int64_t w_stride, const float* w_scales,
                        const float* bias, int64_t M, int64_t N, int64_t K, int out_dtype,

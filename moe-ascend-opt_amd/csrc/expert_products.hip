@@ -6,9 +6,10 @@
 //
 // Sums run in fp32 (int32 for int8, exact) in an order that follows from the
 // sizes, the expert and the output's column: a row's results are the same bits
-// wherever it lies and however many rows the experts have.  Operands are read as they lie in
-// memory: rows along the sum as the matrix instruction takes them, rows across
-// it through transposed LDS reads, so no product needs a transposed copy.
+// wherever it lies and however many rows the experts have.  Operands are read
+// as they lie in memory: rows along the sum as the matrix instruction takes
+// them, rows across it through transposed LDS reads, so no product needs a
+// transposed copy.
 //
 // Which kernel: few_rows_kernel for calls of little work, else tiles of 256 x
 // 256 outputs down to 128 x 64 (kFewWork, tile_shape).  Measured: bf16 8192 x
@@ -510,6 +511,22 @@ __device__ __forceinline__ void zero_rows(__amdgpu_buffer_rsrc_t y, uint32_t ld,
   }
 }
 
+// An int8 product's output, sum * ws * xs + bias.  fp32 outputs: in 64 bits (the
+// scales' product is exact), rounded once; in fp32 throughout each operation
+// would round, 1.4 times the error (mean, sums of 2048 products), and the time is
+// the same (8192 x 8192 x 4096 260 us): the stores take longer.  16-bit outputs: in fp32, four
+// roundings of 2^-24 beside the last one of 2^-11 or 2^-8; 64 bits would cost a
+// tile of 256 x 256 its registers (8192 x 8192 x 4096 bf16 227 us, 260 so).  A sum
+// times a scale beyond kWide may leave the range of fp32 where the output does
+// not: then the other scale comes first (a product by a tiny scale is exact).
+constexpr float kWide = 0x1p96f;
+template <int OUT>
+__device__ __forceinline__ float scaled(int32_t sum, float ws, float xs, float bias, bool wide) {
+  if constexpr (OUT == 2) return (float)__builtin_fma((double)sum, (double)ws * (double)xs, (double)bias);
+  const bool swap = wide && __builtin_fabsf(ws) > kWide;
+  return (float)sum * (swap ? xs : ws) * (swap ? ws : xs) + bias;
+}
+
 // The values of a wave's subtiles as they leave a tile's products: lane (r, q)
 // has columns 4 q .. 4 q + 3 of subtile i in row r of subtile j.  16-bit
 // values change places between lane rows 2 k and 2 k + 1, so that a lane
@@ -627,12 +644,25 @@ struct Rows {
       start<SMALL>(ring);
       ring.fence();
     }
-    store_tile<OUT, NP, NQ>(out_buffer<OUT>(a.y, (int64_t)done.row0 * a.ldy + d0), (uint32_t)(a.ldy * kOutBytes<OUT>), done.rows, cols,
-                            out_vec<OUT>(a.y, a.ldy), wp, wq, [&](int i, int j, int k) {
-                              const float v = (float)acc[i][j][k];
-                              if constexpr (kElem == 1) return v * ws[i][k] * xs[j] + bias[i][k];
-                              return v;
-                            });
+    auto store = [&](auto wide) {
+      store_tile<OUT, NP, NQ>(out_buffer<OUT>(a.y, (int64_t)done.row0 * a.ldy + d0), (uint32_t)(a.ldy * kOutBytes<OUT>), done.rows, cols,
+                              out_vec<OUT>(a.y, a.ldy), wp, wq, [&](int i, int j, int k) {
+                                if constexpr (kElem == 1)
+                                  return scaled<OUT>(acc[i][j][k], ws[i][k], xs[j], bias[i][k], decltype(wide)::value);
+                                else return acc[i][j][k];
+                              });
+    };
+    if constexpr (kElem == 1 && OUT != 2) {
+      bool wide = false;
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) wide |= !(__builtin_fabsf(ws[i][k]) <= kWide);
+      if (__builtin_amdgcn_ballot_w64(wide)) store(std::true_type{});
+      else store(std::false_type{});
+    } else {
+      store(std::false_type{});
+    }
     return same;
   }
   template <bool SMALL>
@@ -737,8 +767,9 @@ __device__ __forceinline__ void few_item(const RowProductArgs& a, float* sums, c
     for (int k = 1; k < 4; ++k) v += part[(k * MT + m) * kWave + (n >> 2) * 16 + row][n & 3];
     const int mr = 16 * m + row, p = p0 + n;
     if (mr < it.rows && p < a.P) {
-      float f = (float)v;
-      if constexpr (kElem == 1) f = f * a.ws[(int64_t)it.e * a.P + p] * a.xs[it.row0 + mr] + (a.bias ? a.bias[p] : 0.0f);
+      float f;
+      if constexpr (kElem == 1) f = scaled<OUT>(v, a.ws[(int64_t)it.e * a.P + p], a.xs[it.row0 + mr], a.bias ? a.bias[p] : 0.0f, true);
+      else f = v;
       const int64_t at = (int64_t)(it.row0 + mr) * a.ldy + p;
       if constexpr (OUT == 2) reinterpret_cast<float*>(a.y)[at] = f;
       else reinterpret_cast<uint16_t*>(a.y)[at] = pack1<OUT>(f);

@@ -245,3 +245,48 @@ def test_results_follow_from_the_row_alone(cuda, dt, M, E, N, K):
         assert torch.equal(y, first[0][:n]) and torch.equal(dx, first[1][:n]), (n, others)
         if n == most:
             assert torch.equal(ops.moe_grouped_matmul_dw(dy, x, s)[e], first[2]), (n, others)
+
+
+def _int8_exact(x, xs, w, ws, bias):
+    """The sum, the scales' product and the bias in 64 bits (each operation off by at most 2^-53 of what it works on), rounded
+    to fp32: half a step."""
+    p = (x.double() @ w.double().t()) * (xs.double().unsqueeze(1) * ws.double())
+    b = torch.zeros_like(ws, dtype=torch.float64) if bias is None else bias.double()
+    return p + b, ref.round_bound(p + b, (p.abs() + b.abs()) * 2.0 ** -51, torch.float32)
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 300, 2048), (60, 1000, 4096), (200, 19001, 2048), (131, 20000, 1040), (1000, 2100, 1024),
+                                   (128, 16001, 1040), (333, 1001, 8208), (2000, 6001, 272)])
+def test_int8_fp32_outputs_rounded_once(cuda, M, N, K):
+    """The few-rows kernel and each tile shape: 32-bit outputs have no rounding before the last."""
+    x, xs, w, ws = _codes(cuda, N + K, (M, K), (N, K))
+    bias = torch.randn(N, generator=torch.Generator(device="cuda").manual_seed(N), device=cuda)
+    ops = torch.ops.nanovllm
+    for b in (bias, None):
+        assert ref.within(ops.int8_matmul(x, xs, w, ws, b, torch.float32), *_int8_exact(x, xs, w, ws, b)) <= 1.0
+    s = _starts([M])
+    y = ops.moe_grouped_matmul_int8(x, xs, w[None], ws[None], s.to(cuda), torch.float32)
+    assert ref.within(y, *_int8_exact(x, xs, w, ws, None)) <= 1.0
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 300, 2048), (200, 19001, 2048), (131, 20000, 1040), (1000, 2100, 1024), (333, 1001, 8208),
+                                   (2000, 6000, 272)])
+def test_int8_scales_of_any_size(cuda, M, N, K):
+    """A sum times one scale leaves the range of fp32, the output does not (every third channel alone, too); outputs below fp32's
+    normal values; no sum gives 0 whatever the scales; a NaN scale gives NaN."""
+    f = torch.ops.nanovllm.int8_matmul
+    x, xs, w, ws = _codes(cuda, K, (M, K), (N, K))
+    for a, b in ((1e-30, 1e38), (1e38, 1e-30), (1e-30, 1e-10), (1e-12, 1e-36), (1e-24, 1e-24)):
+        xa, wb = xs * a, ws * b
+        for third in (False, True):
+            if third:
+                wb = torch.where(torch.arange(N, device=cuda) % 3 == 0, wb, ws * 1e3)
+                if a > 1:   # outputs of the others would leave the range themselves
+                    wb[torch.arange(N, device=cuda) % 3 != 0] = b
+            assert ref.within(f(x, xa, w, wb, None, torch.float32), *_int8_exact(x, xa, w, wb, None)) <= 1.0, (a, b)
+            assert ref.within(f(x, xa, w, wb, None, torch.bfloat16), *ref.int8_rows(x, xa, w, wb, None, torch.bfloat16)) <= 1.0, (a, b)
+    zero = torch.zeros_like(x)
+    ws[1] = float("nan")
+    for out in OUT:
+        y = f(zero, xs * 1e35, w, ws * 1e35, None, out)
+        assert bool(y[:, 1].isnan().all()) and not bool(y[:, 2:].any()) and not bool(y[:, 0].any())

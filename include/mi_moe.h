@@ -391,8 +391,8 @@ int mi_moe_int8_matmul(const int8_t* x, int64_t x_stride, const float* x_scales,
 int mi_moe_int8_quantize(const void* x, int dtype, int64_t rows, int64_t cols,
                          int64_t row_stride, int8_t* codes, float* scales, void* stream);
 
-/* out = code * scale, the product in fp32 (fp16: the exact one), rounded to
- * dtype: out [rows,cols] fp16, bf16 or fp32. */
+/* out = code * scale, the product in fp32, rounded to dtype: out
+ * [rows,cols] fp16, bf16 or fp32. */
 int mi_moe_int8_dequantize(const int8_t* codes, const float* scales, int64_t rows,
                            int64_t cols, void* out, int dtype, void* stream);
 

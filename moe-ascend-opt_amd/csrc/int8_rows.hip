@@ -148,6 +148,16 @@ __global__ __launch_bounds__(256) void int8_quantize_kernel(const void* __restri
   }
 }
 
+// A code's value: the product in fp32, which the conversion that follows then
+// rounds.  The empty asm keeps the two apart: for fp16 the compiler would make
+// one instruction of them that rounds the exact product, other bits than those
+// of the same codes and scales elsewhere.
+__device__ __forceinline__ float value(int8_t code, float s) {
+  float v = (float)code * s;
+  asm("" : "+v"(v));
+  return v;
+}
+
 // A thread per piece of 8 codes of a row: 8191 x 4096 to fp16 in 16.8 us, 6.0 TB/s.
 template <int DT, bool ALIGNED>
 __global__ __launch_bounds__(256) void int8_dequantize_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scales,
@@ -163,10 +173,10 @@ __global__ __launch_bounds__(256) void int8_dequantize_kernel(const int8_t* __re
     if constexpr (ALIGNED) {
       const u32x2_t w = *reinterpret_cast<const u32x2_t*>(codes + at);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = (float)(int8_t)(w[k >> 2] >> (8 * (k & 3))) * s;
+      for (int k = 0; k < 8; ++k) v[k] = value((int8_t)(w[k >> 2] >> (8 * (k & 3))), s);
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = k < n ? (float)codes[at + k] * s : 0.0f;
+      for (int k = 0; k < 8; ++k) v[k] = k < n ? value(codes[at + k], s) : 0.0f;
     }
     if constexpr (DT == 2) {
       float* o = reinterpret_cast<float*>(out) + at;

@@ -290,3 +290,13 @@ def test_int8_scales_of_any_size(cuda, M, N, K):
     for out in OUT:
         y = f(zero, xs * 1e35, w, ws * 1e35, None, out)
         assert bool(y[:, 1].isnan().all()) and not bool(y[:, 2:].any()) and not bool(y[:, 0].any())
+
+
+@pytest.mark.parametrize("out", OUT)
+@pytest.mark.parametrize("cols", [2048, 2047])
+def test_dequantized_values_bit_for_bit(cuda, out, cols):
+    """code * scale in fp32, then rounded to the output's type, in every type: products of 31 bits that fp32 rounds to a tie of
+    16 bits are among them (one in some thousands)."""
+    q, s = _codes(cuda, cols, (4096, cols))
+    want = (q.float() * s.unsqueeze(1)).to(out)
+    assert torch.equal(torch.ops.nanovllm.int8_dequantize(q, s, out), want)

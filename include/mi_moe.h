@@ -335,12 +335,13 @@ int mi_moe_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t ro
  *   that belong to no expert are 0.  An expert may have no rows.
  * Strides count elements.  x, dy and w are read in 16-byte pieces: their
  * addresses, row lengths and strides are multiples of 16 bytes (8 elements of
- * 16 bits, 16 of int8).  M <= 2^26, N and K <= 2^20, E <= 512.  Sums are in
- * fp32 (int32 for int8), in an order that follows from the sizes, the expert and
- * the output's column: not from where a row lies, nor from how many rows the
- * experts have.  16-bit sums are rounded once; int8 ones as said below.  Each
- * call is one launch, stream-ordered, without a workspace; it can be captured
- * into a graph.  Calls may overlap. */
+ * 16 bits, 16 of int8).  M <= 2^26, N and K <= 2^20, E <= 512, and at most 2^22
+ * tiles of 256 x 256 values an operand or output.  Sums are in fp32 (int32 for
+ * int8), in an order that follows from the sizes, the expert and the output's
+ * column: not from where a row lies, nor from how many rows the experts have.
+ * 16-bit sums are rounded once; int8 ones as said below.  Each call is one
+ * launch, stream-ordered, without a workspace; it can be captured into a graph.
+ * Calls may overlap. */
 
 /* y[r] = W[e] x[r]: x [M,K], w [E,N,K] fp16 or bf16 -> y [M,N], contiguous, of
  * the same type. */

@@ -32,7 +32,8 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 // Offsets within a tile (256 rows, or 64 across) are 32 bits wide.
 constexpr int64_t kMaxDim = (int64_t)1 << 20, kMaxRows = (int64_t)1 << 26, kMaxStride = (int64_t)1 << 22;
-// A launch has at most 2^32 threads.
+// Tiles and their places in the XCDs' runs are numbered in 32 bits; 2^22 tiles are
+// 2^38 values of an operand or output.
 constexpr int64_t kMaxTiles = (int64_t)1 << 22;
 
 int check_sizes(int64_t M, int64_t N, int64_t K, int64_t E) {

@@ -36,7 +36,9 @@ constexpr int kStepRows = 64;
 constexpr int kLds = 163840 - 4096;   // of the operands; a compute unit's less the table of groups
 constexpr uint32_t kOutside = 0x80000000u;     // an offset beyond any buffer: loads give zero
 
-constexpr int kUnits = 256;            // compute units, 32 in each of 8 XCDs
+// Compute units, 32 in each of 8 XCDs.  Tile kernels launch a workgroup for each;
+// those without a tile end at once.
+constexpr int kUnits = 256;
 constexpr int kRun = 32;               // place()
 
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
@@ -568,8 +570,8 @@ __device__ __forceinline__ void store_tile(__amdgpu_buffer_rsrc_t y, uint32_t ld
 }
 
 // ------------------------------------------------------------ rows
-// Items of up to 64 and 128 rows (SMALL) keep three steps in LDS, those of up
-// to 192 and 256 rows two.
+// Items of up to 64 and 128 rows (SMALL) keep three steps of 256 columns in LDS
+// (128 columns: four, 64: six), those of up to 192 and 256 rows two (three, three).
 // WRAP: sums begin at a step of the row that the expert and the block of columns
 // decide, see wrap_sums().
 template <class T, bool WCOLS, int OUT, int NP, bool WRAP>
@@ -875,12 +877,6 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   ring.drain();   // no load to LDS outlives the workgroup
 }
 
-// A workgroup a compute unit, or as many as there are tiles.
-unsigned grid_of(int64_t tiles) {
-  const int64_t all = (tiles + 255) / 256 * 256;   // whole runs of every XCD
-  return (unsigned)(all < kUnits ? all : kUnits);
-}
-
 // Up to this much work (rows * columns * bytes of a weight row) the few-rows
 // kernel runs: it reads the weights at the rate of a copy, but the rows again
 // for every 16 columns.  us, few / tiles: int8, one weight 4096 x 4096: 16 rows
@@ -940,15 +936,13 @@ bool wrap_sums(const RowProductArgs& a) { return a.starts && a.M < (int64_t)kTil
 
 template <class T, bool WCOLS, int OUT, int NP>
 void tiles(const RowProductArgs& a, hipStream_t st) {
-  const int64_t items = a.starts ? items_max(a.M, a.E, a.most) : (a.M + a.most - 1) / a.most;
-  const unsigned grid = grid_of(items * ((a.P + 64 * NP - 1) / (64 * NP)));
   if constexpr (kMayWrap<NP, WCOLS, T>) {
     if (wrap_sums(a)) {
-      row_product_kernel<T, WCOLS, OUT, NP, true><<<grid, kThreads, 0, st>>>(a);
+      row_product_kernel<T, WCOLS, OUT, NP, true><<<kUnits, kThreads, 0, st>>>(a);
       return;
     }
   }
-  row_product_kernel<T, WCOLS, OUT, NP, false><<<grid, kThreads, 0, st>>>(a);
+  row_product_kernel<T, WCOLS, OUT, NP, false><<<kUnits, kThreads, 0, st>>>(a);
 }
 
 template <class T, bool WCOLS, int OUT>
@@ -982,10 +976,8 @@ hipError_t launch_row_product(const RowProductArgs& a, int dt, int w_cols, int o
 }
 
 hipError_t launch_weight_grad(const WeightGradArgs& a, int dt, hipStream_t st) {
-  const int64_t tiles = (int64_t)a.E * ((a.N + kTile - 1) / kTile) * ((a.K + kTile - 1) / kTile);
-  const unsigned grid = grid_of(tiles);
-  if (dt == 1) weight_grad_kernel<BF16, 1><<<grid, kThreads, 0, st>>>(a);
-  else weight_grad_kernel<F16, 0><<<grid, kThreads, 0, st>>>(a);
+  if (dt == 1) weight_grad_kernel<BF16, 1><<<kUnits, kThreads, 0, st>>>(a);
+  else weight_grad_kernel<F16, 0><<<kUnits, kThreads, 0, st>>>(a);
   return hipGetLastError();
 }
 

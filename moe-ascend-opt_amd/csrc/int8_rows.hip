@@ -54,8 +54,9 @@ __device__ __forceinline__ uint32_t amax8(const float (&v)[8], uint32_t m) {
 
 // The codes of eight values: v * (1 / s) is off by less than 127 * 2^-22, so
 // it names the nearest integer unless it lies within 2^-14 of a border; there
-// the quotient in 64 bits does (x and s have 24 bits: a quotient that is no
-// tie is at least 2^-26 of itself away from one, a tie is exact).
+// the quotient in 64 bits does (x and s have 24 bits: a quotient that is no tie
+// k + 1/2 is at least 2^-32 of itself away from one, since x - (k + 1/2) s is a
+// multiple of half a unit of s, and k + 1/2 < 2^7; a tie is exact).
 __device__ __forceinline__ u32x2_t codes8(const float (&v)[8], float s, float inv, bool bad) {
   float q[8];
   bool near = false;

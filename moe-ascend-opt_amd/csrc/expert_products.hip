@@ -516,11 +516,12 @@ __device__ __forceinline__ void zero_rows(__amdgpu_buffer_rsrc_t y, uint32_t ld,
 // An int8 product's output, sum * ws * xs + bias.  fp32 outputs: in 64 bits (the
 // scales' product is exact), rounded once; in fp32 throughout each operation
 // would round, 1.4 times the error (mean, sums of 2048 products), and the time is
-// the same (8192 x 8192 x 4096 260 us): the stores take longer.  16-bit outputs: in fp32, four
-// roundings of 2^-24 beside the last one of 2^-11 or 2^-8; 64 bits would cost a
-// tile of 256 x 256 its registers (8192 x 8192 x 4096 bf16 227 us, 260 so).  A sum
-// times a scale beyond kWide may leave the range of fp32 where the output does
-// not: then the other scale comes first (a product by a tiny scale is exact).
+// the same (8192 x 8192 x 4096 260 us): the stores take longer.  16-bit outputs:
+// in fp32, four roundings of 2^-24 beside the last one of 2^-11 or 2^-8; 64 bits
+// would cost a tile of 256 x 256 its registers (bf16 8192 x 8192 x 4096 227 us, 260
+// so).  A sum times a scale beyond kWide may leave the range of fp32 where the
+// output does not: then the other scale comes first (what it makes smaller than
+// fp32's normal values is an exact multiple of the scale).
 constexpr float kWide = 0x1p96f;
 template <int OUT>
 __device__ __forceinline__ float scaled(int32_t sum, float ws, float xs, float bias, bool wide) {
@@ -685,9 +686,9 @@ struct Rows {
 // rows an expert put the weights' bytes and the products in balance: bf16 32768
 // rows of 128 experts, N=1536 K=2048: 270 us, 3.8 TB/s of what it has to move and
 // 0.76 PFLOP/s (without loads 177 us; with loads of the L2 alone 198); its dx 285.
-// 16384 rows of 8 skewed experts, 4096 x 4096: 468 us, 1.17 PFLOP/s.  Rows that are
-// no whole cache lines (K=1440) make twice the requests to the L2: 30000 rows
-// of 64 experts, N=4096: 431 us, 0.82 PFLOP/s.
+// 16384 rows of 8 skewed experts, 4096 x 4096: 470 us, 1.17 PFLOP/s; dx 490.  Rows
+// that are no whole cache lines (K=1440) make 1.5 times the requests to the L2:
+// 30000 rows of 64 experts, N=4096: 431 us, 0.82 PFLOP/s.
 template <class T, bool WCOLS, int OUT, int NP, bool WRAP>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void row_product_kernel(RowProductArgs a) {
   __shared__ __align__(16) unsigned char smem[kLds];

@@ -22,7 +22,8 @@ gradients of x and w (``moe_grouped_matmul_dx`` / ``_dw`` alone), and
 ``moe_grouped_matmul_int8(x, x_scales, w, w_scales, starts, dtype)``.
 ``int8_matmul(x, x_scales, w, w_scales, bias, dtype)`` is the latter with one
 weight [N,K]; ``int8_quantize`` and ``int8_dequantize`` go between values and
-int8 codes with a scale for each row.
+int8 codes with a scale for each row.  Of these ``moe_grouped_matmul`` alone is
+differentiable (once).
 
 The op dispatches on the tensors' device, like the reference's registration
 (Int8-gemm/nanovllm_ops.cpp:410-412).  HIP tensors run the hand-written HIP
